@@ -735,6 +735,7 @@ int64_t status_read(bool clear) { return titb_status_read(clear, cur_stream()); 
 }  // namespace
 
 void bind_attention(pybind11::module_& m);
+void bind_cache(pybind11::module_& m);
 void bind_comm(pybind11::module_& m);
 void bind_core(pybind11::module_& m);
 void bind_symm(pybind11::module_& m);
@@ -812,6 +813,7 @@ PYBIND11_MODULE(_C, m) {
   m.def("status_read", &status_read, py::arg("clear") = true);
   m.def("gemm_set_tma_store", [](bool on) { titb_gemm_set_tma_store(on ? 1 : 0); });
   bind_attention(m);
+  bind_cache(m);
   bind_comm(m);
   bind_core(m);
   bind_symm(m);

@@ -283,6 +283,41 @@ struct TitbAttnDesc {
 TITB_API int titb_attn_fwd(const TitbAttnDesc* d, cudaStream_t stream);
 TITB_API int titb_attn_bwd(const TitbAttnDesc* d, cudaStream_t stream);
 
+// Causal attention over a window and sinks: query i sees key j when j <= i and (i - j < window or j < sinks).  window >= 1,
+// sinks >= 0.  dtype 0 (fp32) or 1 (bf16) for q .. dv; hd a multiple of 8 up to 128.  `attn.dq_accum` is not used.
+struct TitbWindowDesc {
+  TitbAttnDesc attn;
+  int window, sinks, dtype;
+};
+TITB_API int titb_window_attn_fwd(const TitbWindowDesc* d, cudaStream_t stream);
+TITB_API int titb_window_attn_bwd(const TitbWindowDesc* d, cudaStream_t stream);
+
+// ---- paged key-value cache ----------------------------------------------------------------------------
+// k_cache / v_cache: [n_pages, Hkv, page_size, hd], contiguous.  Position p of sequence b is row p % page_size of page
+// page_table[b * table_stride + p / page_size]; entries behind a sequence's last page are not read.  A page number outside
+// [0, n_pages) or a position outside [0, table_width * page_size) is never followed: nothing is written there, such a
+// position is not attended to, and the status word gets kStatusBadPage.
+struct TitbCacheDesc {
+  void* k_cache; void* v_cache;
+  const int* page_table;
+  long long table_stride;
+  int table_width, n_pages, page_size;
+  int B, Hq, Hkv, hd;
+  int window, sinks;   // window >= 1 (INT_MAX: every position), sinks >= 0
+  int dtype;           // 0 fp32, 1 bf16
+};
+// Token t < counts[b] (null: t < T) of sequence b has position starts[b] + t.  qkv: [B, T, (Hq + 2 Hkv) * hd] with the given
+// strides (elements, multiples of 16 bytes).  The keys and values that the token after the last one sees go into the cache.
+// theta > 0: queries and keys are rotated by their position first, pairing element i with i + hd / 2.  q_out [B, T, Hq, hd] and
+// k_out [B, T, Hkv, hd] (each may be null) receive the queries and keys of all T tokens.
+TITB_API int titb_cache_append(const TitbCacheDesc* d, const void* qkv, long long qkv_stride_b, long long qkv_stride_t, int T,
+                               const int* starts, const int* counts, double theta, void* q_out, void* k_out,
+                               cudaStream_t stream);
+// o[b] = attention of the query at position lengths[b] - 1 over positions p < lengths[b] with p >= lengths[b] - window or
+// p < sinks; zeros when there are none.  q: [B, Hq, hd] with q_stride_b elements between sequences; o: contiguous.
+TITB_API int titb_paged_attention(const TitbCacheDesc* d, const void* q, long long q_stride_b, const int* lengths, float scale,
+                                  void* o, cudaStream_t stream);
+
 // ---- gradient-norm clipping (device resident: graph-capturable) -------------------------------------------------
 // Stage 1: per-block partial sums of squares of a flat fp32 buffer (16-byte aligned).  `partials` must hold
 // titb_clip_max_partials() floats; *n_partials receives how many were written.

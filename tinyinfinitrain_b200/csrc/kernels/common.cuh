@@ -18,6 +18,7 @@ enum StatusCode : int {
   kStatusMbarTimeout = 1,   // an mbarrier wait inside a tcgen05/TMA pipeline gave up
   kStatusPeerTimeout = 2,   // a wait on a flag written by another GPU gave up
   kStatusBadShape = 3,
+  kStatusBadPage = 4,       // a page number or position outside a paged cache was met (and not followed)
 };
 
 // Number of SMs of the current device (cached per device); grid sizes and per-SM partial buffers derive from it.

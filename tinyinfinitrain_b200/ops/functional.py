@@ -25,6 +25,7 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from .._lib import C
 
@@ -717,6 +718,220 @@ def causal_attention(q, k, v, scale: Optional[float] = None):
         o = F.scaled_dot_product_attention(qt, kt, vt, is_causal=True, scale=scale, enable_gqa=Hq != Hkv)
         return o.transpose(1, 2).contiguous()
     return _call(_AttentionFn, q, k, v, scale)
+
+
+# ----------------------------------------------------------------- attention over a window and sinks
+_EVERYTHING = 2 ** 31 - 1     # a window that no sequence outgrows
+
+
+def _window_arg(window: Optional[int]) -> int:
+    return _EVERYTHING if window is None else window
+
+
+def window_attention_ref(q, k, v, window: Optional[int], sinks: int = 0, scale=None):
+    """attention_ref with the mask of window_attention."""
+    B, T, Hq, hd = q.shape
+    Hkv = k.shape[2]
+    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    qf, kf, vf = (t.float().transpose(1, 2) for t in (q, k, v))
+    if Hkv != Hq:
+        kf = kf.repeat_interleave(Hq // Hkv, dim=1)
+        vf = vf.repeat_interleave(Hq // Hkv, dim=1)
+    att = (qf @ kf.transpose(-1, -2)) * scale
+    i = torch.arange(T, device=q.device)
+    ahead = i[:, None] - i[None, :]
+    mask = (ahead >= 0) & ((ahead < _window_arg(window)) | (i[None, :] < sinks))
+    att = att.masked_fill(~mask, float("-inf")).softmax(-1)
+    return (att @ vf).transpose(1, 2).to(q.dtype)
+
+
+class _WindowAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, scale):
+        o, lse = C.window_attn_fwd(q, k, v, window, sinks, scale)
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.args = (window, sinks, scale)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse = ctx.saved_tensors
+        dq, dk, dv = C.window_attn_bwd(do, q, k, v, o, lse, *ctx.args)
+        return dq, dk, dv, None, None, None
+
+
+class _WindowAttentionQKVFn(torch.autograd.Function):
+    """Over a fused projection buffer, as _AttentionQKVFn."""
+
+    @staticmethod
+    def forward(ctx, qkv, Hq, Hkv, hd, window, sinks, scale):
+        qkv = qkv.contiguous()
+        o, lse = C.window_attn_fwd(*_AttentionQKVFn._views(qkv, Hq, Hkv, hd), window, sinks, scale)
+        ctx.save_for_backward(qkv, o, lse)
+        ctx.args = (Hq, Hkv, hd, window, sinks, scale)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        qkv, o, lse = ctx.saved_tensors
+        Hq, Hkv, hd, window, sinks, scale = ctx.args
+        dqkv = torch.empty_like(qkv)
+        C.window_attn_bwd(do, *_AttentionQKVFn._views(qkv, Hq, Hkv, hd), o, lse, window, sinks, scale,
+                          *_AttentionQKVFn._views(dqkv, Hq, Hkv, hd))
+        return dqkv, None, None, None, None, None, None
+
+
+def window_attention(q, k, v, window: Optional[int], sinks: int = 0, scale: Optional[float] = None):
+    """Causal self-attention over a bounded context: query i sees key j when ``j <= i`` and (``i - j < window`` or
+    ``j < sinks``), i.e. the last ``window`` positions, its own among them, and the first ``sinks`` of the sequence.
+
+    Shapes and layouts as in :func:`causal_attention`; ``window=None`` is no bound.  float32 or bfloat16; on the GPU a head
+    size that is a multiple of 8 up to 128.  q, k and v have to be finite: inside a tile of 128 positions a key's or value's
+    NaN or infinity reaches queries that do not see it."""
+    hd = q.shape[-1]
+    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    if not q.is_cuda:
+        C.window_check(q, k, v, _window_arg(window), sinks)
+        return window_attention_ref(q, k, v, window, sinks, scale)
+    return _call(_WindowAttentionFn, q, k, v, _window_arg(window), sinks, scale)
+
+
+def window_attention_qkv(qkv, n_head: int, n_kv_head: Optional[int] = None, window: Optional[int] = None, sinks: int = 0,
+                         scale: Optional[float] = None):
+    """:func:`window_attention` on a fused QKV projection [B, T, (Hq + 2 Hkv) * hd] -> [B, T, Hq, hd]."""
+    Hq = n_head
+    Hkv = n_kv_head if n_kv_head is not None else n_head
+    hd = qkv.shape[-1] // (Hq + 2 * Hkv)
+    if qkv.dim() != 3 or hd * (Hq + 2 * Hkv) != qkv.shape[-1]:
+        raise RuntimeError(f"titb200 window_attention: a projection of shape {tuple(qkv.shape)} does not hold "
+                           f"{Hq} + 2 * {Hkv} heads")
+    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    if qkv.is_cuda:
+        return _call(_WindowAttentionQKVFn, qkv, Hq, Hkv, hd, _window_arg(window), sinks, scale)
+    B, T, _ = qkv.shape
+    q, k, v = (t.reshape(B, T, -1, hd) for t in qkv.split((Hq * hd, Hkv * hd, Hkv * hd), dim=-1))
+    return window_attention(q, k, v, window, sinks, scale)
+
+
+# ----------------------------------------------------------------- paged key-value cache
+def _forward_only(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"titb200 {name} has no gradient: call it under torch.no_grad()")
+
+
+def _cache_row(page_table, b: int, pos: int, page_size: int, n_pages: int) -> int:
+    """The page that holds position ``pos`` of sequence b."""
+    slot = pos // page_size
+    if pos < 0 or slot >= page_table.shape[1]:
+        raise IndexError(f"position {pos} of sequence {b} lies outside its {page_table.shape[1]} pages of {page_size}")
+    page = int(page_table[b, slot])
+    if not 0 <= page < n_pages:
+        raise IndexError(f"page {page} of sequence {b} lies outside the cache of {n_pages} pages")
+    return page
+
+
+def cache_append_ref(qkv, k_cache, v_cache, page_table, starts, n_head: int, n_kv_head: int, theta: Optional[float] = None,
+                     counts=None, window: Optional[int] = None, sinks: int = 0):
+    """cache_append token by token: (q, k) of all tokens; the caches are updated in place."""
+    n_pages, Hkv, page_size, hd = k_cache.shape
+    B, T, _ = qkv.shape
+    x = qkv.reshape(B, T, n_head + 2 * Hkv, hd)
+    q, k, v = x[:, :, :n_head], x[:, :, n_head:n_head + Hkv], x[:, :, n_head + Hkv:]
+    if theta is not None:
+        half = hd // 2
+        pos = starts.double()[:, None] + torch.arange(T, dtype=torch.float64, device=qkv.device)
+        ang = pos[:, :, None] * float(theta) ** (torch.arange(half, dtype=torch.float64, device=qkv.device) * (-2.0 / hd))
+        cos, sin = ang.cos().float()[:, :, None], ang.sin().float()[:, :, None]
+
+        def turn(t):
+            a, b = t[..., :half].float(), t[..., half:].float()
+            return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1).to(t.dtype)
+
+        q, k = turn(q), turn(k)
+    for b in range(B):
+        start, count = int(starts[b]), min(T, int(counts[b])) if counts is not None else T
+        for t in range(count):
+            pos = start + t
+            if pos >= start + count - _window_arg(window) or pos < sinks:
+                page = _cache_row(page_table, b, pos, page_size, n_pages)
+                k_cache[page, :, pos % page_size] = k[b, t]
+                v_cache[page, :, pos % page_size] = v[b, t]
+    return q, k
+
+
+def cache_append(qkv, k_cache, v_cache, page_table, starts, n_head: int, n_kv_head: Optional[int] = None,
+                 theta: Optional[float] = None, counts=None, window: Optional[int] = None, sinks: int = 0,
+                 return_k: bool = False):
+    """Writes the keys and values of new tokens into the pages of a cache, after the rotary embedding, and returns their
+    queries [B, T, Hq, hd] (with ``return_k`` the pair of queries and keys, for the attention of a prompt over itself).
+
+    qkv: [B, T, (Hq + 2 Hkv) * hd]; k_cache, v_cache: [pages, Hkv, page_size, hd], contiguous; page_table: int32 [B, n],
+    position p of sequence b being row ``p % page_size`` of page ``page_table[b, p // page_size]``; starts: int32 [B], the
+    position of each sequence's first new token; counts: int32 [B], how many of the T tokens are real (the others, padding
+    behind a shorter prompt, are not written; None: all).  ``theta``: base of the rotary embedding, pairing element i with
+    i + hd / 2; None: no rotation, and the returned tensors are views of qkv.  With ``window`` and ``sinks`` only what the token
+    after the last one sees is written (the last ``window`` positions and the first ``sinks``), so that the pages of a window
+    can be a ring.
+
+    Every written position must have a row of its own.  A page number or position outside the cache raises IndexError on the
+    CPU; on the GPU it is not followed, and ``parallel.health.check_device_status()`` raises."""
+    Hkv = n_kv_head if n_kv_head is not None else n_head
+    _forward_only("cache_append", qkv, k_cache, v_cache)
+    if theta is not None and not theta > 0:
+        raise RuntimeError(f"titb200 cache_append: theta must be positive, got {theta}")
+    args = (qkv, k_cache, v_cache, page_table, starts, n_head, Hkv, theta or 0.0, counts, _window_arg(window), sinks)
+    if not qkv.is_cuda:
+        C.cache_append_check(*args)
+        q, k = cache_append_ref(qkv, k_cache, v_cache, page_table, starts, n_head, Hkv, theta, counts, window, sinks)
+        return (q, k) if return_k else q
+    q, k = C.cache_append(*args, return_k)
+    if theta is None:
+        heads = qkv.unflatten(-1, (n_head + 2 * Hkv, k_cache.shape[-1]))
+        q, k = heads[:, :, :n_head], heads[:, :, n_head:n_head + Hkv]
+    return (q, k) if return_k else q
+
+
+def paged_attention_ref(q, k_cache, v_cache, page_table, lengths, window: Optional[int] = None, sinks: int = 0, scale=None):
+    """paged_attention, sequence by sequence over a gathered copy of its pages."""
+    n_pages, Hkv, page_size, hd = k_cache.shape
+    B, Hq, _ = q.shape
+    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    out = torch.zeros(B, Hq, hd, dtype=q.dtype, device=q.device)
+    for b in range(B):
+        n = int(lengths[b])
+        if n < 0:
+            raise IndexError(f"length {n} of sequence {b} is negative")
+        seen = [p for p in range(n) if p >= n - _window_arg(window) or p < sinks]
+        if not seen:
+            continue
+        pages = torch.tensor([_cache_row(page_table, b, p, page_size, n_pages) for p in seen], device=q.device)
+        rows = torch.tensor([p % page_size for p in seen], device=q.device)
+        k, v = (c[pages, :, rows].float().transpose(0, 1) for c in (k_cache, v_cache))      # [Hkv, n, hd]
+        att = (q[b].float().view(Hkv, Hq // Hkv, hd) @ k.transpose(1, 2) * scale).softmax(-1)
+        out[b] = (att @ v).reshape(Hq, hd).to(q.dtype)
+    return out
+
+
+def paged_attention(q, k_cache, v_cache, page_table, lengths, window: Optional[int] = None, sinks: int = 0,
+                    scale: Optional[float] = None):
+    """Attention of one new token per sequence over the positions that the cache holds, its own among them.
+
+    q: [B, Hq, hd]; caches and page_table as in :func:`cache_append`; lengths: int32 [B], how many positions sequence b has
+    (the query is that of position ``lengths[b] - 1``).  With ``window`` and ``sinks`` the query sees the last ``window`` of
+    them and the first ``sinks``.  Returns [B, Hq, hd]; zeros for a sequence of length 0.  Rows of the pages that hold no visible
+    position are not read, whatever they contain.
+
+    A page number or length outside the cache raises IndexError on the CPU; on the GPU it is not followed, and
+    ``parallel.health.check_device_status()`` raises."""
+    scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    _forward_only("paged_attention", q, k_cache, v_cache)
+    args = (q, k_cache, v_cache, page_table, lengths, _window_arg(window), sinks)
+    if not q.is_cuda:
+        C.paged_attention_check(*args)
+        return paged_attention_ref(q, k_cache, v_cache, page_table, lengths, window, sinks, scale)
+    return C.paged_attention(*args, scale)
 
 
 # -------------------------------------------------------------------- elementwise family

@@ -82,7 +82,7 @@ class HealthMonitor:
 
 
 def check_device_status(clear: bool = True) -> None:
-    """Raises if a device-side bounded wait gave up since the last check."""
+    """Raises if a device-side bounded wait gave up, or a page table led outside its cache, since the last check."""
     from .._lib import C
 
     code = int(C.status_read(clear))
@@ -90,5 +90,7 @@ def check_device_status(clear: bool = True) -> None:
         raise RuntimeError("a tcgen05/TMA pipeline wait timed out inside a kernel (status 1)")
     if code == 2:
         raise PeerFailure(-1, "a device-side wait on another GPU's flag timed out (status 2)")
+    if code == 4:
+        raise RuntimeError("a page number or position outside a paged key-value cache was met (status 4)")
     if code != 0:
         raise RuntimeError(f"kernel status word = {code}")
