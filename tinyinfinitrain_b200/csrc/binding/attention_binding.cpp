@@ -152,6 +152,8 @@ std::vector<Tensor> window_attn_bwd(const Tensor& d_o_, const Tensor& q_, const 
   d.d_o = d_o.data_ptr(); d.dq = dq.data_ptr(); d.dk = dk.data_ptr(); d.dv = dv.data_ptr();
   d.delta = delta.data_ptr<float>();
   d.do_stride_t = token_stride(d_o); d.dq_stride_t = token_stride(dq); d.dk_stride_t = token_stride(dk); d.dv_stride_t = token_stride(dv);
+  Tensor work = at::empty({titb_window_attn_bwd_workspace(&w)}, q.options().dtype(at::kFloat));
+  w.workspace = work.data_ptr<float>();
   check(titb_window_attn_bwd(&w, at::cuda::getCurrentCUDAStream().stream()), "window_attention backward");
   return {dq, dk, dv};
 }

@@ -77,7 +77,19 @@ struct AttnArgs {
   bf16* dv;
   long long dk_stride_t, dv_stride_t;
   int* status;
+  // window attention: query i sees key j <= i when i - j < window or j < sinks (both at most T)
+  int window, sinks;
+  // its backward pass: key blocks that hold sinks, the query blocks that one of their CTAs takes, and the CTAs of a block
+  int sink_blocks, sink_step, sink_parts;
+  float* sink_part;  // fp32 [sink_parts][B][sink_blocks][Hkv][dK, dV][kBlk][hd]
 };
+
+// Bits [lo, hi) of a 32-bit word; lo and hi may lie outside it.
+__device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
+  lo = max(lo, 0);
+  hi = min(hi, 32);
+  return hi <= lo ? 0u : (0xffffffffu >> (32 - (hi - lo))) << lo;
+}
 
 // ------------------------------------------------------------------------- forward
 template <int HD>
@@ -108,7 +120,10 @@ struct FwdCfg {
 // exponentials per block and SM, with the chain S -> maximum -> exponentials -> P of two CTAs (hd 64) to hide it.
 // Measured (B200; before = scalar, tiles of one head in a row): 8 x 1024, 12 heads, hd 64: 39.6 -> 32.3 us; 1 x 1999, 32 / 8
 // heads: 48.8 -> 33.4 us; 4 x 2048: 138 -> 117 us; hd 128, 1 x 4096, 32 / 8 heads: 174 -> 153 us (897 TFLOP/s).
-template <int HD>
+//
+// WIN: a window and sinks.  The CTA visits the key blocks of the sinks and those from its first query's window to its own; a
+// block on either border of what the rows see is masked by a 128-bit mask per row, built from the row's two ranges of keys.
+template <int HD, bool WIN>
 __global__ void __launch_bounds__(kAttnThreads, (HD == 64) ? 2 : 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                 const __grid_constant__ CUtensorMap tv, const AttnArgs p) {
@@ -133,7 +148,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   const int h = blockIdx.x % p.Hq, b = blockIdx.x / p.Hq;
   const int hk = h / (p.Hq / p.Hkv);
   const int q0 = qb * kBlk;
-  const int nblk = qb + 1;
+  const int first_blk = WIN ? max(0, q0 - p.window + 1) / kBlk : 0;                         // of the window
+  const int n_sink_blk = WIN ? min((p.sinks + kBlk - 1) / kBlk, first_blk) : 0;
+  const int nblk = n_sink_blk + qb - first_blk + 1;
+  auto key0 = [&](int j) { return (WIN ? (j < n_sink_blk ? j : first_blk + j - n_sink_blk) : j) * kBlk; };
 
   if (threadIdx.x == 0) {
     ptx::mbar_init(q_full, 1);
@@ -179,13 +197,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c)
           ptx::tma_load_3d(smem + Cfg::kK + st * Cfg::kTileBytes + c * kChunkBytes, &tk, &k_full[st], hk * HD + c * 64,
-                           j * kBlk, b);
+                           key0(j), b);
         if (!ptx::mbar_wait(&v_empty[st], ((j >> 1) & 1) ^ 1u, abort_flag)) break;
         ptx::mbar_expect_tx(&v_full[st], Cfg::kTileBytes);
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c)
           ptx::tma_load_3d(smem + Cfg::kV + st * Cfg::kTileBytes + c * kChunkBytes, &tv, &v_full[st], hk * HD + c * 64,
-                           j * kBlk, b);
+                           key0(j), b);
       }
     }
   } else if (warp == 1) {
@@ -256,8 +274,26 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       ptx::tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(s_free);   // the score columns may be overwritten by S(j+1)
-      const int kv0 = j * kBlk;
-      if (j == qb) {  // diagonal block: keys after the query are masked
+      const int kv0 = key0(j);
+      if (WIN) {
+        // a block before the rows' own in which the last row's window does not begin yet, or that lies among the sinks: whole
+        const bool whole = kv0 != q0 && (kv0 + p.window > q0 + kBlk - 1 || kv0 + kBlk <= p.sinks);
+        if (!whole) {
+          const uint32_t ninf = __float_as_uint(-INFINITY);
+          const int sink_end = p.sinks - kv0, lo = q_idx - p.window + 1 - kv0, hi = q_idx + 1 - kv0;
+          auto mask_chunk = [&](uint32_t (&r)[32], int c) {
+            // both ranges end with the row's own key
+            const uint32_t see = bit_range(-32 * c, min(sink_end, hi) - 32 * c) | bit_range(lo - 32 * c, hi - 32 * c);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(see & (1u << e))) r[e] = ninf;
+          };
+          mask_chunk(r0, 0);
+          mask_chunk(r1, 1);
+          mask_chunk(r2, 2);
+          mask_chunk(r3, 3);
+        }
+      } else if (j == qb) {  // diagonal block: keys after the query are masked
         const uint32_t ninf = __float_as_uint(-INFINITY);
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
@@ -301,7 +337,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           if (need) m_ref = m_blk;
         }
       }
-      const float neg = -m_ref;
+      const float neg = WIN && m_ref == -INFINITY ? 0.f : -m_ref;   // a row may see nothing of its first blocks
       float rs0 = 0.f, rs1 = 0.f;
       auto exp_chunk = [&](uint32_t (&r)[32], int c) {
         uint32_t pk[16];
@@ -413,7 +449,11 @@ struct BwdCfg {
 // Measured (B200, with the delta and conversion passes; before = scores untransposed, P and dS through shared memory, dQ
 // flushed by the element-wise warps): hd 128, 1 x 4096, 32 / 8 heads: 978 -> 351 us (980 TFLOP/s); hd 64, 4 x 2048,
 // 32 / 8 heads: 376 -> 249 us; 8 x 1024, 12 heads: 117 -> 91 us; 3 x 777, 12 heads: 50 -> 32 us.
-template <int HD>
+//
+// WIN: a window and sinks.  A block of keys meets the query blocks up to its last key's window.  A block that holds sinks meets
+// all later ones, which would make its CTA the last by far: its query blocks are split over sink_parts CTAs, which leave
+// fp32 sums that attn_sink_join_kernel adds in order.
+template <int HD, bool WIN>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                 const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
@@ -441,10 +481,21 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   const int warp = ptx::warp_index(), lane = threadIdx.x & 31;
   const int nqb = (p.T + kBlk - 1) / kBlk;
   // key block 0 meets every query block: the longest CTAs of all heads start first
-  const int jb = blockIdx.y;
+  // (WIN: the parts of the sinks' blocks come first)
+  const int n_sink_ctas = WIN ? p.sink_blocks * p.sink_parts : 0;
+  const bool sink_cta = WIN && static_cast<int>(blockIdx.y) < n_sink_ctas;
+  const int part = sink_cta ? blockIdx.y % p.sink_parts : 0;
+  const int jb = !WIN ? blockIdx.y : sink_cta ? blockIdx.y / p.sink_parts : blockIdx.y - n_sink_ctas + p.sink_blocks;
   const int hk = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv;
   const int G = p.Hq / p.Hkv;
-  const int nq = nqb - jb;     // query blocks jb .. nqb-1
+  int ib = jb, nq = nqb - jb;  // query blocks ib .. ib + nq - 1
+  if (sink_cta) {
+    ib += part * p.sink_step;
+    nq = min(nqb - ib, p.sink_step);
+    if (nq <= 0) return;       // the later blocks have fewer parts
+  } else if (WIN) {
+    nq = min(nq, static_cast<int>((jb * static_cast<long long>(kBlk) + kBlk - 1 + p.window - 1) / kBlk) - jb + 1);
+  }
   const int niter = G * nq;
 
   if (threadIdx.x == 0) {
@@ -497,7 +548,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
     bool ok = true;
     int it = 0;
     for (; it < niter; ++it) {
-      const int g = it / nq, i = jb + (it - g * nq);
+      const int g = it / nq, i = ib + (it - g * nq);
       const int h = hk * G + g;
       const int st = it & 1, dst = it % DS;
       // row statistics: requested before the waits; rows past the end of the sequence get lse = +inf, which turns their
@@ -637,7 +688,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
             make_uint4(r[u * 4], r[u * 4 + 1], r[u * 4 + 2], r[u * 4 + 3]);
     };
     for (int it = 0; it < niter; ++it) {
-      const int g = it / nq, i = jb + (it - g * nq);
+      const int g = it / nq, i = ib + (it - g * nq);
       const int x = (hk * G + g) * HD, y = i * kBlk + quad * 32;
       if (!ptx::mbar_wait_warp(dq_full, it & 1, abort_flag)) break;
       ptx::tc_fence_after_sync();
@@ -695,7 +746,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       ptx::tmem_ld32(tS, pr[0]);
       ptx::tmem_ld32(tS + 32, pr[1]);
       ptx::tmem_ld_wait();
-      const bool diag = it % nq == 0;                // keys after the query get probability zero
+      const int q0 = (ib + it % nq) * kBlk;
+      // keys after the query get probability zero, with a window those before it too
+      const bool diag = !WIN && it % nq == 0;
+      uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+      const bool border = WIN && (q0 == jb * kBlk || q0 + kBlk - 1 - jb * kBlk >= p.window);
+      if (border) {
+        const int key = jb * kBlk + row, lo = key - q0 - half * 64, hi = key < p.sinks ? kBlk : lo + p.window;
+        see[0] = bit_range(lo, hi);
+        see[1] = bit_range(lo - 32, hi - 32);
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t pk[16];
@@ -712,6 +772,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
             if (row > q + 1) x1 = 0.f;
             if (row > q + 2) x2 = 0.f;
             if (row > q + 3) x3 = 0.f;
+          }
+          if (border) {
+            if (!(see[c] & (1u << e))) x0 = 0.f;
+            if (!(see[c] & (2u << e))) x1 = 0.f;
+            if (!(see[c] & (4u << e))) x2 = 0.f;
+            if (!(see[c] & (8u << e))) x3 = 0.f;
           }
           pk[e / 2] = pack_bf16x2(x0, x1);
           pk[e / 2 + 1] = pack_bf16x2(x2, x3);
@@ -771,7 +837,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           uint32_t r[32];
           ptx::tmem_ld32(tmem_base + col + lane_sel + c * 32, r);
           ptx::tmem_ld_wait();
-          if (kv_idx < p.T) {
+          if (sink_cta && p.sink_parts > 1) {
+            float* sum = p.sink_part + ((((static_cast<long long>(part) * p.B + b) * p.sink_blocks + jb) * p.Hkv + hk) * 2 + 1 - which) * (kBlk * HD) +
+                         row * HD + c * 32;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(sum + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
+          } else if (kv_idx < p.T) {
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
               uint4 u;
@@ -848,6 +920,31 @@ __global__ void attn_dq_convert_kernel(const float* __restrict__ acc, bf16* __re
   }
 }
 
+// dK and dV of the sinks' blocks: the sums of their parts, in order.  One thread per four elements of a row.
+template <int HD>
+__global__ void attn_sink_join_kernel(const AttnArgs p) {
+  const int nqb = (p.T + kBlk - 1) / kBlk, rows = min(p.T, p.sink_blocks * kBlk);
+  const long long n = static_cast<long long>(p.B) * rows * p.Hkv * 2 * (HD / 4);
+  const long long part_size = static_cast<long long>(p.B) * p.sink_blocks * p.Hkv * 2 * kBlk * HD;
+  for (long long x = blockIdx.x * (long long)blockDim.x + threadIdx.x; x < n; x += (long long)gridDim.x * blockDim.x) {
+    const int d = static_cast<int>(x % (HD / 4)) * 4;
+    long long r = x / (HD / 4);
+    const int which = static_cast<int>(r % 2), hk = static_cast<int>(r / 2 % p.Hkv);
+    r = r / 2 / p.Hkv;
+    const int t = static_cast<int>(r % rows), b = static_cast<int>(r / rows), jb = t / kBlk;
+    const float* src = p.sink_part + (((static_cast<long long>(b) * p.sink_blocks + jb) * p.Hkv + hk) * 2 + which) * (kBlk * HD) + (t % kBlk) * HD + d;
+    const int parts = (nqb - jb + p.sink_step - 1) / p.sink_step;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < parts; ++c) {
+      const float4 f = *reinterpret_cast<const float4*>(src + c * part_size);
+      sum.x += f.x; sum.y += f.y; sum.z += f.z; sum.w += f.w;
+    }
+    const long long bt = static_cast<long long>(b) * p.T + t;
+    bf16* dst = (which == 0 ? p.dk + bt * p.dk_stride_t : p.dv + bt * p.dv_stride_t) + hk * HD + d;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+  }
+}
+
 static bool attn_check(const TitbAttnDesc* d) {
   if (d->hd != 64 && d->hd != 128) return false;
   if (d->Hq % d->Hkv) return false;
@@ -857,15 +954,15 @@ static bool attn_check(const TitbAttnDesc* d) {
   return true;
 }
 
-template <int HD>
-static int attn_fwd_launch(const TitbAttnDesc* d, cudaStream_t st) {
+template <int HD, bool WIN = false>
+static int attn_fwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 0, int sinks = 0) {
   using Cfg = FwdCfg<HD>;
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) dev = 0;
   if (!attr_set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<HD, WIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
     attr_set[dev] = true;
   }
@@ -879,22 +976,38 @@ static int attn_fwd_launch(const TitbAttnDesc* d, cudaStream_t st) {
   AttnArgs a{};
   a.B = d->B; a.T = d->T; a.Hq = d->Hq; a.Hkv = d->Hkv; a.hd = HD;
   a.scale = d->scale;
+  a.window = window; a.sinks = sinks;
   a.o = static_cast<bf16*>(d->o); a.lse = d->lse; a.o_stride_t = d->o_stride_t;
   a.status = titb_status_ptr();
   dim3 grid(static_cast<unsigned>(d->Hq) * d->B, (d->T + kBlk - 1) / kBlk);
-  launch_dependent(attn_fwd_kernel<HD>, grid, kAttnThreads, Cfg::kSmem, st, tq, tk, tv, a);
+  launch_dependent(attn_fwd_kernel<HD, WIN>, grid, kAttnThreads, Cfg::kSmem, st, tq, tk, tv, a);
   return static_cast<int>(cudaGetLastError());
 }
 
-template <int HD>
-static int attn_bwd_launch(const TitbAttnDesc* d, cudaStream_t st) {
+// How the backward pass of window attention splits the key blocks of the sinks: parts no longer than what another block of
+// keys takes, or than a quarter of an SM's share of all work.
+struct SinkSplit {
+  int blocks, step, parts;
+};
+static SinkSplit sink_split(const TitbAttnDesc& d, int window, int sinks) {
+  const long long nqb = (d.T + kBlk - 1) / kBlk, near = (window + 2LL * kBlk - 2) / kBlk + 1;
+  const long long blocks = (sinks + kBlk - 1) / kBlk;
+  if (blocks == 0) return {0, 1, 1};
+  const long long work = static_cast<long long>(d.Hkv) * d.B * (blocks * nqb + (nqb - blocks) * near);
+  const long long share = work / (device_sm_count() * 4LL);
+  const long long step = near > share ? near : share;
+  return {static_cast<int>(blocks), static_cast<int>(step < nqb ? step : nqb), static_cast<int>((nqb + step - 1) / step)};
+}
+
+template <int HD, bool WIN = false>
+static int attn_bwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 0, int sinks = 0, float* sink_part = nullptr) {
   using Cfg = BwdCfg<HD>;
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) dev = 0;
   if (!attr_set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(attn_bwd_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(attn_bwd_kernel<HD, WIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
     attr_set[dev] = true;
   }
@@ -918,14 +1031,39 @@ static int attn_bwd_launch(const TitbAttnDesc* d, cudaStream_t st) {
   a.dk = static_cast<bf16*>(d->dk); a.dv = static_cast<bf16*>(d->dv);
   a.dk_stride_t = d->dk_stride_t; a.dv_stride_t = d->dv_stride_t;
   a.status = titb_status_ptr();
-  dim3 grid(static_cast<unsigned>(d->Hkv) * d->B, (d->T + kBlk - 1) / kBlk);
-  launch_dependent(attn_bwd_kernel<HD>, grid, kBwdThreads, Cfg::kSmem, st, tq, tk, tv, tdo, tdq, a);
+  unsigned jobs = (d->T + kBlk - 1) / kBlk;
+  if (WIN) {
+    const SinkSplit split = sink_split(*d, window, sinks);
+    a.window = window; a.sinks = sinks;
+    a.sink_blocks = split.blocks; a.sink_step = split.step; a.sink_parts = split.parts; a.sink_part = sink_part;
+    jobs += split.blocks * (split.parts - 1);
+  }
+  dim3 grid(static_cast<unsigned>(d->Hkv) * d->B, jobs);
+  launch_dependent(attn_bwd_kernel<HD, WIN>, grid, kBwdThreads, Cfg::kSmem, st, tq, tk, tv, tdo, tdq, a);
+  if (WIN && a.sink_blocks > 0 && a.sink_parts > 1) {
+    const int rows = a.sink_blocks * kBlk < d->T ? a.sink_blocks * kBlk : d->T;
+    const long long blocks = (static_cast<long long>(d->B) * rows * d->Hkv * 2 * (HD / 4) + 255) / 256, most = device_sm_count() * 8LL;
+    attn_sink_join_kernel<HD><<<static_cast<int>(blocks < most ? blocks : most), 256, 0, st>>>(a);
+  }
   const long long bt = static_cast<long long>(d->B) * d->T;
   const int width = d->Hq * HD;
   int cb = static_cast<int>((bt * (width / 8) + 255) / 256);
   if (cb > device_sm_count() * 8) cb = device_sm_count() * 8;
   attn_dq_convert_kernel<<<cb, 256, 0, st>>>(d->dq_accum, static_cast<bf16*>(d->dq), bt, width, d->dq_stride_t);
   return static_cast<int>(cudaGetLastError());
+}
+
+// bf16 window attention, hd 64 or 128 (window_attention.cu checks the operands); window and sinks at most T.
+int window_tc_fwd(const TitbAttnDesc* d, int window, int sinks, cudaStream_t st) {
+  return d->hd == 64 ? attn_fwd_launch<64, true>(d, st, window, sinks) : attn_fwd_launch<128, true>(d, st, window, sinks);
+}
+int window_tc_bwd(const TitbAttnDesc* d, int window, int sinks, float* sink_part, cudaStream_t st) {
+  return d->hd == 64 ? attn_bwd_launch<64, true>(d, st, window, sinks, sink_part)
+                     : attn_bwd_launch<128, true>(d, st, window, sinks, sink_part);
+}
+long long window_tc_sink_floats(const TitbAttnDesc* d, int window, int sinks) {
+  const SinkSplit s = sink_split(*d, window, sinks);
+  return s.parts > 1 ? static_cast<long long>(s.parts) * d->B * s.blocks * d->Hkv * 2 * kBlk * d->hd : 0;
 }
 
 }  // namespace titb

@@ -1,5 +1,5 @@
 // Causal attention over a window of the last positions and a few first ones (sinks), on the CUDA cores: fp32 tensors, and bf16
-// tensors whose head size the tensor-core kernels do not take.
+// tensors whose head size the tensor-core kernels (attention_tcgen05.cu) do not take.
 //
 //   visible(i, j) = j <= i and (i - j < window or j < sinks)
 //   forward   S = scale Q K^T, O = softmax over the visible j of S times V, lse = log of the softmax's denominator
@@ -16,6 +16,11 @@
 #include "common.cuh"
 
 namespace titb {
+
+// bf16 heads of 64 and 128 (attention_tcgen05.cu)
+int window_tc_fwd(const TitbAttnDesc* d, int window, int sinks, cudaStream_t st);
+int window_tc_bwd(const TitbAttnDesc* d, int window, int sinks, float* sink_part, cudaStream_t st);
+long long window_tc_sink_floats(const TitbAttnDesc* d, int window, int sinks);
 
 constexpr int kWinThreads = 256;   // 16 x 16 threads over a tile
 constexpr int kWinRows = 64;       // rows of the tile that a CTA owns
@@ -416,14 +421,18 @@ __global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p
   }
 }
 
+// more than the sequence changes nothing
+static int window_of(const TitbWindowDesc* w) { return w->window < w->attn.T ? w->window : w->attn.T; }
+static int sinks_of(const TitbWindowDesc* w) { return w->sinks < w->attn.T ? w->sinks : w->attn.T; }
+static bool on_tensor_cores(const TitbWindowDesc* w) { return w->dtype == 1 && (w->attn.hd == 64 || w->attn.hd == 128); }
+
 static WinArgs win_args(const TitbWindowDesc* w) {
   const TitbAttnDesc& d = w->attn;
   WinArgs a{};
   a.q = d.q; a.k = d.k; a.v = d.v; a.o = d.o; a.lse = d.lse;
   a.d_o = d.d_o; a.dq = d.dq; a.dk = d.dk; a.dv = d.dv; a.delta = d.delta;
   a.T = d.T; a.Hq = d.Hq; a.Hkv = d.Hkv; a.hd = d.hd; a.scale = d.scale;
-  a.window = w->window < d.T ? w->window : d.T;   // more than the sequence changes nothing
-  a.sinks = w->sinks < d.T ? w->sinks : d.T;
+  a.window = window_of(w); a.sinks = sinks_of(w);
   a.q_st = d.q_stride_t; a.k_st = d.k_stride_t; a.v_st = d.v_stride_t; a.o_st = d.o_stride_t;
   a.do_st = d.do_stride_t; a.dq_st = d.dq_stride_t; a.dk_st = d.dk_stride_t; a.dv_st = d.dv_stride_t;
   return a;
@@ -472,6 +481,7 @@ TITB_API int titb_window_attn_fwd(const TitbWindowDesc* w, cudaStream_t st) {
   (void)cudaGetLastError();
   if (w->attn.B <= 0 || w->attn.T <= 0 || w->attn.Hq <= 0) return 0;
   if (const int rc = win_check(w, false)) return rc;
+  if (on_tensor_cores(w)) return window_tc_fwd(&w->attn, window_of(w), sinks_of(w), st);
   if (w->dtype == 1) return w->attn.hd <= 64 ? win_fwd<bf16, 64>(w, st) : win_fwd<bf16, 128>(w, st);
   return w->attn.hd <= 64 ? win_fwd<float, 64>(w, st) : win_fwd<float, 128>(w, st);
 }
@@ -480,6 +490,18 @@ TITB_API int titb_window_attn_bwd(const TitbWindowDesc* w, cudaStream_t st) {
   (void)cudaGetLastError();
   if (w->attn.B <= 0 || w->attn.T <= 0 || w->attn.Hq <= 0) return 0;
   if (const int rc = win_check(w, true)) return rc;
+  if (on_tensor_cores(w)) {
+    TitbAttnDesc d = w->attn;
+    d.dq_accum = w->workspace;
+    float* sink_part = w->workspace + static_cast<long long>(d.B) * d.T * d.Hq * d.hd;
+    return window_tc_bwd(&d, window_of(w), sinks_of(w), sink_part, st);
+  }
   if (w->dtype == 1) return w->attn.hd <= 64 ? win_bwd<bf16, 64>(w, st) : win_bwd<bf16, 128>(w, st);
   return w->attn.hd <= 64 ? win_bwd<float, 64>(w, st) : win_bwd<float, 128>(w, st);
+}
+
+TITB_API long long titb_window_attn_bwd_workspace(const TitbWindowDesc* w) {
+  const TitbAttnDesc& d = w->attn;
+  if (d.B <= 0 || d.T <= 0 || d.Hq <= 0 || win_check(w, false) || !on_tensor_cores(w)) return 0;
+  return static_cast<long long>(d.B) * d.T * d.Hq * d.hd + window_tc_sink_floats(&d, window_of(w), sinks_of(w));
 }
