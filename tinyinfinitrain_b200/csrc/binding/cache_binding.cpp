@@ -116,8 +116,11 @@ Tensor paged_attention(const Tensor& q_, const Tensor& k_cache, const Tensor& v_
   const Tensor q = usable ? q_ : q_.clone(at::MemoryFormat::Contiguous);
   Tensor o = at::empty(q_.sizes(), q.options());
   const TitbCacheDesc d = cache_desc(k_cache, v_cache, table, q.size(1), window, sinks);
+  const int64_t bytes = titb_paged_attention_workspace(&d);
+  Tensor work;
+  if (bytes > 0) work = at::empty({bytes}, q.options().dtype(at::kByte));
   check(titb_paged_attention(&d, q.data_ptr(), q.stride(0), lengths.data_ptr<int>(), (float)scale, o.data_ptr(),
-                             at::cuda::getCurrentCUDAStream().stream()),
+                             bytes > 0 ? work.data_ptr() : nullptr, at::cuda::getCurrentCUDAStream().stream()),
         "paged_attention");
   return o;
 }

@@ -317,9 +317,11 @@ TITB_API int titb_cache_append(const TitbCacheDesc* d, const void* qkv, long lon
                                const int* starts, const int* counts, double theta, void* q_out, void* k_out,
                                cudaStream_t stream);
 // o[b] = attention of the query at position lengths[b] - 1 over positions p < lengths[b] with p >= lengths[b] - window or
-// p < sinks; zeros when there are none.  q: [B, Hq, hd] with q_stride_b elements between sequences; o: contiguous.
+// p < sinks; zeros when there are none.  q: [B, Hq, hd] with q_stride_b elements between sequences; o: contiguous.  workspace:
+// titb_paged_attention_workspace() bytes, 16-byte aligned, this call's own until it has run.
+TITB_API long long titb_paged_attention_workspace(const TitbCacheDesc* d);
 TITB_API int titb_paged_attention(const TitbCacheDesc* d, const void* q, long long q_stride_b, const int* lengths, float scale,
-                                  void* o, cudaStream_t stream);
+                                  void* o, void* workspace, cudaStream_t stream);
 
 // ---- gradient-norm clipping (device resident: graph-capturable) -------------------------------------------------
 // Stage 1: per-block partial sums of squares of a flat fp32 buffer (16-byte aligned).  `partials` must hold

@@ -142,94 +142,581 @@ struct PagedArgs {
   const int* lengths;
   void* o;
   float scale;
+  float* parts;   // per CTA two slots of partial results, [heads][hd] sums, [heads] maxima, [heads] denominators
+  int4* joins;    // per CTA the item whose first tiles it took, when others took the rest
 };
 
-constexpr int kPagedWarps = 4;
-constexpr int kPagedHeads = 4;   // query heads that share the loads of a pass over the cache
+// The work is cut into tiles of TILE positions of one item, an item being a sequence, one of its kv heads and up to HG of
+// the query heads that share it.  All tiles in a row (by sequence, then item, then position) are dealt to the CTAs in equal
+// runs, whatever the lengths, which only the device knows: a long sequence is split over as many CTAs as its share of the work,
+// and short ones share a CTA.  An item that a CTA holds from end to end is finished there.  Of any other the CTA leaves the
+// sums, their maximum and denominator in its slots (0: the item began before its run, 1: it goes on behind it), and
+// paged_join_kernel adds the slots up in order.
+__device__ __forceinline__ int paged_limit(const CacheArgs& c) {
+  return static_cast<int>(min(static_cast<long long>(c.table_width) * c.page_size, 0x7fffffffLL));
+}
+template <int HG>
+__device__ __forceinline__ int items_of(const CacheArgs& c) {
+  return c.Hkv * ((c.Hq / c.Hkv + HG - 1) / HG);
+}
 
-// One CTA per (sequence, kv head, group of query heads).  L lanes hold a row (16 bytes each); every group of L lanes takes
-// rows of its own and keeps its own running maximum, sum and output, which meet at the end.
-template <typename T, int L>
-__global__ void __launch_bounds__(kPagedWarps * 32) paged_attention_kernel(const PagedArgs p) {
-  constexpr int VN = 16 / sizeof(T), kRows = 32 / L, kGroups = kPagedWarps * kRows;
-  __shared__ float sm_m[kPagedHeads][kGroups], sm_l[kPagedHeads][kGroups];
-  __shared__ float sm_o[kPagedHeads][kGroups][L * VN];
-  const CacheArgs& c = p.c;
-  const int lane = threadIdx.x & 31, grp = (threadIdx.x >> 5) * kRows + lane / L, d0 = (lane % L) * VN;
-  const int G = c.Hq / c.Hkv, hgroups = (G + kPagedHeads - 1) / kPagedHeads;
-  const int hk = blockIdx.x / hgroups, g0 = (blockIdx.x % hgroups) * kPagedHeads, b = blockIdx.y;
-  const int ng = min(kPagedHeads, G - g0);
-  const bool in_head = d0 < c.hd;
-  const int limit = static_cast<int>(min(static_cast<long long>(c.table_width) * c.page_size, 0x7fffffffLL));
-  const int length = p.lengths[b];
-  if ((length < 0 || length > limit) && threadIdx.x == 0) atomicExch(c.status, kStatusBadPage);
-  const Seen seen = seen_of(length, limit, c.window, c.sinks);
-  const PageMap map = c.map(b);
+// A run of tiles.
+template <int TILE, int HG>
+struct TileWalk {
+  int b, item, t, n_tiles;
+  Seen seen;
+  __device__ __forceinline__ void enter(const PagedArgs& p, int limit) {
+    seen = seen_of(p.lengths[b], limit, p.c.window, p.c.sinks);
+    n_tiles = (seen.n + TILE - 1) / TILE;
+  }
+  __device__ __forceinline__ void next(const PagedArgs& p, int limit) {
+    if (++t < n_tiles) return;
+    t = 0;
+    if (++item < items_of<HG>(p.c)) return;
+    item = 0;
+    do {
+      if (++b >= p.c.B) return;   // behind the last tile
+      enter(p, limit);
+    } while (n_tiles == 0);
+  }
+};
 
-  float q[kPagedHeads][VN], o[kPagedHeads][VN] = {}, m[kPagedHeads], l[kPagedHeads];
-#pragma unroll
-  for (int g = 0; g < kPagedHeads; ++g) {
-    m[g] = -INFINITY;
-    l[g] = 0.f;
-#pragma unroll
-    for (int e = 0; e < VN; ++e) q[g][e] = 0.f;
-    if (g < ng && in_head) {
-      const Pack<T, VN> x = ld128(static_cast<const T*>(p.q) + b * p.q_stride_b + (hk * G + g0 + g) * c.hd + d0);
-#pragma unroll
-      for (int e = 0; e < VN; ++e) q[g][e] = to_f32(x.v[e]) * p.scale;
-    }
+struct Run {
+  int n;          // tiles of this CTA
+  long long per;  // tiles of every CTA but the last ones
+  long long first;
+};
+
+// This CTA's run, and the walk at its first tile.  Threads count the tiles of neighbouring sequences; a scan over the block
+// gives the sequence in which the run begins.  All threads of the CTA.
+template <int TILE, int HG, int THREADS>
+__device__ __forceinline__ Run begin_run(const PagedArgs& p, TileWalk<TILE, HG>& walk) {
+  __shared__ long long warp_sum[THREADS / 32];
+  __shared__ int at_b;
+  __shared__ long long at_rem;
+  const int limit = paged_limit(p.c), items = items_of<HG>(p.c), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunk = (p.c.B + THREADS - 1) / THREADS, b0 = min(p.c.B, static_cast<int>(threadIdx.x) * chunk), b1 = min(p.c.B, b0 + chunk);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int length = p.lengths[b];
+    if (blockIdx.x == 0 && (length < 0 || length > limit)) atomicExch(p.c.status, kStatusBadPage);
+    mine += static_cast<long long>((seen_of(length, limit, p.c.window, p.c.sinks).n + TILE - 1) / TILE) * items;
   }
-  for (int v = grp; v - grp < seen.n; v += kGroups) {   // all lanes take part in every round's shuffles
-    const long long row = v < seen.n ? map.row(seen.pos(v), c.Hkv, hk) : -1;
-    if (v < seen.n && row < 0 && lane % L == 0) atomicExch(c.status, kStatusBadPage);
-    Pack<T, VN> kx{}, vx{};
-    if (row >= 0 && in_head) {
-      kx = ld128(static_cast<const T*>(c.k_cache) + row * c.hd + d0);
-      vx = ld128(static_cast<const T*>(c.v_cache) + row * c.hd + d0);
-    }
+  long long scan = mine;
 #pragma unroll
-    for (int g = 0; g < kPagedHeads; ++g) {
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < VN; ++e) s = fmaf(q[g][e], to_f32(kx.v[e]), s);
-#pragma unroll
-      for (int w = 1; w < L; w <<= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-      if (row < 0) continue;
-      const float top = fmaxf(m[g], s), ref = top == -INFINITY ? 0.f : top;   // a score may be -inf
-      const float keep = expf(m[g] - ref), x = expf(s - ref);
-      m[g] = top;
-      l[g] = fmaf(l[g], keep, x);
-#pragma unroll
-      for (int e = 0; e < VN; ++e) o[g][e] = fmaf(o[g][e], keep, x * to_f32(vx.v[e]));
-    }
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, scan, d);
+    if (lane >= d) scan += x;
   }
+  if (lane == 31) warp_sum[warp] = scan;
+  __syncthreads();
+  long long before = scan - mine, total = 0;
 #pragma unroll
-  for (int g = 0; g < kPagedHeads; ++g) {
-    if (lane % L == 0) {
-      sm_m[g][grp] = m[g];
-      sm_l[g][grp] = l[g];
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+  Run run;
+  run.per = (total + gridDim.x - 1) / gridDim.x;
+  run.first = blockIdx.x * run.per;
+  run.n = static_cast<int>(max(0LL, min(run.per, total - run.first)));
+  if (run.n > 0 && run.first >= before && run.first < before + mine) {
+    long long rem = run.first - before;
+    int b = b0;
+    for (;; ++b) {
+      const long long here = static_cast<long long>((seen_of(p.lengths[b], limit, p.c.window, p.c.sinks).n + TILE - 1) / TILE) * items;
+      if (rem < here) break;
+      rem -= here;
     }
-#pragma unroll
-    for (int e = 0; e < VN; ++e) sm_o[g][grp][d0 + e] = o[g][e];
+    at_b = b;
+    at_rem = rem;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < ng * c.hd; i += kPagedWarps * 32) {
-    const int g = i / c.hd, d = i % c.hd;
-    float top = -INFINITY, sum = 0.f, acc = 0.f;
-    for (int w = 0; w < kGroups; ++w) top = fmaxf(top, sm_m[g][w]);
-    for (int w = 0; w < kGroups; ++w) {
-      if (sm_l[g][w] == 0.f) continue;
-      const float f = expf(sm_m[g][w] - top);
-      sum = fmaf(sm_l[g][w], f, sum);
-      acc = fmaf(sm_o[g][w][d], f, acc);
+  if (run.n > 0) {
+    walk.b = at_b;
+    walk.enter(p, limit);
+    walk.item = static_cast<int>(at_rem / walk.n_tiles);
+    walk.t = static_cast<int>(at_rem % walk.n_tiles);
+  }
+  return run;
+}
+
+// Zeros for the sequences that see nothing.
+template <typename T>
+__device__ __forceinline__ void clear_empty(const PagedArgs& p) {
+  const int limit = paged_limit(p.c), n = p.c.Hq * p.c.hd;
+  for (int b = blockIdx.x; b < p.c.B; b += gridDim.x)
+    if (min(p.lengths[b], limit) <= 0)
+      for (int i = threadIdx.x; i < n; i += blockDim.x) static_cast<T*>(p.o)[static_cast<long long>(b) * n + i] = from_f32<T>(0.f);
+}
+
+template <int HG>
+__device__ __forceinline__ long long slot_floats(const CacheArgs& c) { return HG * (c.hd + 2); }
+
+// The end of an item, or of this CTA's run inside one: the sums of `W` workers (o: [W][HG][pitch], m, l: [W][HG], base-2 maxima)
+// become the output or a partial result.  All threads; begins and ends with a barrier of the CTA.
+template <typename T, int HG, int W>
+__device__ __forceinline__ void finish_item(const PagedArgs& p, int b, int item, bool whole, bool began_before, const float* o,
+                                            int worker_stride, int pitch, const float (*m)[HG], const float (*l)[HG]) {
+  const CacheArgs& c = p.c;
+  const int G = c.Hq / c.Hkv, hgroups = (G + HG - 1) / HG, hk = item / hgroups, g0 = item % hgroups * HG, ng = min(HG, G - g0);
+  float* slot = p.parts + (blockIdx.x * 2LL + (began_before ? 0 : 1)) * slot_floats<HG>(c);
+  __syncthreads();
+  for (int i = threadIdx.x; i < ng * (c.hd / 4); i += blockDim.x) {
+    const int g = i / (c.hd / 4), d = i % (c.hd / 4) * 4;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, m[w][g]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (m[w][g] == -INFINITY && l[w][g] == 0.f) continue;   // saw nothing
+      const float f = exp2f(m[w][g] - ref);
+      const float4 x = *reinterpret_cast<const float4*>(o + w * worker_stride + g * pitch + d);
+      sum = fmaf(l[w][g], f, sum);
+      acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
+      acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
     }
-    static_cast<T*>(p.o)[(static_cast<long long>(b) * c.Hq + hk * G + g0 + g) * c.hd + d] = from_f32<T>(sum > 0.f ? acc / sum : 0.f);
+    if (whole) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      T* dst = static_cast<T*>(p.o) + (static_cast<long long>(b) * c.Hq + hk * G + g0 + g) * c.hd + d;
+      Pack<T, 4> r;
+      r.v[0] = from_f32<T>(acc.x * inv); r.v[1] = from_f32<T>(acc.y * inv);
+      r.v[2] = from_f32<T>(acc.z * inv); r.v[3] = from_f32<T>(acc.w * inv);
+      *reinterpret_cast<Pack<T, 4>*>(dst) = r;
+    } else {
+      *reinterpret_cast<float4*>(slot + g * c.hd + d) = acc;
+      if (d == 0) {
+        slot[HG * c.hd + g] = top;
+        slot[HG * (c.hd + 1) + g] = sum;
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// One CTA per CTA of the main kernel: the item that began in that one's run and went on behind it.
+template <typename T, int HG>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs p) {
+  dependency_wait();
+  const CacheArgs& c = p.c;
+  const int4 join = p.joins[blockIdx.x];   // sequence, item, last CTA, in use
+  if (!join.w) return;
+  const int G = c.Hq / c.Hkv, hgroups = (G + HG - 1) / HG, hk = join.y / hgroups, g0 = join.y % hgroups * HG, ng = min(HG, G - g0);
+  const long long size = slot_floats<HG>(c);
+  const float* first = p.parts + (blockIdx.x * 2LL + 1) * size;
+  const float* rest = p.parts + (blockIdx.x + 1) * 2LL * size;
+  const int n_rest = join.z - blockIdx.x;
+  for (int i = threadIdx.x; i < ng * (c.hd / 4); i += blockDim.x) {
+    const int g = i / (c.hd / 4), d = i % (c.hd / 4) * 4;
+    const int at_m = HG * c.hd + g, at_l = HG * (c.hd + 1) + g, at_o = g * c.hd + d;
+    float top = first[at_m];
+    for (int r = 0; r < n_rest; ++r) top = fmaxf(top, rest[r * 2 * size + at_m]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+    auto add = [&](const float* s) {
+      const float f = exp2f(s[at_m] - ref);
+      const float4 x = *reinterpret_cast<const float4*>(s + at_o);
+      sum = fmaf(s[at_l], f, sum);
+      acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
+      acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+    };
+    add(first);
+    for (int r = 0; r < n_rest; ++r) add(rest + r * 2 * size);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T* dst = static_cast<T*>(p.o) + (static_cast<long long>(join.x) * c.Hq + hk * G + g0 + g) * c.hd + d;
+    Pack<T, 4> o;
+    o.v[0] = from_f32<T>(acc.x * inv); o.v[1] = from_f32<T>(acc.y * inv);
+    o.v[2] = from_f32<T>(acc.z * inv); o.v[3] = from_f32<T>(acc.w * inv);
+    *reinterpret_cast<Pack<T, 4>*>(dst) = o;
+  }
+}
+
+constexpr int kPagedThreads = 128;
+
+// At the last tile of a CTA's run, for the join: whether its item began in the run and goes on behind it, and up to which CTA.
+template <int TILE, int HG>
+__device__ __forceinline__ void note_join(const PagedArgs& p, const Run& run, const TileWalk<TILE, HG>& at) {
+  if (threadIdx.x != 0 || p.joins == nullptr) return;
+  const long long last = run.first + run.n - 1 + (at.n_tiles - 1 - at.t);   // the item's last tile
+  const bool use = at.t < run.n && at.t + 1 < at.n_tiles;
+  p.joins[blockIdx.x] = make_int4(at.b, at.item, static_cast<int>(last / run.per), use);
+}
+
+// ---- any head size, fp32 arithmetic on the CUDA cores.  L lanes hold a row (16 bytes each); every group of L lanes takes rows
+// of its own, kBatch at a time, and keeps its own running maximum, sum and output.
+constexpr int kPagedHeads = 4;   // query heads that share the loads of a pass over the cache
+constexpr int kPagedTile = 64;
+
+template <typename T, int L>
+__global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const PagedArgs p) {
+  constexpr int VN = 16 / sizeof(T), kRows = 32 / L, kGroups = kPagedThreads / L, kBatch = 4, HG = kPagedHeads;
+  static_assert(kPagedTile % kGroups == 0 && kPagedTile / kGroups % kBatch == 0, "tile rows per group");
+  __shared__ float sm_m[kGroups][HG], sm_l[kGroups][HG];
+  __shared__ __align__(16) float sm_o[kGroups][HG][L * VN];
+  dependency_wait();
+  dependents_launch();
+  const CacheArgs& c = p.c;
+  const int lane = threadIdx.x & 31, grp = (threadIdx.x >> 5) * kRows + lane / L, d0 = (lane % L) * VN;
+  const int G = c.Hq / c.Hkv, hgroups = (G + HG - 1) / HG, limit = paged_limit(c);
+  const bool in_head = d0 < c.hd;
+  TileWalk<kPagedTile, HG> walk;
+  const Run run = begin_run<kPagedTile, HG, kPagedThreads>(p, walk);
+  clear_empty<T>(p);
+  if (run.n == 0) {
+    if (threadIdx.x == 0 && p.joins) p.joins[blockIdx.x].w = 0;
+    return;
+  }
+  const float sc = p.scale * 1.4426950408889634f;
+
+  float q[HG][VN], o[HG][VN], m[HG], l[HG];
+  bool began_before = walk.t > 0, fresh = true;
+  for (int it = 0; it < run.n; ++it) {
+    const int hk = walk.item / hgroups, g0 = walk.item % hgroups * HG;
+    if (fresh) {
+#pragma unroll
+      for (int g = 0; g < HG; ++g) {
+        m[g] = -INFINITY;
+        l[g] = 0.f;
+#pragma unroll
+        for (int e = 0; e < VN; ++e) q[g][e] = o[g][e] = 0.f;
+        if (g0 + g < G && in_head) {
+          const Pack<T, VN> x = ld128(static_cast<const T*>(p.q) + walk.b * p.q_stride_b + static_cast<long long>(hk * G + g0 + g) * c.hd + d0);
+#pragma unroll
+          for (int e = 0; e < VN; ++e) q[g][e] = to_f32(x.v[e]) * sc;
+        }
+      }
+      fresh = false;
+    }
+    const PageMap map = c.map(walk.b);
+    for (int r = 0; r < kPagedTile / kGroups; r += kBatch) {
+      long long row[kBatch];
+      Pack<T, VN> kx[kBatch], vx[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int v = walk.t * kPagedTile + (r + u) * kGroups + grp;
+        row[u] = v < walk.seen.n ? map.row(walk.seen.pos(v), c.Hkv, hk) : -1;
+        if (v < walk.seen.n && row[u] < 0) atomicExch(c.status, kStatusBadPage);
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        kx[u] = vx[u] = Pack<T, VN>{};
+        if (row[u] >= 0 && in_head) {
+          kx[u] = ld128(static_cast<const T*>(c.k_cache) + row[u] * c.hd + d0);
+          vx[u] = ld128(static_cast<const T*>(c.v_cache) + row[u] * c.hd + d0);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < HG; ++g) {
+        if (g0 + g >= G) break;
+        float s[kBatch], top = m[g];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          s[u] = 0.f;
+#pragma unroll
+          for (int e = 0; e < VN; ++e) s[u] = fmaf(q[g][e], to_f32(kx[u].v[e]), s[u]);
+#pragma unroll
+          for (int w = 1; w < L; w <<= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], w);
+          if (row[u] < 0) s[u] = -INFINITY;
+          top = fmaxf(top, s[u]);
+        }
+        const float ref = top == -INFINITY ? 0.f : top;   // nothing seen yet, or scores of -inf
+        const float keep = exp2f(m[g] - ref);
+        m[g] = top;
+        l[g] *= keep;
+#pragma unroll
+        for (int e = 0; e < VN; ++e) o[g][e] *= keep;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const float x = exp2f(s[u] - ref);
+          l[g] += x;
+#pragma unroll
+          for (int e = 0; e < VN; ++e) o[g][e] = fmaf(x, to_f32(vx[u].v[e]), o[g][e]);
+        }
+      }
+    }
+    const bool item_ends = walk.t + 1 == walk.n_tiles;
+    if (item_ends || it + 1 == run.n) {
+#pragma unroll
+      for (int g = 0; g < HG; ++g) {
+        if (lane % L == 0) {
+          sm_m[grp][g] = m[g];
+          sm_l[grp][g] = l[g];
+        }
+#pragma unroll
+        for (int e = 0; e < VN; ++e) sm_o[grp][g][d0 + e] = o[g][e];
+      }
+      if (it + 1 == run.n) note_join(p, run, walk);
+      finish_item<T, HG, kGroups>(p, walk.b, walk.item, item_ends && !began_before, began_before, &sm_o[0][0][0], HG * L * VN, L * VN,
+                                  sm_m, sm_l);
+      began_before = false;
+      fresh = true;
+    }
+    if (it + 1 < run.n) walk.next(p, limit);
+  }
+}
+
+// ---- bf16 heads of 64 and 128: matrix instructions on rows that arrive asynchronously
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+// 16 bytes into shared memory, or 16 zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void load_matrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void load_matrix4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// C[16 x 8] += A[16 x 16] B[16 x 8]
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr int kMmaHeads = 16;    // rows of the matrix instructions: the query heads of an item
+
+template <int HD>
+struct PagedMma {
+  static constexpr int kKeys = 2048 / HD;              // rows of a warp's step: 4 KB of keys and 4 KB of values
+  static constexpr int kTile = 4 * kKeys;              // of a CTA's
+  static constexpr int kStages = 3;
+  static constexpr int kStepBytes = 2 * kKeys * HD * 2;
+  static constexpr int kMeta = 4 * kStages * kStepBytes;
+  static constexpr int kStat = kMeta + 4 * kStages * 16;
+  static constexpr int kSmem = kStat + 2 * 4 * kMmaHeads * 4;
+};
+
+// Each of the four warps takes its quarter of every tile: it copies the rows into a ring of its own (no barrier of the CTA
+// inside an item), multiplies them with the item's queries, keeps its own maximum, sum and output, and meets the others at
+// the item's end.  The rows are swizzled (16-byte unit u of row r at u ^ (r & 7)), so that both the plain and the transposing
+// matrix loads are free of bank conflicts.  UPPER: more than eight query heads in an item.
+template <int HD, bool UPPER>
+__global__ void __launch_bounds__(kPagedThreads) paged_mma_kernel(const PagedArgs p) {
+  using Cfg = PagedMma<HD>;
+  constexpr int KEYS = Cfg::kKeys, STAGES = Cfg::kStages, HG = kMmaHeads;
+  constexpr int kUnits = HD / 8, kRowsPerCopy = 32 / kUnits, kCopies = KEYS / kRowsPerCopy;
+  extern __shared__ __align__(128) uint8_t smem[];
+  dependency_wait();
+  dependents_launch();
+  const CacheArgs& c = p.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int G = c.Hq / c.Hkv, hgroups = (G + HG - 1) / HG, limit = paged_limit(c);
+  uint8_t* ring = smem + warp * STAGES * Cfg::kStepBytes;
+  int4* meta = reinterpret_cast<int4*>(smem + Cfg::kMeta) + warp * STAGES;
+  float(*sm_m)[HG] = reinterpret_cast<float(*)[HG]>(smem + Cfg::kStat);
+  float(*sm_l)[HG] = sm_m + 4;
+
+  TileWalk<Cfg::kTile, HG> ahead;   // runs ahead of the arithmetic
+  const Run run = begin_run<Cfg::kTile, HG, kPagedThreads>(p, ahead);
+  clear_empty<bf16>(p);
+  if (run.n == 0) {
+    if (threadIdx.x == 0 && p.joins) p.joins[blockIdx.x].w = 0;
+    return;
+  }
+  bool began_before = ahead.t > 0;
+
+  // The cache row of this lane's key of the step that is copied next (-1: none), looked up a step early.
+  int row = -1;
+  auto look_up = [&]() {
+    row = -1;
+    const int v = ahead.t * Cfg::kTile + warp * KEYS + lane;
+    if (lane < KEYS && v < ahead.seen.n) {
+      row = static_cast<int>(c.map(ahead.b).row(ahead.seen.pos(v), c.Hkv, ahead.item / hgroups));
+      if (row < 0) atomicExch(c.status, kStatusBadPage);
+    }
+  };
+  int issued = 0;
+  auto copy_step = [&]() {
+    if (issued < run.n) {
+      const int st = issued % STAGES;
+      const uint32_t base = smem_addr(ring + st * Cfg::kStepBytes);
+      const uint32_t real = __ballot_sync(0xffffffffu, row >= 0);
+      if (lane == 0)
+        meta[st] = make_int4(static_cast<int>(real), ahead.b, ahead.item, (ahead.t + 1 == ahead.n_tiles ? 1 : 0) | (ahead.t == 0 ? 2 : 0));
+      if (issued + 1 == run.n) note_join(p, run, ahead);
+      const int u = lane % kUnits;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int r = i * kRowsPerCopy + lane / kUnits;
+        const int src = __shfl_sync(0xffffffffu, row, r);
+        const long long off = static_cast<long long>(max(src, 0)) * HD + u * 8;
+        const uint32_t dst = base + r * HD * 2 + ((u ^ (r & 7)) << 4);
+        copy16(dst, static_cast<const bf16*>(c.k_cache) + off, src >= 0);
+        copy16(dst + KEYS * HD * 2, static_cast<const bf16*>(c.v_cache) + off, src >= 0);
+      }
+      if (++issued < run.n) {
+        ahead.next(p, limit);
+        look_up();
+      }
+    }
+    copy_commit();
+  };
+
+  uint32_t q[HD / 16][4];
+  float o[HD / 8][4];
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  const float sc = p.scale * 1.4426950408889634f;
+  const int gr = lane >> 2, tq = lane & 3;
+
+  look_up();
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) copy_step();
+  bool fresh = true;
+  for (int it = 0; it < run.n; ++it) {
+    copy_wait<STAGES - 2>();
+    __syncwarp();
+    copy_step();   // into the stage that the step before this one has read
+    const int st = it % STAGES;
+    const int4 info = meta[st];
+    const uint32_t real = static_cast<uint32_t>(info.x);
+    if (fresh) {
+      fresh = false;
+      const int hk = info.z / hgroups, g0 = info.z % hgroups * HG;
+      const bf16* src = static_cast<const bf16*>(p.q) + info.y * p.q_stride_b + static_cast<long long>(hk * G + g0) * HD + tq * 2;
+      const bool lo = g0 + gr < G, hi = UPPER && g0 + gr + 8 < G;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        q[k][0] = lo ? *reinterpret_cast<const uint32_t*>(src + gr * HD + k * 16) : 0u;
+        q[k][2] = lo ? *reinterpret_cast<const uint32_t*>(src + gr * HD + k * 16 + 8) : 0u;
+        q[k][1] = hi ? *reinterpret_cast<const uint32_t*>(src + (gr + 8) * HD + k * 16) : 0u;
+        q[k][3] = hi ? *reinterpret_cast<const uint32_t*>(src + (gr + 8) * HD + k * 16 + 8) : 0u;
+      }
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+      m0 = m1 = -INFINITY;
+      l0 = l1 = 0.f;
+    }
+    if (real != 0) {
+      const uint32_t kb = smem_addr(ring + st * Cfg::kStepBytes), vb = kb + KEYS * HD * 2;
+      float s[KEYS / 8][4];
+#pragma unroll
+      for (int n = 0; n < KEYS / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int n = 0; n < KEYS / 16; ++n) {
+        const int r = n * 16 + (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          uint32_t f[4];
+          load_matrix4(f, kb + r * HD * 2 + (((2 * k + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
+          mma16(s[2 * n], q[k], f[0], f[1]);
+          mma16(s[2 * n + 1], q[k], f[2], f[3]);
+        }
+      }
+      // scores in units of log 2; lanes of a quad share a head
+      float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < KEYS / 8; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bool see = real & (1u << (n * 8 + e)) << (2 * tq);
+          s[n][e] = see ? s[n][e] * sc : -INFINITY;
+          t0 = fmaxf(t0, s[n][e]);
+          if (UPPER) {
+            s[n][2 + e] = see ? s[n][2 + e] * sc : -INFINITY;
+            t1 = fmaxf(t1, s[n][2 + e]);
+          }
+        }
+      }
+      t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
+      t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2));
+      if (UPPER) {
+        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
+        t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
+      }
+      if (__any_sync(0xffffffffu, t0 > m0 || (UPPER && t1 > m1))) {
+        const float n0 = fmaxf(m0, t0), a0 = exp2_fast(m0 - (n0 == -INFINITY ? 0.f : n0));
+        float a1 = 1.f;
+        m0 = n0;
+        l0 *= a0;
+        if (UPPER) {
+          const float n1 = fmaxf(m1, t1);
+          a1 = exp2_fast(m1 - (n1 == -INFINITY ? 0.f : n1));
+          m1 = n1;
+          l1 *= a1;
+        }
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d) {
+          o[d][0] *= a0;
+          o[d][1] *= a0;
+          if (UPPER) {
+            o[d][2] *= a1;
+            o[d][3] *= a1;
+          }
+        }
+      }
+      const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+      uint32_t pf[KEYS / 16][4];
+#pragma unroll
+      for (int n = 0; n < KEYS / 8; ++n) {
+        const float x0 = exp2_fast(s[n][0] - r0), x1 = exp2_fast(s[n][1] - r0);
+        l0 += x0 + x1;
+        // the product takes P rounded to bf16; its sum is taken before that
+        pf[n / 2][(n & 1) * 2] = pack_bf16x2(x0, x1);
+        if (UPPER) {
+          const float y0 = exp2_fast(s[n][2] - r1), y1 = exp2_fast(s[n][3] - r1);
+          l1 += y0 + y1;
+          pf[n / 2][(n & 1) * 2 + 1] = pack_bf16x2(y0, y1);
+        } else {
+          pf[n / 2][(n & 1) * 2 + 1] = 0u;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < KEYS / 16; ++n) {
+        const int r = n * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) {
+          uint32_t f[4];
+          load_matrix4_t(f, vb + r * HD * 2 + (((2 * d + (lane >> 4)) ^ (r & 7)) << 4));
+          mma16(o[2 * d], pf[n], f[0], f[1]);
+          mma16(o[2 * d + 1], pf[n], f[2], f[3]);
+        }
+      }
+    }
+    const bool item_ends = info.w & 1;
+    if (item_ends || it + 1 == run.n) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+      if (tq == 0) {
+        sm_m[warp][gr] = m0;
+        sm_l[warp][gr] = l0;
+        sm_m[warp][gr + 8] = m1;
+        sm_l[warp][gr + 8] = l1;
+      }
+      // this warp's sums go where the step's rows were, which it has read; nothing is copied there before the next step
+      __syncwarp();
+      float* sum = reinterpret_cast<float*>(ring + st * Cfg::kStepBytes);
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d) {
+        *reinterpret_cast<float2*>(sum + gr * HD + d * 8 + tq * 2) = make_float2(o[d][0], o[d][1]);
+        if (UPPER) *reinterpret_cast<float2*>(sum + (gr + 8) * HD + d * 8 + tq * 2) = make_float2(o[d][2], o[d][3]);
+      }
+      finish_item<bf16, HG, 4>(p, info.y, info.z, item_ends && !began_before, began_before,
+                               reinterpret_cast<const float*>(smem + st * Cfg::kStepBytes), STAGES * Cfg::kStepBytes / 4, HD, sm_m, sm_l);
+      began_before = false;
+      fresh = true;
+    }
   }
 }
 
 static int cache_check(const TitbCacheDesc* d) {
   if (d->hd <= 0 || d->hd > 128 || d->hd % 8 || d->Hkv <= 0 || d->Hq % d->Hkv || d->page_size <= 0 || d->table_width < 0 ||
-      d->n_pages < 0 || d->sinks < 0 || d->window < 1 || (d->dtype != 0 && d->dtype != 1))
+      d->n_pages < 0 || static_cast<long long>(d->n_pages) * d->Hkv > 0x7fffffffLL / d->page_size || d->sinks < 0 || d->window < 1 || (d->dtype != 0 && d->dtype != 1))
     return TITB_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(d->k_cache) & 15) || (reinterpret_cast<uintptr_t>(d->v_cache) & 15)) return TITB_ERR_ALIGNMENT;
   return 0;
@@ -248,12 +735,35 @@ static int append_launch(const AppendArgs& a, cudaStream_t st) {
   return static_cast<int>(cudaGetLastError());
 }
 
-template <typename T, int L>
-static int paged_launch(const PagedArgs& a, cudaStream_t st) {
-  const int G = a.c.Hq / a.c.Hkv;
-  const dim3 grid(a.c.Hkv * ((G + kPagedHeads - 1) / kPagedHeads), a.c.B);
-  paged_attention_kernel<T, L><<<grid, kPagedWarps * 32, 0, st>>>(a);
-  return static_cast<int>(cudaGetLastError());
+// The grid of the attention over the cache follows what the page table could hold; the work is dealt on the device.
+struct PagedPlan {
+  bool mma, join;
+  int heads, ctas;
+};
+static PagedPlan paged_plan(const TitbCacheDesc* d) {
+  PagedPlan plan{};
+  plan.mma = d->dtype == 1 && (d->hd == 64 || d->hd == 128);
+  plan.heads = plan.mma ? kMmaHeads : kPagedHeads;
+  const int tile = !plan.mma ? kPagedTile : d->hd == 64 ? PagedMma<64>::kTile : PagedMma<128>::kTile;
+  const long long held = static_cast<long long>(d->table_width) * d->page_size, seen = static_cast<long long>(d->window) + d->sinks;
+  const long long tiles = ((held < seen ? held : seen) + tile - 1) / tile;
+  const int G = d->Hq / d->Hkv;
+  const long long items = static_cast<long long>(d->B) * d->Hkv * ((G + plan.heads - 1) / plan.heads);
+  // two CTAs of the matrix kernel fit on an SM (99 KB of shared memory each), four of the other (registers)
+  const long long most = device_sm_count() * (plan.mma ? 2LL : 4LL);
+  plan.ctas = static_cast<int>(tiles == 0 ? 1 : items > most / tiles ? most : items * tiles);
+  plan.join = tiles > 1;   // otherwise every item is one tile
+  return plan;
+}
+static long long plan_slot_floats(const TitbCacheDesc* d, const PagedPlan& plan) { return static_cast<long long>(plan.heads) * (d->hd + 2); }
+
+template <typename K>
+static int paged_launch(K kernel, const PagedArgs& a, const PagedPlan& plan, int smem, cudaStream_t st) {
+  if (smem > 0) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  return static_cast<int>(launch_dependent(kernel, dim3(plan.ctas), dim3(kPagedThreads), smem, st, a));
 }
 
 }  // namespace titb
@@ -282,17 +792,44 @@ TITB_API int titb_cache_append(const TitbCacheDesc* d, const void* qkv, long lon
   return d->dtype == 1 ? append_launch<bf16>(a, st) : append_launch<float>(a, st);
 }
 
+TITB_API long long titb_paged_attention_workspace(const TitbCacheDesc* d) {
+  if (d->B <= 0 || d->Hq <= 0 || cache_check(d)) return 0;
+  const PagedPlan plan = paged_plan(d);
+  return plan.join ? plan.ctas * (2 * plan_slot_floats(d, plan) * 4 + static_cast<long long>(sizeof(int4))) : 0;
+}
+
 TITB_API int titb_paged_attention(const TitbCacheDesc* d, const void* q, long long q_stride_b, const int* lengths, float scale,
-                                  void* o, cudaStream_t st) {
+                                  void* o, void* workspace, cudaStream_t st) {
   (void)cudaGetLastError();
   if (d->B <= 0 || d->Hq <= 0) return 0;
   if (const int rc = cache_check(d)) return rc;
-  if (d->B > 65535) return TITB_ERR_SHAPE;
   auto bad = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
-  if (bad(q) || bad(o) || (q_stride_b & (d->dtype == 1 ? 7 : 3))) return TITB_ERR_ALIGNMENT;
+  if (bad(q) || bad(o) || bad(workspace) || (q_stride_b & (d->dtype == 1 ? 7 : 3))) return TITB_ERR_ALIGNMENT;
+  const PagedPlan plan = paged_plan(d);
   PagedArgs a{};
   a.c = cache_args(d);
   a.q = q; a.q_stride_b = q_stride_b; a.lengths = lengths; a.o = o; a.scale = scale;
-  if (d->dtype == 1) return d->hd <= 64 ? paged_launch<bf16, 8>(a, st) : paged_launch<bf16, 16>(a, st);
-  return d->hd <= 64 ? paged_launch<float, 16>(a, st) : paged_launch<float, 32>(a, st);
+  if (plan.join) {
+    a.joins = static_cast<int4*>(workspace);
+    a.parts = reinterpret_cast<float*>(a.joins + plan.ctas);
+  }
+  int rc;
+  if (plan.mma) {
+    const bool upper = d->Hq / d->Hkv > 8;
+    if (d->hd == 64)
+      rc = upper ? paged_launch(paged_mma_kernel<64, true>, a, plan, PagedMma<64>::kSmem, st)
+                 : paged_launch(paged_mma_kernel<64, false>, a, plan, PagedMma<64>::kSmem, st);
+    else
+      rc = upper ? paged_launch(paged_mma_kernel<128, true>, a, plan, PagedMma<128>::kSmem, st)
+                 : paged_launch(paged_mma_kernel<128, false>, a, plan, PagedMma<128>::kSmem, st);
+  } else if (d->dtype == 1) {
+    rc = d->hd <= 64 ? paged_launch(paged_attention_kernel<bf16, 8>, a, plan, 0, st)
+                     : paged_launch(paged_attention_kernel<bf16, 16>, a, plan, 0, st);
+  } else {
+    rc = d->hd <= 64 ? paged_launch(paged_attention_kernel<float, 16>, a, plan, 0, st)
+                     : paged_launch(paged_attention_kernel<float, 32>, a, plan, 0, st);
+  }
+  if (rc != 0 || !plan.join) return rc;
+  auto join = d->dtype == 0 ? paged_join_kernel<float, kPagedHeads> : plan.mma ? paged_join_kernel<bf16, kMmaHeads> : paged_join_kernel<bf16, kPagedHeads>;
+  return static_cast<int>(launch_dependent(join, dim3(plan.ctas), dim3(128), 0, st, a));
 }
