@@ -19,6 +19,12 @@ void check(int rc, const char* what) {
   TORCH_CHECK(rc == 0, "titb200: ", what, " failed: ", cudaGetErrorString(static_cast<cudaError_t>(rc)));
 }
 
+void forward_only(const char* what, std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : tensors)
+    TORCH_CHECK(!t->requires_grad(), "titb200 ", what, " has no gradient: call it under torch.no_grad()");
+}
+
 // What both operators ask of the cache, on any device.
 void cache_check(const char* what, const Tensor& x, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table,
                  const Tensor& per_seq, int64_t B, int64_t Hq, int64_t Hkv, int64_t hd, int64_t window, int64_t sinks) {
@@ -60,6 +66,7 @@ TitbCacheDesc cache_desc(const Tensor& k_cache, const Tensor& v_cache, const Ten
 
 void append_check(const Tensor& qkv, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& starts,
                   int64_t n_head, int64_t n_kv_head, double theta, const optional<Tensor>& counts, int64_t window, int64_t sinks) {
+  forward_only("cache_append", {&qkv, &k_cache, &v_cache});
   TORCH_CHECK(qkv.dim() == 3, "titb200 cache_append: expects a projection [B, T, (n_head + 2 n_kv_head) * head_dim]");
   TORCH_CHECK(n_head > 0 && n_kv_head > 0 && k_cache.dim() == 4 && qkv.size(2) == (n_head + 2 * n_kv_head) * k_cache.size(3),
               "titb200 cache_append: a projection of width ", qkv.size(2), " does not hold ", n_head, " + 2 * ", n_kv_head,
@@ -73,8 +80,8 @@ void append_check(const Tensor& qkv, const Tensor& k_cache, const Tensor& v_cach
   TORCH_CHECK(qkv.size(1) < INT_MAX, "titb200 cache_append: too many tokens");
 }
 
-// theta == 0: no rotation.  Returns q [B, T, Hq, hd] (undefined without rotation: the caller has it in qkv) and k (when asked).
-std::vector<Tensor> cache_append(const Tensor& qkv_, Tensor& k_cache, Tensor& v_cache, const Tensor& table, const Tensor& starts,
+// theta == 0: no rotation.  Returns q [B, T, Hq, hd], or with return_k the pair of q and k; without rotation views of qkv.
+py::object cache_append(const Tensor& qkv_, Tensor& k_cache, Tensor& v_cache, const Tensor& table, const Tensor& starts,
                                  int64_t n_head, int64_t n_kv_head, double theta, const optional<Tensor>& counts, int64_t window,
                                  int64_t sinks, bool return_k) {
   TORCH_CHECK(qkv_.is_cuda(), "titb200 cache_append: CUDA tensors");
@@ -95,11 +102,21 @@ std::vector<Tensor> cache_append(const Tensor& qkv_, Tensor& k_cache, Tensor& v_
                           counts.has_value() ? counts->data_ptr<int>() : nullptr, theta, q.defined() ? q.data_ptr() : nullptr,
                           k.defined() ? k.data_ptr() : nullptr, at::cuda::getCurrentCUDAStream().stream()),
         "cache_append");
-  return {q, k};
+  if (theta == 0.0) {
+    const auto view = [&](int64_t first, int64_t heads) {
+      return qkv_.as_strided({B, T, heads, hd}, {qkv_.stride(0), qkv_.stride(1), hd * qkv_.stride(2), qkv_.stride(2)},
+                             qkv_.storage_offset() + first * hd * qkv_.stride(2));
+    };
+    q = view(0, n_head);
+    if (return_k) k = view(n_head, n_kv_head);
+  }
+  if (return_k) return py::make_tuple(q, k);
+  return py::cast(q);
 }
 
 void paged_check(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& lengths,
                  int64_t window, int64_t sinks) {
+  forward_only("paged_attention", {&q, &k_cache, &v_cache});
   TORCH_CHECK(q.dim() == 3 && k_cache.dim() == 4, "titb200 paged_attention: q [B, Hq, hd], caches [pages, Hkv, page_size, hd]");
   cache_check("paged_attention", q, k_cache, v_cache, table, lengths, q.size(0), q.size(1), k_cache.size(1), q.size(2), window,
               sinks);

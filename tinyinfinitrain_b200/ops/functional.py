@@ -816,11 +816,6 @@ def window_attention_qkv(qkv, n_head: int, n_kv_head: Optional[int] = None, wind
 
 
 # ----------------------------------------------------------------- paged key-value cache
-def _forward_only(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"titb200 {name} has no gradient: call it under torch.no_grad()")
-
-
 def _cache_row(page_table, b: int, pos: int, page_size: int, n_pages: int) -> int:
     """The page that holds position ``pos`` of sequence b."""
     slot = pos // page_size
@@ -878,18 +873,15 @@ def cache_append(qkv, k_cache, v_cache, page_table, starts, n_head: int, n_kv_he
     Every written position must have a row of its own.  A page number or position outside the cache raises IndexError on the
     CPU; on the GPU it is not followed, and ``parallel.health.check_device_status()`` raises."""
     Hkv = n_kv_head if n_kv_head is not None else n_head
-    _forward_only("cache_append", qkv, k_cache, v_cache)
-    if theta is not None and not theta > 0:
-        raise RuntimeError(f"titb200 cache_append: theta must be positive, got {theta}")
-    args = (qkv, k_cache, v_cache, page_table, starts, n_head, Hkv, theta or 0.0, counts, _window_arg(window), sinks)
-    if not qkv.is_cuda:
-        C.cache_append_check(*args)
-        q, k = cache_append_ref(qkv, k_cache, v_cache, page_table, starts, n_head, Hkv, theta, counts, window, sinks)
-        return (q, k) if return_k else q
-    q, k = C.cache_append(*args, return_k)
     if theta is None:
-        heads = qkv.unflatten(-1, (n_head + 2 * Hkv, k_cache.shape[-1]))
-        q, k = heads[:, :, :n_head], heads[:, :, n_head:n_head + Hkv]
+        theta = 0.0
+    elif not theta > 0:
+        raise RuntimeError(f"titb200 cache_append: theta must be positive, got {theta}")
+    args = (qkv, k_cache, v_cache, page_table, starts, n_head, Hkv, theta, counts, _window_arg(window), sinks)
+    if qkv.is_cuda:
+        return C.cache_append(*args, return_k)
+    C.cache_append_check(*args)
+    q, k = cache_append_ref(qkv, k_cache, v_cache, page_table, starts, n_head, Hkv, theta or None, counts, window, sinks)
     return (q, k) if return_k else q
 
 
@@ -926,12 +918,11 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, window: Optional[i
     A page number or length outside the cache raises IndexError on the CPU; on the GPU it is not followed, and
     ``parallel.health.check_device_status()`` raises."""
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
-    _forward_only("paged_attention", q, k_cache, v_cache)
     args = (q, k_cache, v_cache, page_table, lengths, _window_arg(window), sinks)
-    if not q.is_cuda:
-        C.paged_attention_check(*args)
-        return paged_attention_ref(q, k_cache, v_cache, page_table, lengths, window, sinks, scale)
-    return C.paged_attention(*args, scale)
+    if q.is_cuda:
+        return C.paged_attention(*args, scale)
+    C.paged_attention_check(*args)
+    return paged_attention_ref(q, k_cache, v_cache, page_table, lengths, window, sinks, scale)
 
 
 # -------------------------------------------------------------------- elementwise family
