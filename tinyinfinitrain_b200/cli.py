@@ -29,6 +29,7 @@ def build_parser(family: str) -> argparse.ArgumentParser:
     p.add_argument("--num_iteration", type=int, default=10)
     p.add_argument("--text_length", type=int, default=64)
     p.add_argument("--freq_generate_txt", type=int, default=0)
+    p.add_argument("--kv_cache", action="store_true", help="generate text over a key-value cache instead of re-running the window")
     p.add_argument("--learning_rate", type=float, default=1e-4)
     p.add_argument("--weight_decay", type=float, default=0.0)
     p.add_argument("--max_grad_norm", type=float, default=0.0, help="clip the global gradient norm (0 = off)")
@@ -52,6 +53,8 @@ def build_parser(family: str) -> argparse.ArgumentParser:
     p.add_argument("--n_head", type=int, default=0, help="override the number of attention heads")
     p.add_argument("--n_kv_head", type=int, default=0, help="override the number of key / value heads (LLaMA-3)")
     p.add_argument("--ffn_dim", type=int, default=0, help="override the SwiGLU width (LLaMA-3)")
+    p.add_argument("--attention_window", type=int, default=0, help="attend to the last N positions only (0 = all)")
+    p.add_argument("--attention_sinks", type=int, default=0, help="first positions that stay visible beside --attention_window")
     p.add_argument("--vocab_size", type=int, default=0, help="override the vocabulary size (synthetic data only)")
     p.add_argument("--save", default="", help="checkpoint directory to write at the end (and every --save_every steps)")
     p.add_argument("--save_every", type=int, default=0, help="also checkpoint every N optimizer steps (0 = only at the end)")
@@ -71,7 +74,11 @@ def _config(family: str, args):
     cfg = dataclasses.replace(cfg)
     if args.n_layer:
         cfg.n_layer = args.n_layer
-    for name in ("n_embd", "n_head", "n_kv_head", "ffn_dim"):
+    if args.attention_window < 0 or args.attention_sinks < 0:
+        raise SystemExit("--attention_window and --attention_sinks must not be negative")
+    if args.attention_sinks and not args.attention_window:
+        raise SystemExit("--attention_sinks needs --attention_window")
+    for name in ("n_embd", "n_head", "n_kv_head", "ffn_dim", "attention_window", "attention_sinks"):
         if getattr(args, name) and hasattr(cfg, name):
             setattr(cfg, name, getattr(args, name))
     if args.vocab_size:
@@ -141,6 +148,8 @@ def train_main(family: str, argv=None) -> int:
         cls = GPT2 if family == "gpt2" else LLaMA3
         model = cls.FromLLMC(args.llmc_filepath, device=dev, dtype=dtype) if args.llmc_filepath else \
             cls(cfg, device=dev, dtype=dtype, seed=args.seed)
+        # a checkpoint brings a configuration of its own, which says nothing about the window
+        model.config.attention_window, model.config.attention_sinks = cfg.attention_window, cfg.attention_sinks
         if args.optimizer == "sgd":
             opt = tit.optim.SGD(model.parameters(), args.learning_rate)
         else:
@@ -173,7 +182,7 @@ def train_main(family: str, argv=None) -> int:
                       flush=True)
             log.log(step=step + 1, loss=lossf, lr=lr, **rep)
             if tok is not None and args.freq_generate_txt and (step + 1) % args.freq_generate_txt == 0:
-                tok.GenerateText(model, B, T, args.text_length, dev, stream=sys.stdout)
+                tok.GenerateText(model, B, T, args.text_length, dev, stream=sys.stdout, use_cache=args.kv_cache)
             if args.save and args.save_every and (step + 1) % args.save_every == 0 and step + 1 < args.num_iteration:
                 save_checkpoint(args.save, model, opt, step + 1)
         if args.save:

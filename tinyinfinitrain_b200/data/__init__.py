@@ -94,10 +94,11 @@ class Tokenizer:
 
     @torch.no_grad()
     def GenerateText(self, model, batch_size: int, sequence_length: int, text_length: int, device,
-                     rng_state: int = 1337, stream=None) -> str:
+                     rng_state: int = 1337, stream=None, use_cache: bool = False) -> str:
         """Fills a [batch, seq] window with the end token, writes the prompt "The meaning of life is",
-        then samples one token at a time from row 0 with llm.c's xorshift generator (no KV cache,
-        the whole window is re-run per token, as in the reference)."""
+        then samples one token at a time from row 0 with llm.c's xorshift generator.  The whole window
+        is re-run per token, as in the reference; with ``use_cache`` (the models of this package) the
+        prompt is run once and every token once, over a key-value cache."""
         eot = self.GetEndToken()
         x = torch.full((batch_size, sequence_length), eot, dtype=torch.int64)
         prompt = self._t.Prompt()
@@ -105,11 +106,17 @@ class Tokenizer:
         out = "The meaning of life is"
         state = rng_state
         limit = min(text_length, sequence_length)
+        cache = model.new_cache(1, sequence_length) if use_cache else None
         for t in range(len(prompt), limit):
-            logits = model(x.to(device))
-            if isinstance(logits, (tuple, list)):
-                logits = logits[0]
-            probs = torch.softmax(logits[0, t - 1].float().cpu(), dim=-1)
+            if use_cache:
+                fresh = x[:1, :t] if t == len(prompt) else x[:1, t - 1:t]
+                logits = model(fresh.to(device), cache=cache)[0]
+            else:
+                logits = model(x.to(device))
+                if isinstance(logits, (tuple, list)):
+                    logits = logits[0]
+                logits = logits[0, t - 1]
+            probs = torch.softmax(logits.float().cpu(), dim=-1)
             coin, state = C.random_f32(state)
             tok = C.sample_mult(probs, coin)
             x[0, t] = tok

@@ -35,6 +35,9 @@ class GPT2Config:
     n_head: int = 12
     n_embd: int = 768
     padded_vocab_size: Optional[int] = None
+    # > 0: a token attends to the last attention_window positions and the first attention_sinks ones only
+    attention_window: int = 0
+    attention_sinks: int = 0
 
     def __post_init__(self):
         if self.padded_vocab_size is None:
@@ -62,16 +65,22 @@ class CausalSelfAttention(nn.Module):
     def __init__(self, config: GPT2Config, device=None, dtype=torch.float32):
         super().__init__()
         assert config.n_embd % config.n_head == 0
+        self.config = config
         self.n_head, self.n_embd = config.n_head, config.n_embd
         self.c_attn = nn.Linear(config.n_embd, 3 * config.n_embd, device=device, dtype=dtype)
         self.c_proj = nn.Linear(config.n_embd, config.n_embd, device=device, dtype=dtype)
 
-    def forward(self, x, residual=None):
+    def forward(self, x, residual=None, cache=None, layer: int = 0):
         B, T, Cdim = x.shape
-        H, hd = self.n_head, Cdim // self.n_head
+        H, cfg = self.n_head, self.config
         qkv = self.c_attn(x)  # [B, T, 3C]; q, k, v are read in place by the attention kernel
-        y = ops.causal_attention_qkv(qkv, H).reshape(B, T, Cdim)
-        return self.c_proj(y, residual)
+        if cache is not None:
+            y = cache.attend(layer, qkv, H)
+        elif cfg.attention_window:
+            y = ops.window_attention_qkv(qkv, H, H, cfg.attention_window, cfg.attention_sinks)
+        else:
+            y = ops.causal_attention_qkv(qkv, H)
+        return self.c_proj(y.reshape(B, T, Cdim), residual)
 
 
 class MLP(nn.Module):
@@ -97,9 +106,9 @@ class Block(nn.Module):
         self.ln_2 = nn.LayerNorm(config.n_embd, device=device, dtype=dtype)
         self.mlp = MLP(config, device=device, dtype=dtype)
 
-    def forward(self, x):
+    def forward(self, x, cache=None, layer: int = 0):
         h, x = self.ln_1.fork(x)
-        x = self.attn(h, residual=x)
+        x = self.attn(h, residual=x, cache=cache, layer=layer)
         h, x = self.ln_2.fork(x)
         x = self.mlp(h, residual=x)
         return x
@@ -151,14 +160,45 @@ class GPT2(nn.Module):
             self.transformer["wte"].weight[cfg.vocab_size:].zero_()
 
     # ---- forward ------------------------------------------------------------------------------
-    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, return_logits: bool = True):
+    def new_cache(self, batch: int, max_len: Optional[int] = None, page_size: int = 64) -> nn.PagedKVCache:
+        """An empty cache for ``batch`` sequences of up to ``max_len`` tokens (the model's context by default, and at most)."""
+        cfg, w = self.config, self.lm_head.weight
+        max_len = max_len or cfg.block_size
+        if max_len > cfg.block_size:
+            raise ValueError(f"a cache of {max_len} positions exceeds block size {cfg.block_size}")
+        if (max_len + page_size - 1) // page_size * page_size > cfg.block_size:
+            page_size = math.gcd(page_size, cfg.block_size)     # pages end with the position table
+        return nn.PagedKVCache(cfg.n_layer, batch, max_len, cfg.n_head, cfg.n_embd // cfg.n_head, page_size,
+                               cfg.attention_window or None, cfg.attention_sinks, w.device, w.dtype)
+
+    @torch.no_grad()
+    def _forward_cached(self, idx, cache, counts):
+        tr = self.transformer
+        pos = cache.begin(idx, counts)
+        x = ops.embedding(idx, tr["wte"].weight)
+        # a sequence that outgrows its pages is reported by the cache's kernels; its position must not lead out of the table
+        x = x + ops.embedding(pos.clamp_(max=self.config.block_size - 1), tr["wpe"].weight)
+        for i, block in enumerate(tr["h"]):
+            x = block(x, cache, i)
+        logits = ops.linear(tr["ln_f"](cache.last_rows(x)), self.lm_head.weight)
+        cache.end()
+        return logits[..., :self.config.vocab_size]
+
+    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, return_logits: bool = True, cache=None,
+                counts: Optional[torch.Tensor] = None):
         """``idx``: int64 [B, T].  Without ``targets`` returns logits [B, T, vocab_size].
+        With ``cache`` (``new_cache``) the tokens are appended to it, without gradients, and the logits of the token
+        after them are returned, [B, vocab_size]; ``counts`` (int32 [B]) gives the lengths of prompts that are padded
+        behind to the longest one's.
         With ``targets`` returns ``(logits, loss)``; ``return_logits=False`` takes the fused
         projection + loss path that never materialises a separate gradient tensor and
         returns ``(None, loss)``."""
         cfg = self.config
         B, T = idx.shape
         assert T <= cfg.block_size, f"sequence of length {T} exceeds block size {cfg.block_size}"
+        if cache is not None:
+            assert targets is None, "a cache is for generating text: there is no loss"
+            return self._forward_cached(idx, cache, counts)
         tr = self.transformer
         x = ops.embedding(idx, tr["wte"].weight, tr["wpe"].weight)
         for block in tr["h"]:
@@ -180,6 +220,8 @@ class GPT2(nn.Module):
         """Training FLOPs per token: 6 N for the dense layers plus causal attention."""
         cfg = self.config
         n_dense = sum(p.numel() for n, p in self.named_parameters() if "wpe" not in n)
+        if cfg.attention_window:             # a query sees min(T, window + sinks) positions in the long run
+            T = min(T, 2 * (cfg.attention_window + cfg.attention_sinks))
         return 6.0 * n_dense + 6.0 * cfg.n_layer * cfg.n_embd * T
 
     # ---- llm.c checkpoints (example/gpt2/net.cc:228-377) ------------------------------------------

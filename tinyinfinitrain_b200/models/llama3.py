@@ -33,6 +33,9 @@ class LLaMA3Config:
     ffn_dim: int = 8192
     norm_eps: float = 1e-5
     rope_theta: float = 500000.0
+    # > 0: a token attends to the last attention_window positions and the first attention_sinks ones only
+    attention_window: int = 0
+    attention_sinks: int = 0
 
     @property
     def head_dim(self) -> int:
@@ -55,13 +58,18 @@ class LLaMA3Attention(nn.Module):
         self.c_attn = nn.Linear(cfg.n_embd, (cfg.n_head + 2 * cfg.n_kv_head) * hd, bias=False, device=device, dtype=dtype)
         self.c_proj = nn.Linear(cfg.n_embd, cfg.n_embd, bias=False, device=device, dtype=dtype)
 
-    def forward(self, x, residual=None, pos_offset: int = 0):
+    def forward(self, x, residual=None, pos_offset: int = 0, cache=None, layer: int = 0):
         cfg = self.cfg
         B, T, Cdim = x.shape
         qkv = self.c_attn(x)
+        if cache is not None:
+            return self.c_proj(cache.attend(layer, qkv, cfg.n_head, cfg.rope_theta).reshape(B, T, Cdim), residual)
         qkv = ops.rope_qkv(qkv, cfg.n_head + cfg.n_kv_head, cfg.head_dim, pos_offset, cfg.rope_theta)
-        y = ops.causal_attention_qkv(qkv, cfg.n_head, cfg.n_kv_head).reshape(B, T, Cdim)
-        return self.c_proj(y, residual)
+        if cfg.attention_window:
+            y = ops.window_attention_qkv(qkv, cfg.n_head, cfg.n_kv_head, cfg.attention_window, cfg.attention_sinks)
+        else:
+            y = ops.causal_attention_qkv(qkv, cfg.n_head, cfg.n_kv_head)
+        return self.c_proj(y.reshape(B, T, Cdim), residual)
 
 
 class LLaMA3MLP(nn.Module):
@@ -86,9 +94,9 @@ class LLaMA3Block(nn.Module):
         self.ln_2 = nn.RMSNorm(cfg.n_embd, cfg.norm_eps, device=device, dtype=dtype)
         self.mlp = LLaMA3MLP(cfg, device=device, dtype=dtype)
 
-    def forward(self, x):
+    def forward(self, x, cache=None, layer: int = 0):
         h, x = self.ln_1.fork(x)
-        x = self.attn(h, residual=x)
+        x = self.attn(h, residual=x, cache=cache, layer=layer)
         h, x = self.ln_2.fork(x)
         x = self.mlp(h, residual=x)
         return x
@@ -119,10 +127,34 @@ class LLaMA3(nn.Module):
             else:
                 init.Normal(p, 0.0, 0.02, generator=seed)
 
-    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, return_logits: bool = True):
+    def new_cache(self, batch: int, max_len: Optional[int] = None, page_size: int = 64) -> nn.PagedKVCache:
+        """An empty cache for ``batch`` sequences of up to ``max_len`` tokens (the model's context by default)."""
+        cfg, w = self.config, self.lm_head.weight
+        return nn.PagedKVCache(cfg.n_layer, batch, max_len or cfg.block_size, cfg.n_kv_head, cfg.head_dim, page_size,
+                               cfg.attention_window or None, cfg.attention_sinks, w.device, w.dtype)
+
+    @torch.no_grad()
+    def _forward_cached(self, idx, cache, counts):
+        tr = self.transformer
+        cache.begin(idx, counts)
+        x = ops.embedding(idx, tr["wte"].weight)
+        for i, block in enumerate(tr["h"]):
+            x = block(x, cache, i)
+        logits = ops.linear(tr["ln_f"](cache.last_rows(x)), self.lm_head.weight)
+        cache.end()
+        return logits
+
+    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, return_logits: bool = True, cache=None,
+                counts: Optional[torch.Tensor] = None):
+        """``idx``: int64 [B, T].  With ``cache`` (``new_cache``) the tokens are appended to it, without gradients, and the
+        logits of the token after them are returned, [B, vocab_size]; ``counts`` (int32 [B]) gives the lengths of prompts
+        that are padded behind to the longest one's."""
         cfg = self.config
         B, T = idx.shape
         assert T <= cfg.block_size
+        if cache is not None:
+            assert targets is None, "a cache is for generating text: there is no loss"
+            return self._forward_cached(idx, cache, counts)
         tr = self.transformer
         x = ops.embedding(idx, tr["wte"].weight)
         for block in tr["h"]:
@@ -141,6 +173,8 @@ class LLaMA3(nn.Module):
 
     def flops_per_token(self, T: int) -> float:
         n_dense = sum(p.numel() for n, p in self.named_parameters() if "wte" not in n)
+        if self.config.attention_window:     # a query sees min(T, window + sinks) positions in the long run
+            T = min(T, 2 * (self.config.attention_window + self.config.attention_sinks))
         return 6.0 * n_dense + 6.0 * self.config.n_layer * self.config.n_embd * T
 
     @classmethod

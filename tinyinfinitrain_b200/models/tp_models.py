@@ -112,8 +112,10 @@ def unshard_state_dict(shards, cfg, vocab_rows: int) -> Dict[str, torch.Tensor]:
 class TPAttention(nn.Module):
     kType = "CausalSelfAttention"
 
-    def __init__(self, n_embd, n_head, n_kv_head, comm, bias, rope_theta=None, device=None, dtype=torch.float32):
+    def __init__(self, n_embd, n_head, n_kv_head, comm, bias, rope_theta=None, device=None, dtype=torch.float32, window: int = 0,
+                 sinks: int = 0):
         super().__init__()
+        self.window, self.sinks = window, sinks
         self.hd = n_embd // n_head
         q0, q1 = head_range(n_head, comm.world, comm.rank)
         k0, k1 = head_range(n_kv_head, comm.world, comm.rank)
@@ -128,7 +130,10 @@ class TPAttention(nn.Module):
         qkv = self.c_attn(x_s).view(B, T, -1)
         if self.rope_theta is not None:
             qkv = ops.rope_qkv(qkv, self.hq + self.hk, self.hd, 0, self.rope_theta)
-        y = ops.causal_attention_qkv(qkv, self.hq, self.hk)
+        if self.window:
+            y = ops.window_attention_qkv(qkv, self.hq, self.hk, self.window, self.sinks)
+        else:
+            y = ops.causal_attention_qkv(qkv, self.hq, self.hk)
         return self.c_proj(y.reshape(B * T, self.hq * self.hd), residual_s)
 
 
@@ -168,12 +173,14 @@ class TPBlock(nn.Module):
         if llama:
             self.ln_1 = nn.RMSNorm(cfg.n_embd, cfg.norm_eps, device=device, dtype=dtype)
             self.ln_2 = nn.RMSNorm(cfg.n_embd, cfg.norm_eps, device=device, dtype=dtype)
-            self.attn = TPAttention(cfg.n_embd, cfg.n_head, cfg.n_kv_head, comm, False, cfg.rope_theta, device, dtype)
+            self.attn = TPAttention(cfg.n_embd, cfg.n_head, cfg.n_kv_head, comm, False, cfg.rope_theta, device, dtype,
+                                    cfg.attention_window, cfg.attention_sinks)
             self.mlp = TPLLaMAMLP(cfg.n_embd, cfg.ffn_dim, comm, device, dtype)
         else:
             self.ln_1 = nn.LayerNorm(cfg.n_embd, device=device, dtype=dtype)
             self.ln_2 = nn.LayerNorm(cfg.n_embd, device=device, dtype=dtype)
-            self.attn = TPAttention(cfg.n_embd, cfg.n_head, cfg.n_head, comm, True, None, device, dtype)
+            self.attn = TPAttention(cfg.n_embd, cfg.n_head, cfg.n_head, comm, True, None, device, dtype, cfg.attention_window,
+                                    cfg.attention_sinks)
             self.mlp = TPGPT2MLP(cfg.n_embd, comm, device, dtype)
         for ln in (self.ln_1, self.ln_2):
             for p in ln.parameters():
