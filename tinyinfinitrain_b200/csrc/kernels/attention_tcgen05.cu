@@ -41,6 +41,7 @@ constexpr int kAttnThreads = 192;
 constexpr int kBlk = 128;             // query rows per CTA tile and keys per step
 constexpr int kChunkBytes = kBlk * 128;  // one [128 rows x 64 bf16] swizzled sub-tile
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSinkCols = 16;         // keys of a narrow block of sinks
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -92,15 +93,16 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
 }
 
 // ------------------------------------------------------------------------- forward
-template <int HD>
+template <int HD, bool WIN>
 struct FwdCfg {
+  static constexpr bool kTwin = WIN && HD == 128;   // two CTAs on an SM, P in tensor memory (see below)
   static constexpr int kTileBytes = kBlk * HD * 2;  // Q, K or V tile
-  static constexpr int kStages = 2;
+  static constexpr int kStages = kTwin ? 1 : 2;
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + kTileBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
   static constexpr int kP = kV + kStages * kTileBytes;
-  static constexpr int kBar = kP + kBlk * kBlk * 2;
+  static constexpr int kBar = kP + (kTwin ? 0 : kBlk * kBlk * 2);
   static constexpr int kSmem = kBar + 128;
   static constexpr int kTmemCols = 256;  // S: [0,128)  O_blk: [128, 128+HD)
 };
@@ -123,11 +125,17 @@ struct FwdCfg {
 //
 // WIN: a window and sinks.  The CTA visits the key blocks of the sinks and those from its first query's window to its own; a
 // block on either border of what the rows see is masked by a 128-bit mask per row, built from the row's two ranges of keys.
+// Up to kSinkCols sinks that lie before the window are a block of kSinkCols keys.  At hd 128 (kTwin) the few blocks of a CTA
+// do not hide its set-up and its chain of dependent steps, so two CTAs share the SM: K and V in one stage each, P in tensor
+// memory over S as the A operand of P V, which leaves 96 KB of shared memory to a CTA.  S(j+1) is then issued behind P(j) V(j):
+// the other CTA's products fill the gap.  Measured: TODO
 template <int HD, bool WIN>
-__global__ void __launch_bounds__(kAttnThreads, (HD == 64) ? 2 : 1)
+__global__ void __launch_bounds__(kAttnThreads, (HD == 64 || WIN) ? 2 : 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                 const __grid_constant__ CUtensorMap tv, const AttnArgs p) {
-  using Cfg = FwdCfg<HD>;
+  using Cfg = FwdCfg<HD, WIN>;
+  constexpr int S = Cfg::kStages;
+  constexpr bool kTwin = Cfg::kTwin;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBar);
   uint64_t* q_full = bars;          // 1
@@ -151,6 +159,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   const int first_blk = WIN ? max(0, q0 - p.window + 1) / kBlk : 0;                         // of the window
   const int n_sink_blk = WIN ? min((p.sinks + kBlk - 1) / kBlk, first_blk) : 0;
   const int nblk = n_sink_blk + qb - first_blk + 1;
+  const bool narrow = WIN && n_sink_blk == 1 && p.sinks <= kSinkCols;   // the sinks' block is kSinkCols wide
   auto key0 = [&](int j) { return (WIN ? (j < n_sink_blk ? j : first_blk + j - n_sink_blk) : j) * kBlk; };
 
   if (threadIdx.x == 0) {
@@ -191,14 +200,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       for (int c = 0; c < HD / 64; ++c)
         ptx::tma_load_3d(smem + Cfg::kQ + c * kChunkBytes, &tq, q_full, h * HD + c * 64, q0, b);
       for (int j = 0; j < nblk; ++j) {
-        const int st = j & 1;
-        if (!ptx::mbar_wait(&k_empty[st], ((j >> 1) & 1) ^ 1u, abort_flag)) break;
+        const int st = j % S;
+        if (!ptx::mbar_wait(&k_empty[st], ((j / S) & 1) ^ 1u, abort_flag)) break;
         ptx::mbar_expect_tx(&k_full[st], Cfg::kTileBytes);
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c)
           ptx::tma_load_3d(smem + Cfg::kK + st * Cfg::kTileBytes + c * kChunkBytes, &tk, &k_full[st], hk * HD + c * 64,
                            key0(j), b);
-        if (!ptx::mbar_wait(&v_empty[st], ((j >> 1) & 1) ^ 1u, abort_flag)) break;
+        if (!ptx::mbar_wait(&v_empty[st], ((j / S) & 1) ^ 1u, abort_flag)) break;
         ptx::mbar_expect_tx(&v_full[st], Cfg::kTileBytes);
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c)
@@ -210,6 +219,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
     if (ptx::elect_one()) {
       const uint32_t idesc_s = ptx::make_idesc_bf16(128, 128, 0, 0);
       const uint32_t idesc_o = ptx::make_idesc_bf16(128, HD, 0, 1);
+      const uint32_t idesc_sink = ptx::make_idesc_bf16(128, kSinkCols, 0, 0);
       const uint32_t q_base = ptx::smem_u32(smem + Cfg::kQ);
       const uint32_t p_base = ptx::smem_u32(smem + Cfg::kP);
       const uint64_t q_desc = ptx::make_smem_desc(q_base, 16, 1024);
@@ -217,14 +227,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       const uint64_t p_desc = ptx::make_smem_desc(p_base, 16, 1024);
       const uint64_t v_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + Cfg::kV), kChunkBytes, 1024);
       auto issue_s = [&](int j) {
-        const uint64_t k_desc = desc_add(k_desc0, (j & 1) * Cfg::kTileBytes);
+        const uint64_t k_desc = desc_add(k_desc0, (j % S) * Cfg::kTileBytes);
+        const uint32_t idesc = WIN && narrow && j == 0 ? idesc_sink : idesc_s;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const uint32_t off = (k >> 2) * kChunkBytes + (k & 3) * 32;
-          ptx::mma_f16_ss(tS, desc_add(q_desc, off), desc_add(k_desc, off), idesc_s, k > 0);
+          ptx::mma_f16_ss(tS, desc_add(q_desc, off), desc_add(k_desc, off), idesc, k > 0);
         }
         ptx::tc_commit(s_full);
-        ptx::tc_commit(&k_empty[j & 1]);   // the K tile may be refilled once this product has finished
+        ptx::tc_commit(&k_empty[j % S]);   // the K tile may be refilled once this product has finished
       };
       bool ok = ptx::mbar_wait(q_full, 0, abort_flag) && ptx::mbar_wait(&k_full[0], 0, abort_flag);
       if (ok) {
@@ -232,24 +243,35 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         issue_s(0);
       }
       for (int j = 0; j < nblk && ok; ++j) {
-        if (j + 1 < nblk) {
+        if (!kTwin && j + 1 < nblk) {
           // S(j+1) goes into the score columns as soon as S(j) has been copied to registers
-          if (!ptx::mbar_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, abort_flag)) break;
+          if (!ptx::mbar_wait(&k_full[(j + 1) % S], ((j + 1) / S) & 1, abort_flag)) break;
           if (!ptx::mbar_wait(s_free, j & 1, abort_flag)) break;
           ptx::tc_fence_after_sync();
           issue_s(j + 1);
         }
-        if (!ptx::mbar_wait(&v_full[j & 1], (j >> 1) & 1, abort_flag)) break;
+        if (!ptx::mbar_wait(&v_full[j % S], (j / S) & 1, abort_flag)) break;
         if (!ptx::mbar_wait(p_full, j & 1, abort_flag)) break;
         ptx::tc_fence_after_sync();
-        const uint64_t v_desc = desc_add(v_desc0, (j & 1) * Cfg::kTileBytes);
+        const uint64_t v_desc = desc_add(v_desc0, (j % S) * Cfg::kTileBytes);
+        const int steps = WIN && narrow && j == 0 ? kSinkCols / 16 : kBlk / 16;
 #pragma unroll
         for (int k = 0; k < kBlk / 16; ++k) {
+          if (WIN && k >= steps) break;
           const uint32_t a_off = (k >> 2) * kChunkBytes + (k & 3) * 32;
-          ptx::mma_f16_ss(tO, desc_add(p_desc, a_off), desc_add(v_desc, k * 2048), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+          if constexpr (kTwin)
+            ptx::mma_f16_ts(tO, tS + k * 8, desc_add(v_desc, k * 2048), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+          else
+            ptx::mma_f16_ss(tO, desc_add(p_desc, a_off), desc_add(v_desc, k * 2048), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
         }
         ptx::tc_commit(o_full);
-        ptx::tc_commit(&v_empty[j & 1]);
+        ptx::tc_commit(&v_empty[j % S]);
+        if (kTwin && j + 1 < nblk) {
+          // products run in the order of their issue: P(j) V(j) has read P before S(j+1) takes its columns
+          if (!ptx::mbar_wait(&k_full[(j + 1) % S], ((j + 1) / S) & 1, abort_flag)) break;
+          ptx::tc_fence_after_sync();
+          issue_s(j + 1);
+        }
       }
     }
   } else {
@@ -265,6 +287,46 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
     for (int j = 0; j < nblk; ++j) {
       if (!ptx::mbar_wait_warp(s_full, j & 1, abort_flag)) { ok = false; break; }
       ptx::tc_fence_after_sync();
+      if (WIN && narrow && j == 0) {
+        // the sinks: all of them lie before the rows' windows
+        uint32_t r[16], pk[16];
+        ptx::tmem_ld16(tS + lane_sel, r);
+        ptx::tmem_ld_wait();
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (!kTwin && lane == 0) ptx::mbar_arrive(s_free);
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < kSinkCols; ++e) {
+          if (e >= p.sinks) r[e] = __float_as_uint(-INFINITY);
+          top = fmaxf(top, __uint_as_float(r[e]));
+        }
+        m_ref = top * sc;
+        const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
+        float rs0 = 0.f, rs1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < kSinkCols; e += 2) {
+          const float p0 = ex2(fmaf(__uint_as_float(r[e]), sc, neg)), p1 = ex2(fmaf(__uint_as_float(r[e + 1]), sc, neg));
+          rs0 += p0;
+          rs1 += p1;
+          pk[e >> 1] = pack_bf16x2(p0, p1);
+          pk[8 + (e >> 1)] = 0u;
+        }
+        l += rs0 + rs1;
+        if constexpr (kTwin) {
+          ptx::tmem_st16(tS + lane_sel, pk);
+          ptx::tmem_st_wait();
+        } else {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            *reinterpret_cast<uint4*>(p_smem + swz_off(row, u)) = make_uint4(pk[u * 4], pk[u * 4 + 1], pk[u * 4 + 2], pk[u * 4 + 3]);
+          ptx::fence_proxy_async_smem();
+        }
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(p_full);
+        continue;
+      }
       uint32_t r0[32], r1[32], r2[32], r3[32];
       ptx::tmem_ld32(tS + lane_sel + 0, r0);
       ptx::tmem_ld32(tS + lane_sel + 32, r1);
@@ -273,7 +335,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       ptx::tmem_ld_wait();
       ptx::tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(s_free);   // the score columns may be overwritten by S(j+1)
+      if (!kTwin && lane == 0) ptx::mbar_arrive(s_free);   // the score columns may be overwritten by S(j+1)
       const int kv0 = key0(j);
       if (WIN) {
         // a block before the rows' own in which the last row's window does not begin yet, or that lies among the sinks: whole
@@ -312,14 +374,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         mx3 = max3(mx3, __uint_as_float(r3[e]), __uint_as_float(r3[e + 1]));
       }
       const float m_blk = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sc;
-      bool waited_o = (j == 0);
+      bool waited_o = kTwin || j == 0;   // kTwin: S(j) was issued behind the product before
       if (j == 0) {
         m_ref = m_blk;
       } else {
         const bool need = m_blk > m_ref + kLazy;
         if (__any_sync(0xffffffffu, need)) {
           // the previous P V product must have landed before O is rescaled in place
-          if (!ptx::mbar_wait_warp(o_full, (j - 1) & 1, abort_flag)) { ok = false; break; }
+          if (!waited_o && !ptx::mbar_wait_warp(o_full, (j - 1) & 1, abort_flag)) { ok = false; break; }
           ptx::tc_fence_after_sync();
           waited_o = true;
           const float alpha = need ? ex2(m_ref - m_blk) : 1.f;
@@ -354,6 +416,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           // P(j-1) V(j-1) must have finished reading the P buffer before it is overwritten
           if (!ptx::mbar_wait_warp(o_full, (j - 1) & 1, abort_flag)) ok = false;
         }
+        if constexpr (kTwin) {
+          ptx::tmem_st16(tS + lane_sel + c * 16, pk);
+          return;
+        }
 #pragma unroll
         for (int u = 0; u < 4; ++u)
           *reinterpret_cast<uint4*>(p_smem + swz_off(row, c * 4 + u)) =
@@ -365,7 +431,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       exp_chunk(r2, 2);
       exp_chunk(r3, 3);
       l += rs0 + rs1;
-      ptx::fence_proxy_async_smem();
+      if constexpr (kTwin) ptx::tmem_st_wait();
+      else ptx::fence_proxy_async_smem();
       ptx::tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(p_full);
@@ -956,7 +1023,7 @@ static bool attn_check(const TitbAttnDesc* d) {
 
 template <int HD, bool WIN = false>
 static int attn_fwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 0, int sinks = 0) {
-  using Cfg = FwdCfg<HD>;
+  using Cfg = FwdCfg<HD, WIN>;
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
