@@ -84,7 +84,7 @@ void window_check(const Tensor& q, const Tensor& k, const Tensor& v, int64_t win
               "titb200 window_attention: only float32 and bfloat16 tensors are supported, got ", q.scalar_type());
   TORCH_CHECK(q.size(3) > 0 && q.size(3) <= 128 && q.size(3) % 8 == 0,
               "titb200 window_attention: head_dim must be a multiple of 8 up to 128, got ", q.size(3));
-  TORCH_CHECK(q.size(1) <= 64 * 65535LL && q.size(0) * q.size(2) < (1LL << 31), "titb200 window_attention: too many tokens or heads");
+  TORCH_CHECK(q.size(1) <= 32 * 32767LL && q.size(0) * q.size(2) < (1LL << 31), "titb200 window_attention: too many tokens or heads");
 }
 
 // Elements between the tokens of a [B, T, H, hd] view, taken from a dimension that has more than one entry.

@@ -22,17 +22,23 @@ int window_tc_fwd(const TitbAttnDesc* d, int window, int sinks, cudaStream_t st)
 int window_tc_bwd(const TitbAttnDesc* d, int window, int sinks, float* sink_part, cudaStream_t st);
 long long window_tc_sink_floats(const TitbAttnDesc* d, int window, int sinks);
 
-constexpr int kWinThreads = 256;   // 16 x 16 threads over a tile
-constexpr int kWinRows = 64;       // rows of the tile that a CTA owns
-constexpr int kWinPitch = kWinRows + 4;
+constexpr int kWinThreads = 128;   // 8 x 16 threads of 4 x 4 scores
+constexpr int kWinRows = 32;       // rows of the tile that a CTA owns
+constexpr int kWinStep = 64;       // rows of the other operand that arrive at a time
+// pitches of the transposed tiles [HD][rows]: rows stay 16-byte aligned and neighbouring heads' elements 4 banks apart
+constexpr int kRowPitch = kWinRows + 4, kStepPitch = kWinStep + 4;
 
 struct WinArgs {
   const void *q, *k, *v, *d_o;
   void *o, *dq, *dk, *dv;
   float *lse, *delta;
-  int T, Hq, Hkv, hd, window, sinks;
+  int B, T, Hq, Hkv, hd, window, sinks;
   float scale;
   long long q_st, k_st, v_st, o_st, do_st, dq_st, dk_st, dv_st;   // elements between tokens
+  // key tiles that hold sinks, the query steps that one of their CTAs takes, the CTAs of a tile, and their sums, fp32
+  // [parts][B][sink_tiles][Hkv][dK, dV][kWinRows][hd]
+  int sink_tiles, sink_step, sink_parts;
+  float* sink_part;
 };
 
 __device__ __forceinline__ bool win_visible(int i, int j, int window, int sinks) {
@@ -55,33 +61,20 @@ __device__ __forceinline__ float4 load4(const T* base, long long t, long long st
   }
   return r;
 }
-template <typename T>
-__device__ __forceinline__ void store4(T* p, float4 r) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = r;
-  } else {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(r.x, r.y), pack_bf16x2(r.z, r.w));
-  }
-}
 
-// ROWS rows from row t0 on into shared memory: transposed ([HD][pitch], one row's element d at tr[d * pitch + row]) and / or
-// as they are ([ROWS][HD + 4]).
-template <typename T, int HD, int ROWS, bool TR, bool RM>
-__device__ __forceinline__ void load_tile(const T* base, long long stride, int t0, int n_rows, int hd, float* tr, int pitch,
-                                          float* rm) {
-  constexpr int kVecs = HD / 4;
-  for (int i = threadIdx.x; i < ROWS * kVecs; i += kWinThreads) {
-    // eight lanes along the head, four rows: whole 128-byte segments of fp32 rows
+// ROWS rows from row t0 on, transposed, into shared memory: element d of a row at tile[d * pitch + row].  Two lanes take 32
+// bytes of a row and sixteen rows share a warp, which makes whole sectors of the loads and 32 banks of the stores.
+template <typename T, int HD, int ROWS>
+__device__ __forceinline__ void load_tile(const T* base, long long stride, int t0, int n_rows, int hd, float* tile, int pitch) {
+#pragma unroll 8
+  for (int i = threadIdx.x; i < ROWS * HD / 4; i += kWinThreads) {
     const int lane = i & 31, grp = i >> 5;
-    const int d = ((grp % (kVecs / 8)) * 8 + (lane & 7)) * 4, r = (grp / (kVecs / 8)) * 4 + (lane >> 3);
+    const int r = grp % (ROWS / 16) * 16 + (lane >> 1), d = (grp / (ROWS / 16) * 2 + (lane & 1)) * 4;
     const float4 x = load4(base, t0 + r, stride, d, n_rows, hd);
-    if (TR) {
-      tr[d * pitch + r] = x.x;
-      tr[(d + 1) * pitch + r] = x.y;
-      tr[(d + 2) * pitch + r] = x.z;
-      tr[(d + 3) * pitch + r] = x.w;
-    }
-    if (RM) *reinterpret_cast<float4*>(rm + r * (HD + 4) + d) = x;
+    tile[d * pitch + r] = x.x;
+    tile[(d + 1) * pitch + r] = x.y;
+    tile[(d + 2) * pitch + r] = x.z;
+    tile[(d + 3) * pitch + r] = x.w;
   }
 }
 
@@ -96,25 +89,72 @@ __device__ __forceinline__ float half_warp_sum(float v) {
   return v;
 }
 
-__device__ __forceinline__ void fma4(float (&acc)[4], float a, float4 b) {
-  acc[0] = fmaf(a, b.x, acc[0]);
-  acc[1] = fmaf(a, b.y, acc[1]);
-  acc[2] = fmaf(a, b.z, acc[2]);
-  acc[3] = fmaf(a, b.w, acc[3]);
+// acc[r][c] += a[r] . b[c] over the head: rows ty * 4 of the owned tile, rows tx * 4 of the step's.
+template <int HD>
+__device__ __forceinline__ void scores(float (&acc)[4][4], const float* own, const float* step, int ty, int tx) {
+#pragma unroll 8
+  for (int d = 0; d < HD; ++d) {
+    const float4 a = *reinterpret_cast<const float4*>(own + d * kRowPitch + ty * 4);
+    const float4 b = *reinterpret_cast<const float4*>(step + d * kStepPitch + tx * 4);
+    const float ar[4] = {a.x, a.y, a.z, a.w}, bc[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[r][c] = fmaf(ar[r], bc[c], acc[r][c]);
+  }
+}
+// w ([step row][own row]) <- s
+__device__ __forceinline__ void store_weights(float* w, const float (&s)[4][4], int ty, int tx) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<float4*>(w + (tx * 4 + c) * kRowPitch + ty * 4) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
+}
+// acc[r][i] += sum over the step's rows n of w[n][own row ty * 4 + r] times element tx + 16 i of row n: the elements are read
+// four rows at a time from the transposed tile.
+template <int HD>
+__device__ __forceinline__ void accumulate(float (&acc)[4][HD / 16], const float* w, const float* step, int ty, int tx) {
+#pragma unroll 2
+  for (int n = 0; n < kWinStep; n += 4) {
+    float4 a[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a[k] = *reinterpret_cast<const float4*>(w + (n + k) * kRowPitch + ty * 4);
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(step + (tx + 16 * i) * kStepPitch + n);
+      const float xk[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        acc[0][i] = fmaf(a[k].x, xk[k], acc[0][i]);
+        acc[1][i] = fmaf(a[k].y, xk[k], acc[1][i]);
+        acc[2][i] = fmaf(a[k].z, xk[k], acc[2][i]);
+        acc[3][i] = fmaf(a[k].w, xk[k], acc[3][i]);
+      }
+    }
+  }
+}
+template <typename T, int HD>
+__device__ __forceinline__ void store_rows(T* base, long long stride, int t0, int n_rows, int hd, const float (&acc)[4][HD / 16],
+                                           int ty, int tx) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (t0 + ty * 4 + r < n_rows)
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i)
+        if (tx + 16 * i < hd) base[(t0 + ty * 4 + r) * stride + tx + 16 * i] = from_f32<T>(acc[r][i]);
 }
 
 template <int HD>
 struct WinFwdSmem {
-  static constexpr int kQ = 0, kK = kQ + HD * kWinPitch, kV = kK + HD * kWinPitch, kP = kV + 64 * (HD + 4);
-  static constexpr int kBytes = (kP + 64 * kWinPitch) * 4;
+  static constexpr int kQ = 0, kK = kQ + HD * kRowPitch, kV = kK + HD * kStepPitch, kP = kV + HD * kStepPitch;
+  static constexpr int kBytes = (kP + kWinStep * kRowPitch) * 4;
 };
 
-// One CTA per 64 queries of a head.  A thread holds 4 x 4 scores and 4 rows x HD / 16 columns of the output.
+// One CTA per 32 queries of a head.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p) {
   using Sm = WinFwdSmem<HD>;
   extern __shared__ __align__(16) float sm[];
-  float *Qt = sm + Sm::kQ, *Kt = sm + Sm::kK, *V = sm + Sm::kV, *Pt = sm + Sm::kP;
+  float *Qt = sm + Sm::kQ, *Kt = sm + Sm::kK, *Vt = sm + Sm::kV, *Pt = sm + Sm::kP;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int h = blockIdx.x % p.Hq, b = blockIdx.x / p.Hq, hk = h / (p.Hq / p.Hkv);
   const int q0 = (gridDim.y - 1 - blockIdx.y) * kWinRows;
@@ -123,28 +163,23 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
   const T* k = static_cast<const T*>(p.k) + row0 * p.k_st + hk * p.hd;
   const T* v = static_cast<const T*>(p.v) + row0 * p.v_st + hk * p.hd;
 
-  load_tile<T, HD, kWinRows, true, false>(q, p.q_st, q0, p.T, p.hd, Qt, kWinPitch, nullptr);
+  load_tile<T, HD, kWinRows>(q, p.q_st, q0, p.T, p.hd, Qt, kRowPitch);
   float acc[4][HD / 16] = {};
   float m[4], l[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
 
-  const int first = max(0, q0 - p.window + 1) / 64, last = min(q0 + kWinRows, p.T) - 1;
-  const int sink_tiles = min((p.sinks + 63) / 64, first);
-  const int n_tiles = sink_tiles + last / 64 - first + 1;
-  for (int it = 0; it < n_tiles; ++it) {
-    const int k0 = (it < sink_tiles ? it : first + it - sink_tiles) * 64;
+  const int first = max(0, q0 - p.window + 1) / kWinStep, last = min(q0 + kWinRows, p.T) - 1;
+  const int sink_steps = min((p.sinks + kWinStep - 1) / kWinStep, first);
+  const int n_steps = sink_steps + last / kWinStep - first + 1;
+  for (int it = 0; it < n_steps; ++it) {
+    const int k0 = (it < sink_steps ? it : first + it - sink_steps) * kWinStep;
     __syncthreads();
-    load_tile<T, HD, 64, true, false>(k, p.k_st, k0, p.T, p.hd, Kt, kWinPitch, nullptr);
-    load_tile<T, HD, 64, false, true>(v, p.v_st, k0, p.T, p.hd, nullptr, 0, V);
+    load_tile<T, HD, kWinStep>(k, p.k_st, k0, p.T, p.hd, Kt, kStepPitch);
+    load_tile<T, HD, kWinStep>(v, p.v_st, k0, p.T, p.hd, Vt, kStepPitch);
     __syncthreads();
     float s[4][4] = {};
-#pragma unroll 8
-    for (int d = 0; d < HD; ++d) {
-      const float4 a = *reinterpret_cast<const float4*>(Qt + d * kWinPitch + ty * 4);
-      const float4 c = *reinterpret_cast<const float4*>(Kt + d * kWinPitch + tx * 4);
-      fma4(s[0], a.x, c); fma4(s[1], a.y, c); fma4(s[2], a.z, c); fma4(s[3], a.w, c);
-    }
+    scores<HD>(s, Qt, Kt, ty, tx);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = q0 + ty * 4 + r;
@@ -155,7 +190,7 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
         top = fmaxf(top, s[r][c]);
       }
       top = fmaxf(m[r], half_warp_max(top));
-      const float ref = top == -INFINITY ? 0.f : top;       // a row may see nothing of its first tiles
+      const float ref = top == -INFINITY ? 0.f : top;       // a row may see nothing of its first steps
       const float keep = expf(m[r] - ref);
       float sum = 0.f;
 #pragma unroll
@@ -166,58 +201,36 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
       l[r] = l[r] * keep + half_warp_sum(sum);
       m[r] = top;
 #pragma unroll
-      for (int c = 0; c < HD / 16; ++c) acc[r][c] *= keep;
+      for (int i2 = 0; i2 < HD / 16; ++i2) acc[r][i2] *= keep;
     }
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      *reinterpret_cast<float4*>(Pt + (tx * 4 + c) * kWinPitch + ty * 4) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
+    store_weights(Pt, s, ty, tx);
     __syncthreads();
-#pragma unroll 4
-    for (int n = 0; n < 64; ++n) {
-      const float4 a = *reinterpret_cast<const float4*>(Pt + n * kWinPitch + ty * 4);
-#pragma unroll
-      for (int c = 0; c < HD / 64; ++c) {
-        const float4 x = *reinterpret_cast<const float4*>(V + n * (HD + 4) + c * 64 + tx * 4);
-        fma4(*reinterpret_cast<float(*)[4]>(&acc[0][c * 4]), a.x, x);
-        fma4(*reinterpret_cast<float(*)[4]>(&acc[1][c * 4]), a.y, x);
-        fma4(*reinterpret_cast<float(*)[4]>(&acc[2][c * 4]), a.z, x);
-        fma4(*reinterpret_cast<float(*)[4]>(&acc[3][c * 4]), a.w, x);
-      }
-    }
+    accumulate<HD>(acc, Pt, Vt, ty, tx);
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int i = q0 + ty * 4 + r;
-    if (i >= p.T) continue;
     const float inv = 1.f / l[r];
-    T* o = static_cast<T*>(p.o) + (row0 + i) * p.o_st + h * p.hd;
 #pragma unroll
-    for (int c = 0; c < HD / 64; ++c) {
-      const int d = c * 64 + tx * 4;
-      if (d < p.hd)
-        store4(o + d, make_float4(acc[r][c * 4] * inv, acc[r][c * 4 + 1] * inv, acc[r][c * 4 + 2] * inv, acc[r][c * 4 + 3] * inv));
-    }
-    if (tx == 0) p.lse[(static_cast<long long>(b) * p.Hq + h) * p.T + i] = m[r] + logf(l[r]);
+    for (int c = 0; c < HD / 16; ++c) acc[r][c] *= inv;
+    if (tx == 0 && i < p.T) p.lse[(static_cast<long long>(b) * p.Hq + h) * p.T + i] = m[r] + logf(l[r]);
   }
+  store_rows<T, HD>(static_cast<T*>(p.o) + row0 * p.o_st + h * p.hd, p.o_st, q0, p.T, p.hd, acc, ty, tx);
 }
-
-// The other operand's rows arrive 32 at a time in the backward kernels.
-constexpr int kWinStep = 32;
-constexpr int kWinStepPitch = kWinStep + 4;
 
 template <int HD>
 struct WinDqSmem {
-  static constexpr int kQ = 0, kDO = kQ + HD * kWinPitch, kK = kDO + HD * kWinPitch, kV = kK + HD * kWinStepPitch,
-                       kKr = kV + HD * kWinStepPitch, kDS = kKr + kWinStep * (HD + 4);
-  static constexpr int kBytes = (kDS + kWinStep * kWinPitch) * 4;
+  static constexpr int kQ = 0, kDO = kQ + HD * kRowPitch, kK = kDO + HD * kRowPitch, kV = kK + HD * kStepPitch,
+                       kDS = kV + HD * kStepPitch;
+  static constexpr int kBytes = (kDS + kWinStep * kRowPitch) * 4;
 };
 
-// One CTA per 64 queries of a head: delta, then dQ.
+// One CTA per 32 queries of a head: delta, then dQ.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p) {
   using Sm = WinDqSmem<HD>;
   extern __shared__ __align__(16) float sm[];
-  float *Qt = sm + Sm::kQ, *Dt = sm + Sm::kDO, *Kt = sm + Sm::kK, *Vt = sm + Sm::kV, *Kr = sm + Sm::kKr, *St = sm + Sm::kDS;
+  float *Qt = sm + Sm::kQ, *Dt = sm + Sm::kDO, *Kt = sm + Sm::kK, *Vt = sm + Sm::kV, *St = sm + Sm::kDS;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int h = blockIdx.x % p.Hq, b = blockIdx.x / p.Hq, hk = h / (p.Hq / p.Hkv);
   const int q0 = (gridDim.y - 1 - blockIdx.y) * kWinRows;
@@ -229,8 +242,8 @@ __global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p)
   const T* o = static_cast<const T*>(p.o) + row0 * p.o_st + h * p.hd;
   const long long stat0 = (static_cast<long long>(b) * p.Hq + h) * p.T;
 
-  load_tile<T, HD, kWinRows, true, false>(q, p.q_st, q0, p.T, p.hd, Qt, kWinPitch, nullptr);
-  load_tile<T, HD, kWinRows, true, false>(d_o, p.do_st, q0, p.T, p.hd, Dt, kWinPitch, nullptr);
+  load_tile<T, HD, kWinRows>(q, p.q_st, q0, p.T, p.hd, Qt, kRowPitch);
+  load_tile<T, HD, kWinRows>(d_o, p.do_st, q0, p.T, p.hd, Dt, kRowPitch);
   float lse[4], delta[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -247,178 +260,142 @@ __global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p)
   }
   float acc[4][HD / 16] = {};
   const int first = max(0, q0 - p.window + 1) / kWinStep, last = min(q0 + kWinRows, p.T) - 1;
-  const int sink_tiles = min((p.sinks + kWinStep - 1) / kWinStep, first);
-  const int n_tiles = sink_tiles + last / kWinStep - first + 1;
-  for (int it = 0; it < n_tiles; ++it) {
-    const int k0 = (it < sink_tiles ? it : first + it - sink_tiles) * kWinStep;
+  const int sink_steps = min((p.sinks + kWinStep - 1) / kWinStep, first);
+  const int n_steps = sink_steps + last / kWinStep - first + 1;
+  for (int it = 0; it < n_steps; ++it) {
+    const int k0 = (it < sink_steps ? it : first + it - sink_steps) * kWinStep;
     __syncthreads();
-    load_tile<T, HD, kWinStep, true, true>(k, p.k_st, k0, p.T, p.hd, Kt, kWinStepPitch, Kr);
-    load_tile<T, HD, kWinStep, true, false>(v, p.v_st, k0, p.T, p.hd, Vt, kWinStepPitch, nullptr);
+    load_tile<T, HD, kWinStep>(k, p.k_st, k0, p.T, p.hd, Kt, kStepPitch);
+    load_tile<T, HD, kWinStep>(v, p.v_st, k0, p.T, p.hd, Vt, kStepPitch);
     __syncthreads();
-    float s[4][2] = {}, dp[4][2] = {};
-#pragma unroll 8
-    for (int d = 0; d < HD; ++d) {
-      const float4 a = *reinterpret_cast<const float4*>(Qt + d * kWinPitch + ty * 4);
-      const float4 g = *reinterpret_cast<const float4*>(Dt + d * kWinPitch + ty * 4);
-      const float2 x = *reinterpret_cast<const float2*>(Kt + d * kWinStepPitch + tx * 2);
-      const float2 y = *reinterpret_cast<const float2*>(Vt + d * kWinStepPitch + tx * 2);
-      const float ar[4] = {a.x, a.y, a.z, a.w}, gr[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[r][0] = fmaf(ar[r], x.x, s[r][0]);
-        s[r][1] = fmaf(ar[r], x.y, s[r][1]);
-        dp[r][0] = fmaf(gr[r], y.x, dp[r][0]);
-        dp[r][1] = fmaf(gr[r], y.y, dp[r][1]);
-      }
-    }
+    float s[4][4] = {}, dp[4][4] = {};
+    scores<HD>(s, Qt, Kt, ty, tx);
+    scores<HD>(dp, Dt, Vt, ty, tx);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < 4; ++c) {
         const int i = q0 + ty * 4 + r;
-        const bool see = i < p.T && win_visible(i, k0 + tx * 2 + c, p.window, p.sinks);
+        const bool see = i < p.T && win_visible(i, k0 + tx * 4 + c, p.window, p.sinks);
         s[r][c] = see ? expf(s[r][c] * p.scale - lse[r]) * (dp[r][c] - delta[r]) * p.scale : 0.f;
       }
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-      *reinterpret_cast<float4*>(St + (tx * 2 + c) * kWinPitch + ty * 4) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
+    store_weights(St, s, ty, tx);
     __syncthreads();
-#pragma unroll 4
-    for (int n = 0; n < kWinStep; ++n) {
-      const float4 a = *reinterpret_cast<const float4*>(St + n * kWinPitch + ty * 4);
-#pragma unroll
-      for (int c = 0; c < HD / 64; ++c) {
-        const float4 x = *reinterpret_cast<const float4*>(Kr + n * (HD + 4) + c * 64 + tx * 4);
-        fma4(*reinterpret_cast<float(*)[4]>(&acc[0][c * 4]), a.x, x);
-        fma4(*reinterpret_cast<float(*)[4]>(&acc[1][c * 4]), a.y, x);
-        fma4(*reinterpret_cast<float(*)[4]>(&acc[2][c * 4]), a.z, x);
-        fma4(*reinterpret_cast<float(*)[4]>(&acc[3][c * 4]), a.w, x);
-      }
-    }
+    accumulate<HD>(acc, St, Kt, ty, tx);
   }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int i = q0 + ty * 4 + r;
-    if (i >= p.T) continue;
-    T* dq = static_cast<T*>(p.dq) + (row0 + i) * p.dq_st + h * p.hd;
-#pragma unroll
-    for (int c = 0; c < HD / 64; ++c) {
-      const int d = c * 64 + tx * 4;
-      if (d < p.hd) store4(dq + d, make_float4(acc[r][c * 4], acc[r][c * 4 + 1], acc[r][c * 4 + 2], acc[r][c * 4 + 3]));
-    }
-  }
+  store_rows<T, HD>(static_cast<T*>(p.dq) + row0 * p.dq_st + h * p.hd, p.dq_st, q0, p.T, p.hd, acc, ty, tx);
 }
 
 template <int HD>
 struct WinDkvSmem {
-  static constexpr int kK = 0, kV = kK + HD * kWinPitch, kQ = kV + HD * kWinPitch, kDO = kQ + HD * kWinStepPitch,
-                       kQr = kDO + HD * kWinStepPitch, kDr = kQr + kWinStep * (HD + 4), kP = kDr + kWinStep * (HD + 4),
-                       kDS = kP + kWinStep * kWinPitch;
-  static constexpr int kBytes = (kDS + kWinStep * kWinPitch) * 4;
+  static constexpr int kK = 0, kV = kK + HD * kRowPitch, kQ = kV + HD * kRowPitch, kDO = kQ + HD * kStepPitch,
+                       kP = kDO + HD * kStepPitch, kDS = kP + kWinStep * kRowPitch;
+  static constexpr int kBytes = (kDS + kWinStep * kRowPitch) * 4;
 };
 
-// One CTA per 64 keys of a kv head, over the query heads that share it; reads the delta that window_dq_kernel wrote.
+// One CTA per 32 keys of a kv head, over the query heads that share it; reads the delta that window_dq_kernel wrote.  The
+// query steps of a tile that holds sinks reach to the end of the sequence and are split over sink_parts CTAs.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p) {
   using Sm = WinDkvSmem<HD>;
   extern __shared__ __align__(16) float sm[];
-  float *Kt = sm + Sm::kK, *Vt = sm + Sm::kV, *Qt = sm + Sm::kQ, *Dt = sm + Sm::kDO, *Qr = sm + Sm::kQr, *Dr = sm + Sm::kDr,
-        *Pt = sm + Sm::kP, *St = sm + Sm::kDS;
+  float *Kt = sm + Sm::kK, *Vt = sm + Sm::kV, *Qt = sm + Sm::kQ, *Dt = sm + Sm::kDO, *Pt = sm + Sm::kP, *St = sm + Sm::kDS;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int hk = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv, G = p.Hq / p.Hkv;
-  const int k0 = blockIdx.y * kWinRows;
+  const int n_sink_ctas = p.sink_tiles * p.sink_parts, y = blockIdx.y;
+  const bool sink_cta = y < n_sink_ctas;
+  const int part = sink_cta ? y % p.sink_parts : 0;
+  const int tile = sink_cta ? y / p.sink_parts : y - n_sink_ctas + p.sink_tiles;
+  const int k0 = tile * kWinRows;
   const long long row0 = static_cast<long long>(b) * p.T;
-  load_tile<T, HD, kWinRows, true, false>(static_cast<const T*>(p.k) + row0 * p.k_st + hk * p.hd, p.k_st, k0, p.T, p.hd, Kt,
-                                          kWinPitch, nullptr);
-  load_tile<T, HD, kWinRows, true, false>(static_cast<const T*>(p.v) + row0 * p.v_st + hk * p.hd, p.v_st, k0, p.T, p.hd, Vt,
-                                          kWinPitch, nullptr);
-  float dk[4][HD / 16] = {}, dv[4][HD / 16] = {};
-  // the last query that sees a key of this tile
+  // query steps, up to the last query that sees a key of this tile
   const long long reach = static_cast<long long>(min(k0 + kWinRows, p.T)) - 1 + p.window - 1;
-  const int last = k0 < p.sinks || reach > p.T - 1 ? p.T - 1 : static_cast<int>(reach);
-  const int first = k0 / kWinStep, n_steps = last / kWinStep - first + 1;
+  const int last = (sink_cta || reach > p.T - 1 ? p.T - 1 : static_cast<int>(reach)) / kWinStep;
+  const int first = k0 / kWinStep + part * p.sink_step;
+  const int n_steps = min(last - first + 1, sink_cta ? p.sink_step : last - first + 1);
+  if (n_steps <= 0) return;   // a later tile has fewer parts
+  load_tile<T, HD, kWinRows>(static_cast<const T*>(p.k) + row0 * p.k_st + hk * p.hd, p.k_st, k0, p.T, p.hd, Kt, kRowPitch);
+  load_tile<T, HD, kWinRows>(static_cast<const T*>(p.v) + row0 * p.v_st + hk * p.hd, p.v_st, k0, p.T, p.hd, Vt, kRowPitch);
+  float dk[4][HD / 16] = {}, dv[4][HD / 16] = {};
   for (int it = 0; it < G * n_steps; ++it) {
     const int h = hk * G + it / n_steps, q0 = (first + it % n_steps) * kWinStep;
     const long long stat0 = (static_cast<long long>(b) * p.Hq + h) * p.T;
     __syncthreads();
-    load_tile<T, HD, kWinStep, true, true>(static_cast<const T*>(p.q) + row0 * p.q_st + h * p.hd, p.q_st, q0, p.T, p.hd, Qt,
-                                           kWinStepPitch, Qr);
-    load_tile<T, HD, kWinStep, true, true>(static_cast<const T*>(p.d_o) + row0 * p.do_st + h * p.hd, p.do_st, q0, p.T, p.hd, Dt,
-                                           kWinStepPitch, Dr);
-    float lse[2], delta[2];
+    load_tile<T, HD, kWinStep>(static_cast<const T*>(p.q) + row0 * p.q_st + h * p.hd, p.q_st, q0, p.T, p.hd, Qt, kStepPitch);
+    load_tile<T, HD, kWinStep>(static_cast<const T*>(p.d_o) + row0 * p.do_st + h * p.hd, p.do_st, q0, p.T, p.hd, Dt, kStepPitch);
+    float lse[4], delta[4];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int i = q0 + tx * 2 + c;
+    for (int c = 0; c < 4; ++c) {
+      const int i = q0 + tx * 4 + c;
       lse[c] = i < p.T ? p.lse[stat0 + i] : 0.f;
       delta[c] = i < p.T ? p.delta[stat0 + i] : 0.f;
     }
     __syncthreads();
-    float s[4][2] = {}, dp[4][2] = {};
-#pragma unroll 8
-    for (int d = 0; d < HD; ++d) {
-      const float4 a = *reinterpret_cast<const float4*>(Kt + d * kWinPitch + ty * 4);
-      const float4 g = *reinterpret_cast<const float4*>(Vt + d * kWinPitch + ty * 4);
-      const float2 x = *reinterpret_cast<const float2*>(Qt + d * kWinStepPitch + tx * 2);
-      const float2 y = *reinterpret_cast<const float2*>(Dt + d * kWinStepPitch + tx * 2);
-      const float ar[4] = {a.x, a.y, a.z, a.w}, gr[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[r][0] = fmaf(ar[r], x.x, s[r][0]);
-        s[r][1] = fmaf(ar[r], x.y, s[r][1]);
-        dp[r][0] = fmaf(gr[r], y.x, dp[r][0]);
-        dp[r][1] = fmaf(gr[r], y.y, dp[r][1]);
-      }
-    }
+    float s[4][4] = {}, dp[4][4] = {};
+    scores<HD>(s, Kt, Qt, ty, tx);
+    scores<HD>(dp, Vt, Dt, ty, tx);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int i = q0 + tx * 2 + c, j = k0 + ty * 4 + r;
+      for (int c = 0; c < 4; ++c) {
+        const int i = q0 + tx * 4 + c, j = k0 + ty * 4 + r;
         const bool see = i < p.T && win_visible(i, j, p.window, p.sinks);
         const float prob = see ? expf(s[r][c] * p.scale - lse[c]) : 0.f;
         s[r][c] = prob;
         dp[r][c] = see ? prob * (dp[r][c] - delta[c]) * p.scale : 0.f;
       }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      *reinterpret_cast<float4*>(Pt + (tx * 2 + c) * kWinPitch + ty * 4) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
-      *reinterpret_cast<float4*>(St + (tx * 2 + c) * kWinPitch + ty * 4) = make_float4(dp[0][c], dp[1][c], dp[2][c], dp[3][c]);
-    }
+    store_weights(Pt, s, ty, tx);
+    store_weights(St, dp, ty, tx);
     __syncthreads();
-#pragma unroll 2
-    for (int n = 0; n < kWinStep; ++n) {
-      const float4 a = *reinterpret_cast<const float4*>(Pt + n * kWinPitch + ty * 4);
-      const float4 g = *reinterpret_cast<const float4*>(St + n * kWinPitch + ty * 4);
-#pragma unroll
-      for (int c = 0; c < HD / 64; ++c) {
-        const float4 x = *reinterpret_cast<const float4*>(Dr + n * (HD + 4) + c * 64 + tx * 4);
-        const float4 y = *reinterpret_cast<const float4*>(Qr + n * (HD + 4) + c * 64 + tx * 4);
-        fma4(*reinterpret_cast<float(*)[4]>(&dv[0][c * 4]), a.x, x);
-        fma4(*reinterpret_cast<float(*)[4]>(&dv[1][c * 4]), a.y, x);
-        fma4(*reinterpret_cast<float(*)[4]>(&dv[2][c * 4]), a.z, x);
-        fma4(*reinterpret_cast<float(*)[4]>(&dv[3][c * 4]), a.w, x);
-        fma4(*reinterpret_cast<float(*)[4]>(&dk[0][c * 4]), g.x, y);
-        fma4(*reinterpret_cast<float(*)[4]>(&dk[1][c * 4]), g.y, y);
-        fma4(*reinterpret_cast<float(*)[4]>(&dk[2][c * 4]), g.z, y);
-        fma4(*reinterpret_cast<float(*)[4]>(&dk[3][c * 4]), g.w, y);
-      }
-    }
+    accumulate<HD>(dv, Pt, Dt, ty, tx);
+    accumulate<HD>(dk, St, Qt, ty, tx);
   }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int j = k0 + ty * 4 + r;
-    if (j >= p.T) continue;
-    T* ok = static_cast<T*>(p.dk) + (row0 + j) * p.dk_st + hk * p.hd;
-    T* ov = static_cast<T*>(p.dv) + (row0 + j) * p.dv_st + hk * p.hd;
-#pragma unroll
-    for (int c = 0; c < HD / 64; ++c) {
-      const int d = c * 64 + tx * 4;
-      if (d < p.hd) {
-        store4(ok + d, make_float4(dk[r][c * 4], dk[r][c * 4 + 1], dk[r][c * 4 + 2], dk[r][c * 4 + 3]));
-        store4(ov + d, make_float4(dv[r][c * 4], dv[r][c * 4 + 1], dv[r][c * 4 + 2], dv[r][c * 4 + 3]));
-      }
-    }
+  if (sink_cta && p.sink_parts > 1) {
+    float* sum = p.sink_part + (((static_cast<long long>(part) * p.B + b) * p.sink_tiles + tile) * p.Hkv + hk) * 2 * kWinRows * p.hd;
+    store_rows<float, HD>(sum, p.hd, 0, kWinRows, p.hd, dk, ty, tx);
+    store_rows<float, HD>(sum + kWinRows * p.hd, p.hd, 0, kWinRows, p.hd, dv, ty, tx);
+  } else {
+    store_rows<T, HD>(static_cast<T*>(p.dk) + row0 * p.dk_st + hk * p.hd, p.dk_st, k0, p.T, p.hd, dk, ty, tx);
+    store_rows<T, HD>(static_cast<T*>(p.dv) + row0 * p.dv_st + hk * p.hd, p.dv_st, k0, p.T, p.hd, dv, ty, tx);
   }
+}
+
+// dK and dV of the sinks' tiles: the sums of their parts, in order.
+template <typename T>
+__global__ void window_join_kernel(const WinArgs p) {
+  const int rows = min(p.T, p.sink_tiles * kWinRows), steps = (p.T + kWinStep - 1) / kWinStep;
+  const long long n = static_cast<long long>(p.B) * rows * p.Hkv * 2 * p.hd;
+  const long long part_size = static_cast<long long>(p.B) * p.sink_tiles * p.Hkv * 2 * kWinRows * p.hd;
+  for (long long x = blockIdx.x * (long long)blockDim.x + threadIdx.x; x < n; x += (long long)gridDim.x * blockDim.x) {
+    const int d = static_cast<int>(x % p.hd);
+    long long r = x / p.hd;
+    const int which = static_cast<int>(r % 2), hk = static_cast<int>(r / 2 % p.Hkv);
+    r = r / 2 / p.Hkv;
+    const int t = static_cast<int>(r % rows), b = static_cast<int>(r / rows), tile = t / kWinRows;
+    const float* src = p.sink_part + (((static_cast<long long>(b) * p.sink_tiles + tile) * p.Hkv + hk) * 2 + which) * kWinRows * p.hd + (t % kWinRows) * p.hd + d;
+    const int parts = (steps - tile * kWinRows / kWinStep + p.sink_step - 1) / p.sink_step;
+    float sum = 0.f;
+    for (int c = 0; c < parts; ++c) sum += src[c * part_size];
+    const long long bt = static_cast<long long>(b) * p.T + t;
+    T* dst = which == 0 ? static_cast<T*>(p.dk) + bt * p.dk_st : static_cast<T*>(p.dv) + bt * p.dv_st;
+    dst[hk * p.hd + d] = from_f32<T>(sum);
+  }
+}
+
+// Parts of a sink tile no longer than what another tile of keys takes, or than a CTA's share of all work.
+struct WinSplit {
+  int tiles, step, parts;
+};
+static WinSplit win_split(const TitbAttnDesc& d, int window, int sinks) {
+  const long long steps = (d.T + kWinStep - 1) / kWinStep, near = (window + kWinRows + kWinStep - 2LL) / kWinStep + 1;
+  const long long tiles = (sinks + kWinRows - 1) / kWinRows, all = (d.T + kWinRows - 1) / kWinRows;
+  if (tiles == 0) return {0, 1, 1};
+  const long long work = static_cast<long long>(d.Hkv) * d.B * (tiles * steps + (all - tiles) * near), share = work / (device_sm_count() * 8LL);
+  const long long step = near > share ? near : share;
+  return {static_cast<int>(tiles), static_cast<int>(step < steps ? step : steps), static_cast<int>((steps + step - 1) / step)};
+}
+static long long win_part_floats(const TitbAttnDesc& d, const WinSplit& s) {
+  return s.parts > 1 ? static_cast<long long>(s.parts) * d.B * s.tiles * d.Hkv * 2 * kWinRows * d.hd : 0;
 }
 
 // more than the sequence changes nothing
@@ -431,7 +408,7 @@ static WinArgs win_args(const TitbWindowDesc* w) {
   WinArgs a{};
   a.q = d.q; a.k = d.k; a.v = d.v; a.o = d.o; a.lse = d.lse;
   a.d_o = d.d_o; a.dq = d.dq; a.dk = d.dk; a.dv = d.dv; a.delta = d.delta;
-  a.T = d.T; a.Hq = d.Hq; a.Hkv = d.Hkv; a.hd = d.hd; a.scale = d.scale;
+  a.B = d.B; a.T = d.T; a.Hq = d.Hq; a.Hkv = d.Hkv; a.hd = d.hd; a.scale = d.scale;
   a.window = window_of(w); a.sinks = sinks_of(w);
   a.q_st = d.q_stride_t; a.k_st = d.k_stride_t; a.v_st = d.v_stride_t; a.o_st = d.o_stride_t;
   a.do_st = d.do_stride_t; a.dq_st = d.dq_stride_t; a.dk_st = d.dk_stride_t; a.dv_st = d.dv_stride_t;
@@ -439,31 +416,39 @@ static WinArgs win_args(const TitbWindowDesc* w) {
 }
 
 template <typename K>
-static cudaError_t win_launch(K kernel, const WinArgs& a, int heads, int B, int smem, cudaStream_t st) {
+static cudaError_t win_launch(K kernel, const WinArgs& a, int heads, int jobs, int smem, cudaStream_t st) {
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid(static_cast<unsigned>(heads) * B, (a.T + kWinRows - 1) / kWinRows);
-  kernel<<<grid, kWinThreads, smem, st>>>(a);
+  kernel<<<dim3(static_cast<unsigned>(heads) * a.B, jobs), kWinThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
 template <typename T, int HD>
 static int win_fwd(const TitbWindowDesc* w, cudaStream_t st) {
-  return static_cast<int>(win_launch(window_fwd_kernel<T, HD>, win_args(w), w->attn.Hq, w->attn.B, WinFwdSmem<HD>::kBytes, st));
+  const WinArgs a = win_args(w);
+  return static_cast<int>(win_launch(window_fwd_kernel<T, HD>, a, a.Hq, (a.T + kWinRows - 1) / kWinRows, WinFwdSmem<HD>::kBytes, st));
 }
 template <typename T, int HD>
 static int win_bwd(const TitbWindowDesc* w, cudaStream_t st) {
-  const WinArgs a = win_args(w);
-  const cudaError_t e = win_launch(window_dq_kernel<T, HD>, a, w->attn.Hq, w->attn.B, WinDqSmem<HD>::kBytes, st);
+  WinArgs a = win_args(w);
+  const WinSplit split = win_split(w->attn, a.window, a.sinks);
+  a.sink_tiles = split.tiles; a.sink_step = split.step; a.sink_parts = split.parts;
+  a.sink_part = w->workspace;
+  const int tiles = (a.T + kWinRows - 1) / kWinRows;
+  cudaError_t e = win_launch(window_dq_kernel<T, HD>, a, a.Hq, tiles, WinDqSmem<HD>::kBytes, st);
   if (e != cudaSuccess) return static_cast<int>(e);
-  return static_cast<int>(win_launch(window_dkv_kernel<T, HD>, a, w->attn.Hkv, w->attn.B, WinDkvSmem<HD>::kBytes, st));
+  e = win_launch(window_dkv_kernel<T, HD>, a, a.Hkv, tiles + split.tiles * (split.parts - 1), WinDkvSmem<HD>::kBytes, st);
+  if (e != cudaSuccess || split.tiles == 0 || split.parts == 1) return static_cast<int>(e);
+  const long long n = win_part_floats(w->attn, split) / split.parts, most = device_sm_count() * 8LL;
+  window_join_kernel<T><<<static_cast<int>((n + 255) / 256 < most ? (n + 255) / 256 : most), 256, 0, st>>>(a);
+  return static_cast<int>(cudaGetLastError());
 }
 
 static int win_check(const TitbWindowDesc* w, bool backward) {
   const TitbAttnDesc& d = w->attn;
   if (d.hd <= 0 || d.hd > 128 || d.hd % 8 || d.Hkv <= 0 || d.Hq % d.Hkv || w->window < 1 || w->sinks < 0) return TITB_ERR_SHAPE;
   // grid: heads x batch along x, tiles along y
-  if (static_cast<long long>(d.Hq) * d.B > 0x7fffffffLL || (d.T + kWinRows - 1LL) / kWinRows > 65535) return TITB_ERR_SHAPE;
+  if (static_cast<long long>(d.Hq) * d.B > 0x7fffffffLL || (d.T + kWinRows - 1LL) / kWinRows > 32767) return TITB_ERR_SHAPE;
   const int mask = w->dtype == 1 ? 7 : 3;
   auto bad = [&](const void* p, long long st) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0 || (st & mask) != 0; };
   if (bad(d.q, d.q_stride_t) || bad(d.k, d.k_stride_t) || bad(d.v, d.v_stride_t) || bad(d.o, d.o_stride_t))
@@ -502,6 +487,7 @@ TITB_API int titb_window_attn_bwd(const TitbWindowDesc* w, cudaStream_t st) {
 
 TITB_API long long titb_window_attn_bwd_workspace(const TitbWindowDesc* w) {
   const TitbAttnDesc& d = w->attn;
-  if (d.B <= 0 || d.T <= 0 || d.Hq <= 0 || win_check(w, false) || !on_tensor_cores(w)) return 0;
+  if (d.B <= 0 || d.T <= 0 || d.Hq <= 0 || win_check(w, false)) return 0;
+  if (!on_tensor_cores(w)) return win_part_floats(d, win_split(d, window_of(w), sinks_of(w)));
   return static_cast<long long>(d.B) * d.T * d.Hq * d.hd + window_tc_sink_floats(&d, window_of(w), sinks_of(w));
 }
