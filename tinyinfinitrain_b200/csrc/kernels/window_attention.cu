@@ -25,8 +25,9 @@ long long window_tc_sink_floats(const TitbAttnDesc* d, int window, int sinks);
 constexpr int kWinThreads = 128;   // 8 x 16 threads of 4 x 4 scores
 constexpr int kWinRows = 32;       // rows of the tile that a CTA owns
 constexpr int kWinStep = 64;       // rows of the other operand that arrive at a time
-// pitches of the transposed tiles [HD][rows]: rows stay 16-byte aligned and neighbouring heads' elements 4 banks apart
-constexpr int kRowPitch = kWinRows + 4, kStepPitch = kWinStep + 4;
+// Tiles are [rows][HD + 4], weights [step row][kWeightPitch]: odd numbers of 16-byte units, so that rows that neighbouring lanes
+// read or write lie in different banks.
+constexpr int kWeightPitch = kWinRows + 4;
 
 struct WinArgs {
   const void *q, *k, *v, *d_o;
@@ -62,19 +63,13 @@ __device__ __forceinline__ float4 load4(const T* base, long long t, long long st
   return r;
 }
 
-// ROWS rows from row t0 on, transposed, into shared memory: element d of a row at tile[d * pitch + row].  Two lanes take 32
-// bytes of a row and sixteen rows share a warp, which makes whole sectors of the loads and 32 banks of the stores.
+// ROWS rows from row t0 on into shared memory.
 template <typename T, int HD, int ROWS>
-__device__ __forceinline__ void load_tile(const T* base, long long stride, int t0, int n_rows, int hd, float* tile, int pitch) {
+__device__ __forceinline__ void load_tile(const T* base, long long stride, int t0, int n_rows, int hd, float* tile) {
 #pragma unroll 8
   for (int i = threadIdx.x; i < ROWS * HD / 4; i += kWinThreads) {
-    const int lane = i & 31, grp = i >> 5;
-    const int r = grp % (ROWS / 16) * 16 + (lane >> 1), d = (grp / (ROWS / 16) * 2 + (lane & 1)) * 4;
-    const float4 x = load4(base, t0 + r, stride, d, n_rows, hd);
-    tile[d * pitch + r] = x.x;
-    tile[(d + 1) * pitch + r] = x.y;
-    tile[(d + 2) * pitch + r] = x.z;
-    tile[(d + 3) * pitch + r] = x.w;
+    const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+    *reinterpret_cast<float4*>(tile + r * (HD + 4) + d) = load4(base, t0 + r, stride, d, n_rows, hd);
   }
 }
 
@@ -89,64 +84,78 @@ __device__ __forceinline__ float half_warp_sum(float v) {
   return v;
 }
 
-// acc[r][c] += a[r] . b[c] over the head: rows ty * 4 of the owned tile, rows tx * 4 of the step's.
+// acc[r][c] = own row ty * 4 + r times step row tx + 16 c.  Even and odd elements of the head are summed apart, two to an
+// instruction.
 template <int HD>
 __device__ __forceinline__ void scores(float (&acc)[4][4], const float* own, const float* step, int ty, int tx) {
-#pragma unroll 8
-  for (int d = 0; d < HD; ++d) {
-    const float4 a = *reinterpret_cast<const float4*>(own + d * kRowPitch + ty * 4);
-    const float4 b = *reinterpret_cast<const float4*>(step + d * kStepPitch + tx * 4);
-    const float ar[4] = {a.x, a.y, a.z, a.w}, bc[4] = {b.x, b.y, b.z, b.w};
+  float even[4][4] = {}, odd[4][4] = {};
+#pragma unroll 4
+  for (int d = 0; d < HD; d += 4) {
+    float4 a[4], b[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4*>(own + (ty * 4 + r) * (HD + 4) + d);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) b[c] = *reinterpret_cast<const float4*>(step + (tx + 16 * c) * (HD + 4) + d);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[r][c] = fmaf(ar[r], bc[c], acc[r][c]);
+      for (int c = 0; c < 4; ++c) {
+        fma2(even[r][c], odd[r][c], a[r].x, a[r].y, b[c].x, b[c].y, even[r][c], odd[r][c]);
+        fma2(even[r][c], odd[r][c], a[r].z, a[r].w, b[c].z, b[c].w, even[r][c], odd[r][c]);
+      }
   }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[r][c] = even[r][c] + odd[r][c];
 }
 // w ([step row][own row]) <- s
 __device__ __forceinline__ void store_weights(float* w, const float (&s)[4][4], int ty, int tx) {
 #pragma unroll
   for (int c = 0; c < 4; ++c)
-    *reinterpret_cast<float4*>(w + (tx * 4 + c) * kRowPitch + ty * 4) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
+    *reinterpret_cast<float4*>(w + (tx + 16 * c) * kWeightPitch + ty * 4) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
 }
-// acc[r][i] += sum over the step's rows n of w[n][own row ty * 4 + r] times element tx + 16 i of row n: the elements are read
-// four rows at a time from the transposed tile.
+// acc[r] += sum over the step's rows n of w[n][own row ty * 4 + r] times elements 64 c + 4 tx .. of row n; two rows to an
+// instruction (acc[c][e][r] with e the element).
 template <int HD>
-__device__ __forceinline__ void accumulate(float (&acc)[4][HD / 16], const float* w, const float* step, int ty, int tx) {
-#pragma unroll 2
-  for (int n = 0; n < kWinStep; n += 4) {
-    float4 a[4];
+__device__ __forceinline__ void accumulate(float (&acc)[HD / 64][4][4], const float* w, const float* step, int ty, int tx) {
+#pragma unroll 4
+  for (int n = 0; n < kWinStep; ++n) {
+    const float4 a = *reinterpret_cast<const float4*>(w + n * kWeightPitch + ty * 4);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) a[k] = *reinterpret_cast<const float4*>(w + (n + k) * kRowPitch + ty * 4);
+    for (int c = 0; c < HD / 64; ++c) {
+      const float4 x = *reinterpret_cast<const float4*>(step + n * (HD + 4) + c * 64 + tx * 4);
+      const float xe[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int i = 0; i < HD / 16; ++i) {
-      const float4 x = *reinterpret_cast<const float4*>(step + (tx + 16 * i) * kStepPitch + n);
-      const float xk[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        acc[0][i] = fmaf(a[k].x, xk[k], acc[0][i]);
-        acc[1][i] = fmaf(a[k].y, xk[k], acc[1][i]);
-        acc[2][i] = fmaf(a[k].z, xk[k], acc[2][i]);
-        acc[3][i] = fmaf(a[k].w, xk[k], acc[3][i]);
+      for (int e = 0; e < 4; ++e) {
+        float(&s)[4] = acc[c][e];
+        fma2(s[0], s[1], a.x, a.y, xe[e], xe[e], s[0], s[1]);
+        fma2(s[2], s[3], a.z, a.w, xe[e], xe[e], s[2], s[3]);
       }
     }
   }
 }
 template <typename T, int HD>
-__device__ __forceinline__ void store_rows(T* base, long long stride, int t0, int n_rows, int hd, const float (&acc)[4][HD / 16],
+__device__ __forceinline__ void store_rows(T* base, long long stride, int t0, int n_rows, int hd, const float (&acc)[HD / 64][4][4],
                                            int ty, int tx) {
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (t0 + ty * 4 + r < n_rows)
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i)
-        if (tx + 16 * i < hd) base[(t0 + ty * 4 + r) * stride + tx + 16 * i] = from_f32<T>(acc[r][i]);
+      for (int c = 0; c < HD / 64; ++c) {
+        const int d = c * 64 + tx * 4;
+        if (d >= hd) continue;
+        Pack<T, 4> x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.v[e] = from_f32<T>(acc[c][e][r]);
+        *reinterpret_cast<Pack<T, 4>*>(base + (t0 + ty * 4 + r) * stride + d) = x;
+      }
 }
 
 template <int HD>
 struct WinFwdSmem {
-  static constexpr int kQ = 0, kK = kQ + HD * kRowPitch, kV = kK + HD * kStepPitch, kP = kV + HD * kStepPitch;
-  static constexpr int kBytes = (kP + kWinStep * kRowPitch) * 4;
+  static constexpr int kQ = 0, kK = kQ + kWinRows * (HD + 4), kV = kK + kWinStep * (HD + 4), kP = kV + kWinStep * (HD + 4);
+  static constexpr int kBytes = (kP + kWinStep * kWeightPitch) * 4;
 };
 
 // One CTA per 32 queries of a head.
@@ -154,7 +163,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p) {
   using Sm = WinFwdSmem<HD>;
   extern __shared__ __align__(16) float sm[];
-  float *Qt = sm + Sm::kQ, *Kt = sm + Sm::kK, *Vt = sm + Sm::kV, *Pt = sm + Sm::kP;
+  float *Qs = sm + Sm::kQ, *Ks = sm + Sm::kK, *Vs = sm + Sm::kV, *Ps = sm + Sm::kP;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int h = blockIdx.x % p.Hq, b = blockIdx.x / p.Hq, hk = h / (p.Hq / p.Hkv);
   const int q0 = (gridDim.y - 1 - blockIdx.y) * kWinRows;
@@ -163,8 +172,8 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
   const T* k = static_cast<const T*>(p.k) + row0 * p.k_st + hk * p.hd;
   const T* v = static_cast<const T*>(p.v) + row0 * p.v_st + hk * p.hd;
 
-  load_tile<T, HD, kWinRows>(q, p.q_st, q0, p.T, p.hd, Qt, kRowPitch);
-  float acc[4][HD / 16] = {};
+  load_tile<T, HD, kWinRows>(q, p.q_st, q0, p.T, p.hd, Qs);
+  float acc[HD / 64][4][4] = {};
   float m[4], l[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
@@ -175,18 +184,18 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
   for (int it = 0; it < n_steps; ++it) {
     const int k0 = (it < sink_steps ? it : first + it - sink_steps) * kWinStep;
     __syncthreads();
-    load_tile<T, HD, kWinStep>(k, p.k_st, k0, p.T, p.hd, Kt, kStepPitch);
-    load_tile<T, HD, kWinStep>(v, p.v_st, k0, p.T, p.hd, Vt, kStepPitch);
+    load_tile<T, HD, kWinStep>(k, p.k_st, k0, p.T, p.hd, Ks);
+    load_tile<T, HD, kWinStep>(v, p.v_st, k0, p.T, p.hd, Vs);
     __syncthreads();
-    float s[4][4] = {};
-    scores<HD>(s, Qt, Kt, ty, tx);
+    float s[4][4];
+    scores<HD>(s, Qs, Ks, ty, tx);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = q0 + ty * 4 + r;
       float top = -INFINITY;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        s[r][c] = win_visible(i, k0 + tx * 4 + c, p.window, p.sinks) ? s[r][c] * p.scale : -INFINITY;
+        s[r][c] = win_visible(i, k0 + tx + 16 * c, p.window, p.sinks) ? s[r][c] * p.scale : -INFINITY;
         top = fmaxf(top, s[r][c]);
       }
       top = fmaxf(m[r], half_warp_max(top));
@@ -201,18 +210,18 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
       l[r] = l[r] * keep + half_warp_sum(sum);
       m[r] = top;
 #pragma unroll
-      for (int i2 = 0; i2 < HD / 16; ++i2) acc[r][i2] *= keep;
+      for (int e = 0; e < HD / 16; ++e) acc[e / 4][e % 4][r] *= keep;
     }
-    store_weights(Pt, s, ty, tx);
+    store_weights(Ps, s, ty, tx);
     __syncthreads();
-    accumulate<HD>(acc, Pt, Vt, ty, tx);
+    accumulate<HD>(acc, Ps, Vs, ty, tx);
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int i = q0 + ty * 4 + r;
     const float inv = 1.f / l[r];
 #pragma unroll
-    for (int c = 0; c < HD / 16; ++c) acc[r][c] *= inv;
+    for (int e = 0; e < HD / 16; ++e) acc[e / 4][e % 4][r] *= inv;
     if (tx == 0 && i < p.T) p.lse[(static_cast<long long>(b) * p.Hq + h) * p.T + i] = m[r] + logf(l[r]);
   }
   store_rows<T, HD>(static_cast<T*>(p.o) + row0 * p.o_st + h * p.hd, p.o_st, q0, p.T, p.hd, acc, ty, tx);
@@ -220,9 +229,9 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
 
 template <int HD>
 struct WinDqSmem {
-  static constexpr int kQ = 0, kDO = kQ + HD * kRowPitch, kK = kDO + HD * kRowPitch, kV = kK + HD * kStepPitch,
-                       kDS = kV + HD * kStepPitch;
-  static constexpr int kBytes = (kDS + kWinStep * kRowPitch) * 4;
+  static constexpr int kQ = 0, kDO = kQ + kWinRows * (HD + 4), kK = kDO + kWinRows * (HD + 4), kV = kK + kWinStep * (HD + 4),
+                       kDS = kV + kWinStep * (HD + 4);
+  static constexpr int kBytes = (kDS + kWinStep * kWeightPitch) * 4;
 };
 
 // One CTA per 32 queries of a head: delta, then dQ.
@@ -230,7 +239,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p) {
   using Sm = WinDqSmem<HD>;
   extern __shared__ __align__(16) float sm[];
-  float *Qt = sm + Sm::kQ, *Dt = sm + Sm::kDO, *Kt = sm + Sm::kK, *Vt = sm + Sm::kV, *St = sm + Sm::kDS;
+  float *Qs = sm + Sm::kQ, *Ds = sm + Sm::kDO, *Ks = sm + Sm::kK, *Vs = sm + Sm::kV, *Ss = sm + Sm::kDS;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int h = blockIdx.x % p.Hq, b = blockIdx.x / p.Hq, hk = h / (p.Hq / p.Hkv);
   const int q0 = (gridDim.y - 1 - blockIdx.y) * kWinRows;
@@ -242,8 +251,8 @@ __global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p)
   const T* o = static_cast<const T*>(p.o) + row0 * p.o_st + h * p.hd;
   const long long stat0 = (static_cast<long long>(b) * p.Hq + h) * p.T;
 
-  load_tile<T, HD, kWinRows>(q, p.q_st, q0, p.T, p.hd, Qt, kRowPitch);
-  load_tile<T, HD, kWinRows>(d_o, p.do_st, q0, p.T, p.hd, Dt, kRowPitch);
+  load_tile<T, HD, kWinRows>(q, p.q_st, q0, p.T, p.hd, Qs);
+  load_tile<T, HD, kWinRows>(d_o, p.do_st, q0, p.T, p.hd, Ds);
   float lse[4], delta[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -258,39 +267,39 @@ __global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p)
     lse[r] = i < p.T ? p.lse[stat0 + i] : 0.f;
     if (tx == 0 && i < p.T) p.delta[stat0 + i] = delta[r];
   }
-  float acc[4][HD / 16] = {};
+  float acc[HD / 64][4][4] = {};
   const int first = max(0, q0 - p.window + 1) / kWinStep, last = min(q0 + kWinRows, p.T) - 1;
   const int sink_steps = min((p.sinks + kWinStep - 1) / kWinStep, first);
   const int n_steps = sink_steps + last / kWinStep - first + 1;
   for (int it = 0; it < n_steps; ++it) {
     const int k0 = (it < sink_steps ? it : first + it - sink_steps) * kWinStep;
     __syncthreads();
-    load_tile<T, HD, kWinStep>(k, p.k_st, k0, p.T, p.hd, Kt, kStepPitch);
-    load_tile<T, HD, kWinStep>(v, p.v_st, k0, p.T, p.hd, Vt, kStepPitch);
+    load_tile<T, HD, kWinStep>(k, p.k_st, k0, p.T, p.hd, Ks);
+    load_tile<T, HD, kWinStep>(v, p.v_st, k0, p.T, p.hd, Vs);
     __syncthreads();
-    float s[4][4] = {}, dp[4][4] = {};
-    scores<HD>(s, Qt, Kt, ty, tx);
-    scores<HD>(dp, Dt, Vt, ty, tx);
+    float s[4][4], dp[4][4];
+    scores<HD>(s, Qs, Ks, ty, tx);
+    scores<HD>(dp, Ds, Vs, ty, tx);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int i = q0 + ty * 4 + r;
-        const bool see = i < p.T && win_visible(i, k0 + tx * 4 + c, p.window, p.sinks);
+        const bool see = i < p.T && win_visible(i, k0 + tx + 16 * c, p.window, p.sinks);
         s[r][c] = see ? expf(s[r][c] * p.scale - lse[r]) * (dp[r][c] - delta[r]) * p.scale : 0.f;
       }
-    store_weights(St, s, ty, tx);
+    store_weights(Ss, s, ty, tx);
     __syncthreads();
-    accumulate<HD>(acc, St, Kt, ty, tx);
+    accumulate<HD>(acc, Ss, Ks, ty, tx);
   }
   store_rows<T, HD>(static_cast<T*>(p.dq) + row0 * p.dq_st + h * p.hd, p.dq_st, q0, p.T, p.hd, acc, ty, tx);
 }
 
 template <int HD>
 struct WinDkvSmem {
-  static constexpr int kK = 0, kV = kK + HD * kRowPitch, kQ = kV + HD * kRowPitch, kDO = kQ + HD * kStepPitch,
-                       kP = kDO + HD * kStepPitch, kDS = kP + kWinStep * kRowPitch;
-  static constexpr int kBytes = (kDS + kWinStep * kRowPitch) * 4;
+  static constexpr int kK = 0, kV = kK + kWinRows * (HD + 4), kQ = kV + kWinRows * (HD + 4), kDO = kQ + kWinStep * (HD + 4),
+                       kP = kDO + kWinStep * (HD + 4), kDS = kP + kWinStep * kWeightPitch;
+  static constexpr int kBytes = (kDS + kWinStep * kWeightPitch) * 4;
 };
 
 // One CTA per 32 keys of a kv head, over the query heads that share it; reads the delta that window_dq_kernel wrote.  The
@@ -299,7 +308,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p) {
   using Sm = WinDkvSmem<HD>;
   extern __shared__ __align__(16) float sm[];
-  float *Kt = sm + Sm::kK, *Vt = sm + Sm::kV, *Qt = sm + Sm::kQ, *Dt = sm + Sm::kDO, *Pt = sm + Sm::kP, *St = sm + Sm::kDS;
+  float *Ks = sm + Sm::kK, *Vs = sm + Sm::kV, *Qs = sm + Sm::kQ, *Ds = sm + Sm::kDO, *Ps = sm + Sm::kP, *Ss = sm + Sm::kDS;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int hk = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv, G = p.Hq / p.Hkv;
   const int n_sink_ctas = p.sink_tiles * p.sink_parts, y = blockIdx.y;
@@ -314,41 +323,41 @@ __global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p
   const int first = k0 / kWinStep + part * p.sink_step;
   const int n_steps = min(last - first + 1, sink_cta ? p.sink_step : last - first + 1);
   if (n_steps <= 0) return;   // a later tile has fewer parts
-  load_tile<T, HD, kWinRows>(static_cast<const T*>(p.k) + row0 * p.k_st + hk * p.hd, p.k_st, k0, p.T, p.hd, Kt, kRowPitch);
-  load_tile<T, HD, kWinRows>(static_cast<const T*>(p.v) + row0 * p.v_st + hk * p.hd, p.v_st, k0, p.T, p.hd, Vt, kRowPitch);
-  float dk[4][HD / 16] = {}, dv[4][HD / 16] = {};
+  load_tile<T, HD, kWinRows>(static_cast<const T*>(p.k) + row0 * p.k_st + hk * p.hd, p.k_st, k0, p.T, p.hd, Ks);
+  load_tile<T, HD, kWinRows>(static_cast<const T*>(p.v) + row0 * p.v_st + hk * p.hd, p.v_st, k0, p.T, p.hd, Vs);
+  float dk[HD / 64][4][4] = {}, dv[HD / 64][4][4] = {};
   for (int it = 0; it < G * n_steps; ++it) {
     const int h = hk * G + it / n_steps, q0 = (first + it % n_steps) * kWinStep;
     const long long stat0 = (static_cast<long long>(b) * p.Hq + h) * p.T;
     __syncthreads();
-    load_tile<T, HD, kWinStep>(static_cast<const T*>(p.q) + row0 * p.q_st + h * p.hd, p.q_st, q0, p.T, p.hd, Qt, kStepPitch);
-    load_tile<T, HD, kWinStep>(static_cast<const T*>(p.d_o) + row0 * p.do_st + h * p.hd, p.do_st, q0, p.T, p.hd, Dt, kStepPitch);
+    load_tile<T, HD, kWinStep>(static_cast<const T*>(p.q) + row0 * p.q_st + h * p.hd, p.q_st, q0, p.T, p.hd, Qs);
+    load_tile<T, HD, kWinStep>(static_cast<const T*>(p.d_o) + row0 * p.do_st + h * p.hd, p.do_st, q0, p.T, p.hd, Ds);
     float lse[4], delta[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const int i = q0 + tx * 4 + c;
+      const int i = q0 + tx + 16 * c;
       lse[c] = i < p.T ? p.lse[stat0 + i] : 0.f;
       delta[c] = i < p.T ? p.delta[stat0 + i] : 0.f;
     }
     __syncthreads();
-    float s[4][4] = {}, dp[4][4] = {};
-    scores<HD>(s, Kt, Qt, ty, tx);
-    scores<HD>(dp, Vt, Dt, ty, tx);
+    float s[4][4], dp[4][4];
+    scores<HD>(s, Ks, Qs, ty, tx);
+    scores<HD>(dp, Vs, Ds, ty, tx);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int i = q0 + tx * 4 + c, j = k0 + ty * 4 + r;
+        const int i = q0 + tx + 16 * c, j = k0 + ty * 4 + r;
         const bool see = i < p.T && win_visible(i, j, p.window, p.sinks);
         const float prob = see ? expf(s[r][c] * p.scale - lse[c]) : 0.f;
         s[r][c] = prob;
         dp[r][c] = see ? prob * (dp[r][c] - delta[c]) * p.scale : 0.f;
       }
-    store_weights(Pt, s, ty, tx);
-    store_weights(St, dp, ty, tx);
+    store_weights(Ps, s, ty, tx);
+    store_weights(Ss, dp, ty, tx);
     __syncthreads();
-    accumulate<HD>(dv, Pt, Dt, ty, tx);
-    accumulate<HD>(dk, St, Qt, ty, tx);
+    accumulate<HD>(dv, Ps, Ds, ty, tx);
+    accumulate<HD>(dk, Ss, Qs, ty, tx);
   }
   if (sink_cta && p.sink_parts > 1) {
     float* sum = p.sink_part + (((static_cast<long long>(part) * p.B + b) * p.sink_tiles + tile) * p.Hkv + hk) * 2 * kWinRows * p.hd;
