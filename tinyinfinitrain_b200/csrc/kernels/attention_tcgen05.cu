@@ -95,16 +95,20 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
 // ------------------------------------------------------------------------- forward
 template <int HD, bool WIN>
 struct FwdCfg {
-  static constexpr bool kTwin = WIN && HD == 128;   // two CTAs on an SM, P in tensor memory (see below)
-  static constexpr int kTileBytes = kBlk * HD * 2;  // Q, K or V tile
-  static constexpr int kStages = kTwin ? 1 : 2;
+  static constexpr int kKeys = WIN && HD == 64 ? 64 : kBlk;   // keys of a step
+  static constexpr int kCtas = !WIN ? (HD == 64 ? 2 : 1) : HD == 64 ? 3 : 2;   // that share an SM
+  static constexpr int kTileBytes = kKeys * HD * 2;  // K or V tile
+  static constexpr int kKvChunk = kKeys * 128;       // its [keys x 64 bf16] sub-tiles
+  static constexpr int kStages = WIN && HD == 128 ? 1 : 2;
   static constexpr int kQ = 0;
-  static constexpr int kK = kQ + kTileBytes;
+  static constexpr int kQBytes = kBlk * HD * 2;
+  static constexpr int kK = kQ + kQBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
   static constexpr int kP = kV + kStages * kTileBytes;
-  static constexpr int kBar = kP + (kTwin ? 0 : kBlk * kBlk * 2);
+  static constexpr int kBar = kP + (WIN ? 0 : kBlk * kBlk * 2);   // WIN: P lies over S in tensor memory
   static constexpr int kSmem = kBar + 128;
-  static constexpr int kTmemCols = 256;  // S: [0,128)  O_blk: [128, 128+HD)
+  static constexpr int kColO = kKeys;                 // S: [0, kKeys)  O: [kColO, kColO + HD)
+  static constexpr int kTmemCols = WIN && HD == 64 ? 128 : 256;
 };
 
 // Forward pipeline.  Per key block j the CTA runs
@@ -125,17 +129,18 @@ struct FwdCfg {
 //
 // WIN: a window and sinks.  The CTA visits the key blocks of the sinks and those from its first query's window to its own; a
 // block on either border of what the rows see is masked by a 128-bit mask per row, built from the row's two ranges of keys.
-// Up to kSinkCols sinks that lie before the window are a block of kSinkCols keys.  At hd 128 (kTwin) the few blocks of a CTA
-// do not hide its set-up and its chain of dependent steps, so two CTAs share the SM: K and V in one stage each, P in tensor
-// memory over S as the A operand of P V, which leaves 96 KB of shared memory to a CTA.  S(j+1) is then issued behind P(j) V(j):
-// the other CTA's products fill the gap.  Measured: TODO
+// Up to kSinkCols sinks that lie before the window are a block of kSinkCols keys.  The few blocks of such a CTA do not hide its
+// set-up and its chain of dependent steps, so kCtas CTAs share the SM: P lies in tensor memory over S, as the A operand of
+// P V, and S(j+1) is issued behind P(j) V(j), while the products of the other CTAs fill the gap; hd 128 keeps one stage of K
+// and V, hd 64 takes 64 keys a step.
+// Measured (B200): hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: 254 -> 188 us; hd 64: TODO
 template <int HD, bool WIN>
-__global__ void __launch_bounds__(kAttnThreads, (HD == 64 || WIN) ? 2 : 1)
+__global__ void __launch_bounds__(kAttnThreads, FwdCfg<HD, WIN>::kCtas)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                 const __grid_constant__ CUtensorMap tv, const AttnArgs p) {
   using Cfg = FwdCfg<HD, WIN>;
   constexpr int S = Cfg::kStages;
-  constexpr bool kTwin = Cfg::kTwin;
+  constexpr int KB = Cfg::kKeys;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBar);
   uint64_t* q_full = bars;          // 1
@@ -156,11 +161,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   const int h = blockIdx.x % p.Hq, b = blockIdx.x / p.Hq;
   const int hk = h / (p.Hq / p.Hkv);
   const int q0 = qb * kBlk;
-  const int first_blk = WIN ? max(0, q0 - p.window + 1) / kBlk : 0;                         // of the window
-  const int n_sink_blk = WIN ? min((p.sinks + kBlk - 1) / kBlk, first_blk) : 0;
-  const int nblk = n_sink_blk + qb - first_blk + 1;
-  const bool narrow = WIN && n_sink_blk == 1 && p.sinks <= kSinkCols;   // the sinks' block is kSinkCols wide
-  auto key0 = [&](int j) { return (WIN ? (j < n_sink_blk ? j : first_blk + j - n_sink_blk) : j) * kBlk; };
+  const int first_blk = WIN ? max(0, q0 - p.window + 1) / KB : 0;                         // of the window
+  const int n_sink_blk = WIN ? min((p.sinks + KB - 1) / KB, first_blk) : 0;
+  const int nblk = WIN ? n_sink_blk + (min(q0 + kBlk, p.T) - 1) / KB - first_blk + 1 : qb + 1;
+  // WIN: the block with the first row's own key comes first, in which every row sees something (a row that has seen nothing yet
+  // moves its maximum, and O with it, at its next block), then the later ones of the tile, the earlier ones, the sinks
+  const int own_blk = q0 / KB, n_own = nblk - n_sink_blk - (own_blk - first_blk), last_sink = WIN && n_sink_blk ? nblk - 1 : -1;
+  const int narrow = n_sink_blk == 1 && p.sinks <= kSinkCols ? last_sink : -1;   // the step whose block is kSinkCols wide
+  auto key0 = [&](int j) {
+    return (!WIN ? j : j < n_own ? own_blk + j : j < nblk - n_sink_blk ? own_blk - 1 - (j - n_own) : j - (nblk - n_sink_blk)) * KB;
+  };
 
   if (threadIdx.x == 0) {
     ptx::mbar_init(q_full, 1);
@@ -188,14 +198,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   const uint32_t tmem_base = *tmem_slot;
   dependency_wait();
   dependents_launch();
-  const uint32_t tS = tmem_base, tO = tmem_base + 128;
+  const uint32_t tS = tmem_base, tO = tmem_base + Cfg::kColO;
   const bool bad_align = (*abort_flag != 0);
 
   if (bad_align) {
     // fall through to the common exit
   } else if (warp == 0) {
     if (ptx::elect_one()) {
-      ptx::mbar_expect_tx(q_full, Cfg::kTileBytes);
+      ptx::mbar_expect_tx(q_full, Cfg::kQBytes);
 #pragma unroll
       for (int c = 0; c < HD / 64; ++c)
         ptx::tma_load_3d(smem + Cfg::kQ + c * kChunkBytes, &tq, q_full, h * HD + c * 64, q0, b);
@@ -205,19 +215,19 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         ptx::mbar_expect_tx(&k_full[st], Cfg::kTileBytes);
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c)
-          ptx::tma_load_3d(smem + Cfg::kK + st * Cfg::kTileBytes + c * kChunkBytes, &tk, &k_full[st], hk * HD + c * 64,
+          ptx::tma_load_3d(smem + Cfg::kK + st * Cfg::kTileBytes + c * Cfg::kKvChunk, &tk, &k_full[st], hk * HD + c * 64,
                            key0(j), b);
         if (!ptx::mbar_wait(&v_empty[st], ((j / S) & 1) ^ 1u, abort_flag)) break;
         ptx::mbar_expect_tx(&v_full[st], Cfg::kTileBytes);
 #pragma unroll
         for (int c = 0; c < HD / 64; ++c)
-          ptx::tma_load_3d(smem + Cfg::kV + st * Cfg::kTileBytes + c * kChunkBytes, &tv, &v_full[st], hk * HD + c * 64,
+          ptx::tma_load_3d(smem + Cfg::kV + st * Cfg::kTileBytes + c * Cfg::kKvChunk, &tv, &v_full[st], hk * HD + c * 64,
                            key0(j), b);
       }
     }
   } else if (warp == 1) {
     if (ptx::elect_one()) {
-      const uint32_t idesc_s = ptx::make_idesc_bf16(128, 128, 0, 0);
+      const uint32_t idesc_s = ptx::make_idesc_bf16(128, KB, 0, 0);
       const uint32_t idesc_o = ptx::make_idesc_bf16(128, HD, 0, 1);
       const uint32_t idesc_sink = ptx::make_idesc_bf16(128, kSinkCols, 0, 0);
       const uint32_t q_base = ptx::smem_u32(smem + Cfg::kQ);
@@ -225,14 +235,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       const uint64_t q_desc = ptx::make_smem_desc(q_base, 16, 1024);
       const uint64_t k_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + Cfg::kK), 16, 1024);
       const uint64_t p_desc = ptx::make_smem_desc(p_base, 16, 1024);
-      const uint64_t v_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + Cfg::kV), kChunkBytes, 1024);
+      const uint64_t v_desc0 = ptx::make_smem_desc(ptx::smem_u32(smem + Cfg::kV), Cfg::kKvChunk, 1024);
       auto issue_s = [&](int j) {
         const uint64_t k_desc = desc_add(k_desc0, (j % S) * Cfg::kTileBytes);
-        const uint32_t idesc = WIN && narrow && j == 0 ? idesc_sink : idesc_s;
+        const uint32_t idesc = WIN && j == narrow ? idesc_sink : idesc_s;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t off = (k >> 2) * kChunkBytes + (k & 3) * 32;
-          ptx::mma_f16_ss(tS, desc_add(q_desc, off), desc_add(k_desc, off), idesc, k > 0);
+          const uint32_t off = (k >> 2) * kChunkBytes + (k & 3) * 32, k_off = (k >> 2) * Cfg::kKvChunk + (k & 3) * 32;
+          ptx::mma_f16_ss(tS, desc_add(q_desc, off), desc_add(k_desc, k_off), idesc, k > 0);
         }
         ptx::tc_commit(s_full);
         ptx::tc_commit(&k_empty[j % S]);   // the K tile may be refilled once this product has finished
@@ -243,7 +253,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         issue_s(0);
       }
       for (int j = 0; j < nblk && ok; ++j) {
-        if (!kTwin && j + 1 < nblk) {
+        if (!WIN && j + 1 < nblk) {
           // S(j+1) goes into the score columns as soon as S(j) has been copied to registers
           if (!ptx::mbar_wait(&k_full[(j + 1) % S], ((j + 1) / S) & 1, abort_flag)) break;
           if (!ptx::mbar_wait(s_free, j & 1, abort_flag)) break;
@@ -254,19 +264,19 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         if (!ptx::mbar_wait(p_full, j & 1, abort_flag)) break;
         ptx::tc_fence_after_sync();
         const uint64_t v_desc = desc_add(v_desc0, (j % S) * Cfg::kTileBytes);
-        const int steps = WIN && narrow && j == 0 ? kSinkCols / 16 : kBlk / 16;
+        const int steps = WIN && j == narrow ? kSinkCols / 16 : KB / 16;
 #pragma unroll
-        for (int k = 0; k < kBlk / 16; ++k) {
+        for (int k = 0; k < KB / 16; ++k) {
           if (WIN && k >= steps) break;
           const uint32_t a_off = (k >> 2) * kChunkBytes + (k & 3) * 32;
-          if constexpr (kTwin)
+          if constexpr (WIN)
             ptx::mma_f16_ts(tO, tS + k * 8, desc_add(v_desc, k * 2048), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
           else
             ptx::mma_f16_ss(tO, desc_add(p_desc, a_off), desc_add(v_desc, k * 2048), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
         }
         ptx::tc_commit(o_full);
         ptx::tc_commit(&v_empty[j % S]);
-        if (kTwin && j + 1 < nblk) {
+        if (WIN && j + 1 < nblk) {
           // products run in the order of their issue: P(j) V(j) has read P before S(j+1) takes its columns
           if (!ptx::mbar_wait(&k_full[(j + 1) % S], ((j + 1) / S) & 1, abort_flag)) break;
           ptx::tc_fence_after_sync();
@@ -287,101 +297,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
     for (int j = 0; j < nblk; ++j) {
       if (!ptx::mbar_wait_warp(s_full, j & 1, abort_flag)) { ok = false; break; }
       ptx::tc_fence_after_sync();
-      if (WIN && narrow && j == 0) {
-        // the sinks: all of them lie before the rows' windows
-        uint32_t r[16], pk[16];
-        ptx::tmem_ld16(tS + lane_sel, r);
-        ptx::tmem_ld_wait();
-        ptx::tc_fence_before_sync();
-        __syncwarp();
-        if (!kTwin && lane == 0) ptx::mbar_arrive(s_free);
-        float top = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < kSinkCols; ++e) {
-          if (e >= p.sinks) r[e] = __float_as_uint(-INFINITY);
-          top = fmaxf(top, __uint_as_float(r[e]));
+      // Moves the reference maximum, and O with it, when a block's maximum exceeds it by too much.
+      bool waited_o = WIN || j == 0;   // WIN: S(j) was issued behind the product before
+      auto settle = [&](float m_blk) {
+        if (j == 0) {
+          m_ref = m_blk;
+          return true;
         }
-        m_ref = top * sc;
-        const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
-        float rs0 = 0.f, rs1 = 0.f;
-#pragma unroll
-        for (int e = 0; e < kSinkCols; e += 2) {
-          const float p0 = ex2(fmaf(__uint_as_float(r[e]), sc, neg)), p1 = ex2(fmaf(__uint_as_float(r[e + 1]), sc, neg));
-          rs0 += p0;
-          rs1 += p1;
-          pk[e >> 1] = pack_bf16x2(p0, p1);
-          pk[8 + (e >> 1)] = 0u;
-        }
-        l += rs0 + rs1;
-        if constexpr (kTwin) {
-          ptx::tmem_st16(tS + lane_sel, pk);
-          ptx::tmem_st_wait();
-        } else {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            *reinterpret_cast<uint4*>(p_smem + swz_off(row, u)) = make_uint4(pk[u * 4], pk[u * 4 + 1], pk[u * 4 + 2], pk[u * 4 + 3]);
-          ptx::fence_proxy_async_smem();
-        }
-        ptx::tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(p_full);
-        continue;
-      }
-      uint32_t r0[32], r1[32], r2[32], r3[32];
-      ptx::tmem_ld32(tS + lane_sel + 0, r0);
-      ptx::tmem_ld32(tS + lane_sel + 32, r1);
-      ptx::tmem_ld32(tS + lane_sel + 64, r2);
-      ptx::tmem_ld32(tS + lane_sel + 96, r3);
-      ptx::tmem_ld_wait();
-      ptx::tc_fence_before_sync();
-      __syncwarp();
-      if (!kTwin && lane == 0) ptx::mbar_arrive(s_free);   // the score columns may be overwritten by S(j+1)
-      const int kv0 = key0(j);
-      if (WIN) {
-        // a block before the rows' own in which the last row's window does not begin yet, or that lies among the sinks: whole
-        const bool whole = kv0 != q0 && (kv0 + p.window > q0 + kBlk - 1 || kv0 + kBlk <= p.sinks);
-        if (!whole) {
-          const uint32_t ninf = __float_as_uint(-INFINITY);
-          const int sink_end = p.sinks - kv0, lo = q_idx - p.window + 1 - kv0, hi = q_idx + 1 - kv0;
-          auto mask_chunk = [&](uint32_t (&r)[32], int c) {
-            // both ranges end with the row's own key
-            const uint32_t see = bit_range(-32 * c, min(sink_end, hi) - 32 * c) | bit_range(lo - 32 * c, hi - 32 * c);
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(see & (1u << e))) r[e] = ninf;
-          };
-          mask_chunk(r0, 0);
-          mask_chunk(r1, 1);
-          mask_chunk(r2, 2);
-          mask_chunk(r3, 3);
-        }
-      } else if (j == qb) {  // diagonal block: keys after the query are masked
-        const uint32_t ninf = __float_as_uint(-INFINITY);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          if (kv0 + e > q_idx) r0[e] = ninf;
-          if (kv0 + 32 + e > q_idx) r1[e] = ninf;
-          if (kv0 + 64 + e > q_idx) r2[e] = ninf;
-          if (kv0 + 96 + e > q_idx) r3[e] = ninf;
-        }
-      }
-      float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 32; e += 2) {
-        mx0 = max3(mx0, __uint_as_float(r0[e]), __uint_as_float(r0[e + 1]));
-        mx1 = max3(mx1, __uint_as_float(r1[e]), __uint_as_float(r1[e + 1]));
-        mx2 = max3(mx2, __uint_as_float(r2[e]), __uint_as_float(r2[e + 1]));
-        mx3 = max3(mx3, __uint_as_float(r3[e]), __uint_as_float(r3[e + 1]));
-      }
-      const float m_blk = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sc;
-      bool waited_o = kTwin || j == 0;   // kTwin: S(j) was issued behind the product before
-      if (j == 0) {
-        m_ref = m_blk;
-      } else {
         const bool need = m_blk > m_ref + kLazy;
         if (__any_sync(0xffffffffu, need)) {
           // the previous P V product must have landed before O is rescaled in place
-          if (!waited_o && !ptx::mbar_wait_warp(o_full, (j - 1) & 1, abort_flag)) { ok = false; break; }
+          if (!waited_o && !ptx::mbar_wait_warp(o_full, (j - 1) & 1, abort_flag)) return false;
           ptx::tc_fence_after_sync();
           waited_o = true;
           const float alpha = need ? ex2(m_ref - m_blk) : 1.f;
@@ -398,7 +324,78 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           l *= alpha;
           if (need) m_ref = m_blk;
         }
+        return true;
+      };
+      if (WIN && j == narrow) {
+        // the sinks: all of them lie before the rows' windows
+        uint32_t r[16], pk[16];
+        ptx::tmem_ld16(tS + lane_sel, r);
+        ptx::tmem_ld_wait();
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < kSinkCols; ++e) {
+          if (e >= p.sinks) r[e] = __float_as_uint(-INFINITY);
+          top = fmaxf(top, __uint_as_float(r[e]));
+        }
+        if (!settle(top * sc)) { ok = false; break; }
+        const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
+        float rs0 = 0.f, rs1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < kSinkCols; e += 2) {
+          const float p0 = ex2(fmaf(__uint_as_float(r[e]), sc, neg)), p1 = ex2(fmaf(__uint_as_float(r[e + 1]), sc, neg));
+          rs0 += p0;
+          rs1 += p1;
+          pk[e >> 1] = pack_bf16x2(p0, p1);
+          pk[8 + (e >> 1)] = 0u;
+        }
+        l += rs0 + rs1;
+        ptx::tmem_st16(tS + lane_sel, pk);
+        ptx::tmem_st_wait();
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(p_full);
+        continue;
       }
+      uint32_t r[KB / 32][32];
+#pragma unroll
+      for (int c = 0; c < KB / 32; ++c) ptx::tmem_ld32(tS + lane_sel + 32 * c, r[c]);
+      ptx::tmem_ld_wait();
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      if (!WIN && lane == 0) ptx::mbar_arrive(s_free);   // the score columns may be overwritten by S(j+1)
+      const int kv0 = key0(j);
+      if (WIN) {
+        // a block before the tile's rows in which the last row's window does not begin yet, or that lies among the sinks: whole
+        const bool whole = kv0 + KB <= q0 && (kv0 + p.window > q0 + kBlk - 1 || kv0 + KB <= p.sinks);
+        if (!whole) {
+          const uint32_t ninf = __float_as_uint(-INFINITY);
+          const int sink_end = p.sinks - kv0, lo = q_idx - p.window + 1 - kv0, hi = q_idx + 1 - kv0;
+#pragma unroll
+          for (int c = 0; c < KB / 32; ++c) {
+            // both ranges end with the row's own key
+            const uint32_t see = bit_range(-32 * c, min(sink_end, hi) - 32 * c) | bit_range(lo - 32 * c, hi - 32 * c);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(see & (1u << e))) r[c][e] = ninf;
+          }
+        }
+      } else if (j == qb) {  // diagonal block: keys after the query are masked
+        const uint32_t ninf = __float_as_uint(-INFINITY);
+#pragma unroll
+        for (int c = 0; c < KB / 32; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (kv0 + 32 * c + e > q_idx) r[c][e] = ninf;
+      }
+      float mx[KB / 32];
+#pragma unroll
+      for (int c = 0; c < KB / 32; ++c) mx[c] = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 32; e += 2)
+#pragma unroll
+        for (int c = 0; c < KB / 32; ++c) mx[c] = max3(mx[c], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
+      const float m_blk = (KB == 128 ? fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[KB / 32 - 2], mx[KB / 32 - 1])) : fmaxf(mx[0], mx[1])) * sc;
+      if (!settle(m_blk)) { ok = false; break; }
       const float neg = WIN && m_ref == -INFINITY ? 0.f : -m_ref;   // a row may see nothing of its first blocks
       float rs0 = 0.f, rs1 = 0.f;
       auto exp_chunk = [&](uint32_t (&r)[32], int c) {
@@ -416,7 +413,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           // P(j-1) V(j-1) must have finished reading the P buffer before it is overwritten
           if (!ptx::mbar_wait_warp(o_full, (j - 1) & 1, abort_flag)) ok = false;
         }
-        if constexpr (kTwin) {
+        if constexpr (WIN) {
           ptx::tmem_st16(tS + lane_sel + c * 16, pk);
           return;
         }
@@ -425,13 +422,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           *reinterpret_cast<uint4*>(p_smem + swz_off(row, c * 4 + u)) =
               make_uint4(pk[u * 4], pk[u * 4 + 1], pk[u * 4 + 2], pk[u * 4 + 3]);
       };
-      exp_chunk(r0, 0);
+      exp_chunk(r[0], 0);
       if (!ok) break;
-      exp_chunk(r1, 1);
-      exp_chunk(r2, 2);
-      exp_chunk(r3, 3);
+#pragma unroll
+      for (int c = 1; c < KB / 32; ++c) exp_chunk(r[c], c);
       l += rs0 + rs1;
-      if constexpr (kTwin) ptx::tmem_st_wait();
+      if constexpr (WIN) ptx::tmem_st_wait();
       else ptx::fence_proxy_async_smem();
       ptx::tc_fence_before_sync();
       __syncwarp();
@@ -1037,8 +1033,8 @@ static int attn_fwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 
   const uint64_t B = d->B, T = d->T, wq = static_cast<uint64_t>(d->Hq) * HD, wkv = static_cast<uint64_t>(d->Hkv) * HD;
   CUtensorMap tq, tk, tv;
   if (!make_tmap_tokens(&tq, d->q, 0, wq, T, B, d->q_stride_t, 64, kBlk) ||
-      !make_tmap_tokens(&tk, d->k, 0, wkv, T, B, d->k_stride_t, 64, kBlk) ||
-      !make_tmap_tokens(&tv, d->v, 0, wkv, T, B, d->v_stride_t, 64, kBlk))
+      !make_tmap_tokens(&tk, d->k, 0, wkv, T, B, d->k_stride_t, 64, Cfg::kKeys) ||
+      !make_tmap_tokens(&tv, d->v, 0, wkv, T, B, d->v_stride_t, 64, Cfg::kKeys))
     return TITB_ERR_TENSOR_MAP;
   AttnArgs a{};
   a.B = d->B; a.T = d->T; a.Hq = d->Hq; a.Hkv = d->Hkv; a.hd = HD;
