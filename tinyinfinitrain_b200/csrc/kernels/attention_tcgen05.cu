@@ -95,20 +95,22 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
 // ------------------------------------------------------------------------- forward
 template <int HD, bool WIN>
 struct FwdCfg {
-  static constexpr int kKeys = WIN && HD == 64 ? 64 : kBlk;   // keys of a step
-  static constexpr int kCtas = !WIN ? (HD == 64 ? 2 : 1) : HD == 64 ? 3 : 2;   // that share an SM
+  static constexpr int kKeys = WIN ? 64 : kBlk;      // keys of a step
+  static constexpr int kCtas = WIN ? (HD == 64 ? 3 : 2) : HD == 64 ? 2 : 1;   // that share an SM
   static constexpr int kTileBytes = kKeys * HD * 2;  // K or V tile
   static constexpr int kKvChunk = kKeys * 128;       // its [keys x 64 bf16] sub-tiles
-  static constexpr int kStages = WIN && HD == 128 ? 1 : 2;
+  static constexpr int kStages = 2;
   static constexpr int kQ = 0;
   static constexpr int kQBytes = kBlk * HD * 2;
   static constexpr int kK = kQ + kQBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
   static constexpr int kP = kV + kStages * kTileBytes;
-  static constexpr int kBar = kP + (WIN ? 0 : kBlk * kBlk * 2);   // WIN: P lies over S in tensor memory
+  static constexpr int kBar = kP + (WIN ? 0 : kBlk * kBlk * 2);   // WIN: P lies in tensor memory
   static constexpr int kSmem = kBar + 128;
-  static constexpr int kColO = kKeys;                 // S: [0, kKeys)  O: [kColO, kColO + HD)
+  // S: [0, kKeys)  O: [kColO, kColO + HD); WIN: P takes 32 columns, at 64 beside O of 128, else in a second allocation
+  static constexpr int kColO = HD == 128 ? 128 : kKeys;
   static constexpr int kTmemCols = WIN && HD == 64 ? 128 : 256;
+  static constexpr int kTmemColsP = WIN && HD == 64 ? 32 : 0;
 };
 
 // Forward pipeline.  Per key block j the CTA runs
@@ -130,10 +132,10 @@ struct FwdCfg {
 // WIN: a window and sinks.  The CTA visits the key blocks of the sinks and those from its first query's window to its own; a
 // block on either border of what the rows see is masked by a 128-bit mask per row, built from the row's two ranges of keys.
 // Up to kSinkCols sinks that lie before the window are a block of kSinkCols keys.  The few blocks of such a CTA do not hide its
-// set-up and its chain of dependent steps, so kCtas CTAs share the SM: P lies in tensor memory over S, as the A operand of
-// P V, and S(j+1) is issued behind P(j) V(j), while the products of the other CTAs fill the gap; hd 128 keeps one stage of K
-// and V, hd 64 takes 64 keys a step.
-// Measured (B200): hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: 254 -> 188 us; hd 64: TODO
+// set-up and its chain of dependent steps (S, maximum, exponentials, P, P V), so kCtas CTAs share the SM, with 64 keys a step
+// and P in tensor memory, as the A operand of P V: 48 or 96 KB of shared memory and 160 or 256 columns to a CTA.
+// Measured (B200): hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: one CTA an SM 254 us, two with 128 keys a step, P over S
+// and S(j+1) issued behind P(j) V(j) 182 us, now TODO; hd 64, 1 x 1999, 32 / 8 heads, window 512: 29, 26, TODO us.
 template <int HD, bool WIN>
 __global__ void __launch_bounds__(kAttnThreads, FwdCfg<HD, WIN>::kCtas)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -154,6 +156,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   uint64_t* s_free = bars + 12;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
   volatile uint32_t* abort_flag = tmem_slot + 1;
+  uint32_t* tmem_slot_p = tmem_slot + 2;
 
   const int warp = ptx::warp_index(), lane = threadIdx.x & 31;
   const int nqb = (p.T + kBlk - 1) / kBlk;
@@ -190,6 +193,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   }
   if (warp == 1) {
     ptx::tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    if (Cfg::kTmemColsP) ptx::tmem_alloc(tmem_slot_p, Cfg::kTmemColsP);
     ptx::tmem_relinquish();
   }
   ptx::tc_fence_before_sync();
@@ -199,6 +203,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   dependency_wait();
   dependents_launch();
   const uint32_t tS = tmem_base, tO = tmem_base + Cfg::kColO;
+  const uint32_t tP = Cfg::kTmemColsP ? *tmem_slot_p : tmem_base + 64;   // WIN
   const bool bad_align = (*abort_flag != 0);
 
   if (bad_align) {
@@ -253,7 +258,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         issue_s(0);
       }
       for (int j = 0; j < nblk && ok; ++j) {
-        if (!WIN && j + 1 < nblk) {
+        if (j + 1 < nblk) {
           // S(j+1) goes into the score columns as soon as S(j) has been copied to registers
           if (!ptx::mbar_wait(&k_full[(j + 1) % S], ((j + 1) / S) & 1, abort_flag)) break;
           if (!ptx::mbar_wait(s_free, j & 1, abort_flag)) break;
@@ -270,18 +275,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           if (WIN && k >= steps) break;
           const uint32_t a_off = (k >> 2) * kChunkBytes + (k & 3) * 32;
           if constexpr (WIN)
-            ptx::mma_f16_ts(tO, tS + k * 8, desc_add(v_desc, k * 2048), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+            ptx::mma_f16_ts(tO, tP + k * 8, desc_add(v_desc, k * 2048), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
           else
             ptx::mma_f16_ss(tO, desc_add(p_desc, a_off), desc_add(v_desc, k * 2048), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
         }
         ptx::tc_commit(o_full);
         ptx::tc_commit(&v_empty[j % S]);
-        if (WIN && j + 1 < nblk) {
-          // products run in the order of their issue: P(j) V(j) has read P before S(j+1) takes its columns
-          if (!ptx::mbar_wait(&k_full[(j + 1) % S], ((j + 1) / S) & 1, abort_flag)) break;
-          ptx::tc_fence_after_sync();
-          issue_s(j + 1);
-        }
       }
     }
   } else {
@@ -298,7 +297,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       if (!ptx::mbar_wait_warp(s_full, j & 1, abort_flag)) { ok = false; break; }
       ptx::tc_fence_after_sync();
       // Moves the reference maximum, and O with it, when a block's maximum exceeds it by too much.
-      bool waited_o = WIN || j == 0;   // WIN: S(j) was issued behind the product before
+      bool waited_o = (j == 0);
       auto settle = [&](float m_blk) {
         if (j == 0) {
           m_ref = m_blk;
@@ -331,6 +330,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         uint32_t r[16], pk[16];
         ptx::tmem_ld16(tS + lane_sel, r);
         ptx::tmem_ld_wait();
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(s_free);
         float top = -INFINITY;
 #pragma unroll
         for (int e = 0; e < kSinkCols; ++e) {
@@ -349,7 +351,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           pk[8 + (e >> 1)] = 0u;
         }
         l += rs0 + rs1;
-        ptx::tmem_st16(tS + lane_sel, pk);
+        if (!waited_o && !ptx::mbar_wait_warp(o_full, (j - 1) & 1, abort_flag)) { ok = false; break; }
+        ptx::tmem_st16(tP + lane_sel, pk);
         ptx::tmem_st_wait();
         ptx::tc_fence_before_sync();
         __syncwarp();
@@ -362,7 +365,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       ptx::tmem_ld_wait();
       ptx::tc_fence_before_sync();
       __syncwarp();
-      if (!WIN && lane == 0) ptx::mbar_arrive(s_free);   // the score columns may be overwritten by S(j+1)
+      if (lane == 0) ptx::mbar_arrive(s_free);   // the score columns may be overwritten by S(j+1)
       const int kv0 = key0(j);
       if (WIN) {
         // a block before the tile's rows in which the last row's window does not begin yet, or that lies among the sinks: whole
@@ -414,7 +417,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           if (!ptx::mbar_wait_warp(o_full, (j - 1) & 1, abort_flag)) ok = false;
         }
         if constexpr (WIN) {
-          ptx::tmem_st16(tS + lane_sel + c * 16, pk);
+          if (ok) ptx::tmem_st16(tP + lane_sel + c * 16, pk);
           return;
         }
 #pragma unroll
@@ -465,6 +468,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   if (warp == 1) {
     __syncwarp();
     ptx::tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    if (Cfg::kTmemColsP) ptx::tmem_dealloc(*tmem_slot_p, Cfg::kTmemColsP);
   }
   if (threadIdx.x == 0 && *abort_flag) atomicExch(p.status, kStatusMbarTimeout);
 }
