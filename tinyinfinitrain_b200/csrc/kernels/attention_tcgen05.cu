@@ -441,12 +441,23 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       ptx::tc_fence_after_sync();
       const float inv = 1.f / l;
       bf16* dst = p.o + (static_cast<long long>(b) * p.T + q_idx) * p.o_stride_t + h * HD;
+      uint8_t* q_smem = smem + Cfg::kQ;   // WIN: no product reads Q any more
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t r[32];
         ptx::tmem_ld32(tO + lane_sel + c * 32, r);
         ptx::tmem_ld_wait();
-        if (q_idx < p.T) {
+        if constexpr (WIN) {
+#pragma unroll
+          for (int d = 0; d < 32; d += 8) {
+            uint4 u;
+            u.x = pack_bf16x2(__uint_as_float(r[d]) * inv, __uint_as_float(r[d + 1]) * inv);
+            u.y = pack_bf16x2(__uint_as_float(r[d + 2]) * inv, __uint_as_float(r[d + 3]) * inv);
+            u.z = pack_bf16x2(__uint_as_float(r[d + 4]) * inv, __uint_as_float(r[d + 5]) * inv);
+            u.w = pack_bf16x2(__uint_as_float(r[d + 6]) * inv, __uint_as_float(r[d + 7]) * inv);
+            *reinterpret_cast<uint4*>(q_smem + swz_off(row, c * 4 + d / 8)) = u;
+          }
+        } else if (q_idx < p.T) {
 #pragma unroll
           for (int d = 0; d < 32; d += 8) {
             uint4 u;
@@ -456,6 +467,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
             u.w = pack_bf16x2(__uint_as_float(r[d + 6]) * inv, __uint_as_float(r[d + 7]) * inv);
             *reinterpret_cast<uint4*>(dst + c * 32 + d) = u;
           }
+        }
+      }
+      if constexpr (WIN) {
+        // a warp's rows leave as whole rows: a store of one unit per row and lane would take a transaction for each
+        __syncwarp();
+#pragma unroll 4
+        for (int i = lane; i < 32 * (HD / 8); i += 32) {
+          const int r = quad * 32 + i / (HD / 8), u = i % (HD / 8);
+          if (q0 + r < p.T)
+            *reinterpret_cast<uint4*>(p.o + (static_cast<long long>(b) * p.T + q0 + r) * p.o_stride_t + h * HD + u * 8) =
+                *reinterpret_cast<const uint4*>(q_smem + swz_off(r, u));
         }
       }
       if (q_idx < p.T)
@@ -519,7 +541,7 @@ struct BwdCfg {
 //
 // WIN: a window and sinks.  A block of keys meets the query blocks up to its last key's window.  A block that holds sinks meets
 // all later ones, which would make its CTA the last by far: its query blocks are split over sink_parts CTAs, which leave
-// fp32 sums that attn_sink_join_kernel adds in order.
+// fp32 sums of the sinks' rows that attn_window_finish_kernel adds in order.
 template <int HD, bool WIN>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -904,13 +926,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           uint32_t r[32];
           ptx::tmem_ld32(tmem_base + col + lane_sel + c * 32, r);
           ptx::tmem_ld_wait();
-          if (sink_cta && p.sink_parts > 1) {
+          if (sink_cta && p.sink_parts > 1 && kv_idx < p.sinks) {
             float* sum = p.sink_part + ((((static_cast<long long>(part) * p.B + b) * p.sink_blocks + jb) * p.Hkv + hk) * 2 + 1 - which) * (kBlk * HD) +
                          row * HD + c * 32;
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
               *reinterpret_cast<uint4*>(sum + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
-          } else if (kv_idx < p.T) {
+          } else if (kv_idx < p.T && part == 0) {   // the first part holds all queries that see the other keys of the block
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
               uint4 u;
@@ -987,28 +1009,43 @@ __global__ void attn_dq_convert_kernel(const float* __restrict__ acc, bf16* __re
   }
 }
 
-// dK and dV of the sinks' blocks: the sums of their parts, in order.  One thread per four elements of a row.
+// The end of the backward pass of window attention: dq from its accumulator, and dK and dV of the sinks, whose parts are
+// added in order.
 template <int HD>
-__global__ void attn_sink_join_kernel(const AttnArgs p) {
-  const int nqb = (p.T + kBlk - 1) / kBlk, rows = min(p.T, p.sink_blocks * kBlk);
-  const long long n = static_cast<long long>(p.B) * rows * p.Hkv * 2 * (HD / 4);
+__global__ void attn_window_finish_kernel(const AttnArgs p, bf16* __restrict__ dq, long long dq_stride_t) {
+  dependents_launch();
+  const int width = p.Hq * HD, wv = width / 8, nqb = (p.T + kBlk - 1) / kBlk;
+  const long long n_dq = static_cast<long long>(p.B) * p.T * wv;
+  const long long n_sink = p.sink_parts > 1 ? static_cast<long long>(p.B) * p.sinks * p.Hkv * 2 * (HD / 4) : 0;
   const long long part_size = static_cast<long long>(p.B) * p.sink_blocks * p.Hkv * 2 * kBlk * HD;
-  for (long long x = blockIdx.x * (long long)blockDim.x + threadIdx.x; x < n; x += (long long)gridDim.x * blockDim.x) {
-    const int d = static_cast<int>(x % (HD / 4)) * 4;
-    long long r = x / (HD / 4);
-    const int which = static_cast<int>(r % 2), hk = static_cast<int>(r / 2 % p.Hkv);
-    r = r / 2 / p.Hkv;
-    const int t = static_cast<int>(r % rows), b = static_cast<int>(r / rows), jb = t / kBlk;
-    const float* src = p.sink_part + (((static_cast<long long>(b) * p.sink_blocks + jb) * p.Hkv + hk) * 2 + which) * (kBlk * HD) + (t % kBlk) * HD + d;
-    const int parts = (nqb - jb + p.sink_step - 1) / p.sink_step;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < parts; ++c) {
-      const float4 f = *reinterpret_cast<const float4*>(src + c * part_size);
-      sum.x += f.x; sum.y += f.y; sum.z += f.z; sum.w += f.w;
+  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n_sink + n_dq; i += (long long)gridDim.x * blockDim.x) {
+    if (i < n_sink) {
+      const int d = static_cast<int>(i % (HD / 4)) * 4;
+      long long r = i / (HD / 4);
+      const int which = static_cast<int>(r % 2), hk = static_cast<int>(r / 2 % p.Hkv);
+      r = r / 2 / p.Hkv;
+      const int t = static_cast<int>(r % p.sinks), b = static_cast<int>(r / p.sinks), jb = t / kBlk;
+      const float* src = p.sink_part + (((static_cast<long long>(b) * p.sink_blocks + jb) * p.Hkv + hk) * 2 + which) * (kBlk * HD) + (t % kBlk) * HD + d;
+      const int parts = (nqb - jb + p.sink_step - 1) / p.sink_step;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int c = 0; c < parts; ++c) {
+        const float4 f = *reinterpret_cast<const float4*>(src + c * part_size);
+        sum.x += f.x; sum.y += f.y; sum.z += f.z; sum.w += f.w;
+      }
+      const long long bt = static_cast<long long>(b) * p.T + t;
+      bf16* dst = (which == 0 ? p.dk + bt * p.dk_stride_t : p.dv + bt * p.dv_stride_t) + hk * HD + d;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+      continue;
     }
-    const long long bt = static_cast<long long>(b) * p.T + t;
-    bf16* dst = (which == 0 ? p.dk + bt * p.dk_stride_t : p.dv + bt * p.dv_stride_t) + hk * HD + d;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+    const long long bt = (i - n_sink) / wv;
+    const int c = static_cast<int>(i - n_sink - bt * wv) * 8;
+    const float4 f0 = *reinterpret_cast<const float4*>(p.dq_accum + bt * width + c);
+    const float4 f1 = *reinterpret_cast<const float4*>(p.dq_accum + bt * width + c + 4);
+    uint4 u;
+    u.x = pack_bf16x2(f0.x, f0.y); u.y = pack_bf16x2(f0.z, f0.w);
+    u.z = pack_bf16x2(f1.x, f1.y); u.w = pack_bf16x2(f1.z, f1.w);
+    *reinterpret_cast<uint4*>(dq + bt * dq_stride_t + c) = u;
   }
 }
 
@@ -1107,15 +1144,14 @@ static int attn_bwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 
   }
   dim3 grid(static_cast<unsigned>(d->Hkv) * d->B, jobs);
   launch_dependent(attn_bwd_kernel<HD, WIN>, grid, kBwdThreads, Cfg::kSmem, st, tq, tk, tv, tdo, tdq, a);
-  if (WIN && a.sink_blocks > 0 && a.sink_parts > 1) {
-    const int rows = a.sink_blocks * kBlk < d->T ? a.sink_blocks * kBlk : d->T;
-    const long long blocks = (static_cast<long long>(d->B) * rows * d->Hkv * 2 * (HD / 4) + 255) / 256, most = device_sm_count() * 8LL;
-    attn_sink_join_kernel<HD><<<static_cast<int>(blocks < most ? blocks : most), 256, 0, st>>>(a);
-  }
   const long long bt = static_cast<long long>(d->B) * d->T;
   const int width = d->Hq * HD;
   int cb = static_cast<int>((bt * (width / 8) + 255) / 256);
   if (cb > device_sm_count() * 8) cb = device_sm_count() * 8;
+  if (WIN) {
+    attn_window_finish_kernel<HD><<<cb, 256, 0, st>>>(a, static_cast<bf16*>(d->dq), d->dq_stride_t);
+    return static_cast<int>(cudaGetLastError());
+  }
   attn_dq_convert_kernel<<<cb, 256, 0, st>>>(d->dq_accum, static_cast<bf16*>(d->dq), bt, width, d->dq_stride_t);
   return static_cast<int>(cudaGetLastError());
 }

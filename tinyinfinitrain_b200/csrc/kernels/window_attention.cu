@@ -359,20 +359,21 @@ __global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p
     accumulate<HD>(dv, Ps, Ds, ty, tx);
     accumulate<HD>(dk, Ss, Qs, ty, tx);
   }
-  if (sink_cta && p.sink_parts > 1) {
-    float* sum = p.sink_part + (((static_cast<long long>(part) * p.B + b) * p.sink_tiles + tile) * p.Hkv + hk) * 2 * kWinRows * p.hd;
-    store_rows<float, HD>(sum, p.hd, 0, kWinRows, p.hd, dk, ty, tx);
-    store_rows<float, HD>(sum + kWinRows * p.hd, p.hd, 0, kWinRows, p.hd, dv, ty, tx);
-  } else {
+  if (part == 0) {   // holds all queries that see keys of the tile that are no sinks
     store_rows<T, HD>(static_cast<T*>(p.dk) + row0 * p.dk_st + hk * p.hd, p.dk_st, k0, p.T, p.hd, dk, ty, tx);
     store_rows<T, HD>(static_cast<T*>(p.dv) + row0 * p.dv_st + hk * p.hd, p.dv_st, k0, p.T, p.hd, dv, ty, tx);
   }
+  if (sink_cta && p.sink_parts > 1) {
+    float* sum = p.sink_part + (((static_cast<long long>(part) * p.B + b) * p.sink_tiles + tile) * p.Hkv + hk) * 2 * kWinRows * p.hd;
+    store_rows<float, HD>(sum, p.hd, 0, p.sinks - k0, p.hd, dk, ty, tx);
+    store_rows<float, HD>(sum + kWinRows * p.hd, p.hd, 0, p.sinks - k0, p.hd, dv, ty, tx);
+  }
 }
 
-// dK and dV of the sinks' tiles: the sums of their parts, in order.
+// dK and dV of the sinks: the sums of their parts, in order, over what part 0 left.
 template <typename T>
 __global__ void window_join_kernel(const WinArgs p) {
-  const int rows = min(p.T, p.sink_tiles * kWinRows), steps = (p.T + kWinStep - 1) / kWinStep;
+  const int rows = p.sinks, steps = (p.T + kWinStep - 1) / kWinStep;
   const long long n = static_cast<long long>(p.B) * rows * p.Hkv * 2 * p.hd;
   const long long part_size = static_cast<long long>(p.B) * p.sink_tiles * p.Hkv * 2 * kWinRows * p.hd;
   for (long long x = blockIdx.x * (long long)blockDim.x + threadIdx.x; x < n; x += (long long)gridDim.x * blockDim.x) {
