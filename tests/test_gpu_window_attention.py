@@ -190,3 +190,40 @@ def test_captured_step_beside_an_eager_one(dtype, hd):
             s.copy_(t)
         graph.replay()
         _compare(*new, 100, 4, captured)
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_a_second_derivative_is_refused(fused):
+    """The gradients of a recorded backward pass are values like any; differentiating them is an error."""
+    q, k, v, do = _inputs(1, 20, 2, 1, 64, F32)
+    leaves = [_fused(q, k, v).requires_grad_()] if fused else [t.requires_grad_() for t in (q, k, v)]
+    o = ops.window_attention_qkv(leaves[0], 2, 1, 5) if fused else ops.window_attention(*leaves, 5)
+    first = torch.autograd.grad(o, leaves, do, create_graph=True)
+    again = torch.autograd.grad(ops.window_attention_qkv(leaves[0], 2, 1, 5) if fused else ops.window_attention(*leaves, 5), leaves, do)
+    assert all(torch.equal(a.detach(), b) for a, b in zip(first, again))
+    with pytest.raises(RuntimeError, match="second derivative"):
+        first[0].sum().backward()
+
+
+def test_without_gradients_and_for_some_inputs_only():
+    q, k, v, do = _inputs(1, 150, 4, 2, 64, BF)
+    with torch.no_grad():
+        plain = ops.window_attention(q, k, v, 30, 2)
+    assert not plain.requires_grad
+    v.requires_grad_()
+    o = ops.window_attention(q, k, v, 30, 2)
+    assert torch.equal(o.detach(), plain)
+    o.backward(do)
+    check("dv", v.grad, attention64(q, k, v, do, visible(150, 30, 2))["dv"])
+    assert q.grad is None
+    with torch.inference_mode():
+        assert torch.equal(ops.window_attention(q, k, v, 30, 2), plain)
+    # two backward passes of one forward, and an output changed in place by the caller
+    o = ops.window_attention(q, k, v, 30, 2)
+    a = torch.autograd.grad(o, v, do, retain_graph=True)[0]
+    b = torch.autograd.grad(o, v, do)[0]
+    assert torch.equal(a, b)
+    o = ops.window_attention(q, k, v, 30, 2)
+    o.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.backward(do)

@@ -3,7 +3,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include <algorithm>
+#include <array>
 #include <climits>
 
 #include "kernels/api.h"
@@ -69,6 +72,15 @@ std::vector<Tensor> attn_bwd(const Tensor& d_o_, const Tensor& q_, const Tensor&
 }
 
 // ---- window and sinks
+void limits_check(const Tensor& t, int64_t B, int64_t T, int64_t Hq, int64_t hd, int64_t window, int64_t sinks) {
+  TORCH_CHECK(window >= 1, "titb200 window_attention: window must be at least 1, got ", window);
+  TORCH_CHECK(sinks >= 0, "titb200 window_attention: sinks must not be negative, got ", sinks);
+  if (!t.is_cuda()) return;
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat,
+              "titb200 window_attention: only float32 and bfloat16 tensors are supported, got ", t.scalar_type());
+  TORCH_CHECK(hd > 0 && hd <= 128 && hd % 8 == 0, "titb200 window_attention: head_dim must be a multiple of 8 up to 128, got ", hd);
+  TORCH_CHECK(T <= 32 * 32767LL && B * Hq < (1LL << 31), "titb200 window_attention: too many tokens or heads");
+}
 void window_check(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks) {
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "titb200 window_attention: q [B, T, Hq, hd], k and v [B, T, Hkv, hd]");
   TORCH_CHECK(k.sizes() == v.sizes(), "titb200 window_attention: k and v must have the same shape");
@@ -77,14 +89,7 @@ void window_check(const Tensor& q, const Tensor& k, const Tensor& v, int64_t win
   TORCH_CHECK(k.size(2) > 0 && q.size(2) % k.size(2) == 0, "titb200 window_attention: Hq must be a multiple of Hkv");
   TORCH_CHECK(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type() && q.device() == k.device() &&
                   q.device() == v.device(), "titb200 window_attention: q, k and v must share dtype and device");
-  TORCH_CHECK(window >= 1, "titb200 window_attention: window must be at least 1, got ", window);
-  TORCH_CHECK(sinks >= 0, "titb200 window_attention: sinks must not be negative, got ", sinks);
-  if (!q.is_cuda()) return;
-  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kFloat,
-              "titb200 window_attention: only float32 and bfloat16 tensors are supported, got ", q.scalar_type());
-  TORCH_CHECK(q.size(3) > 0 && q.size(3) <= 128 && q.size(3) % 8 == 0,
-              "titb200 window_attention: head_dim must be a multiple of 8 up to 128, got ", q.size(3));
-  TORCH_CHECK(q.size(1) <= 32 * 32767LL && q.size(0) * q.size(2) < (1LL << 31), "titb200 window_attention: too many tokens or heads");
+  limits_check(q, q.size(0), q.size(1), q.size(2), q.size(3), window, sinks);
 }
 
 // Elements between the tokens of a [B, T, H, hd] view, taken from a dimension that has more than one entry.
@@ -102,60 +107,156 @@ bool addressable(const Tensor& t) {
 }
 Tensor in_place_or_copy(const Tensor& t) { return addressable(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
-TitbWindowDesc window_desc(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale) {
+// A [B, T, H, hd] operand of the kernels: a tensor of its own, or a slice of a fused projection.
+struct Rows {
+  void* ptr;
+  int64_t stride;   // elements between tokens
+};
+Rows rows_of(const Tensor& t) { return {t.data_ptr(), token_stride(t)}; }
+struct Shape {
+  int64_t B, T, Hq, Hkv, hd;
+};
+
+TitbWindowDesc window_desc(const Shape& s, Rows q, Rows k, Rows v, at::ScalarType type, int64_t window, int64_t sinks, double scale) {
   TitbWindowDesc w{};
   TitbAttnDesc& d = w.attn;
-  d.q = q.data_ptr(); d.k = k.data_ptr(); d.v = v.data_ptr();
-  d.B = (int)q.size(0); d.T = (int)q.size(1); d.Hq = (int)q.size(2); d.Hkv = (int)k.size(2); d.hd = (int)q.size(3);
-  d.q_stride_t = token_stride(q); d.k_stride_t = token_stride(k); d.v_stride_t = token_stride(v);
+  d.q = q.ptr; d.k = k.ptr; d.v = v.ptr;
+  d.B = (int)s.B; d.T = (int)s.T; d.Hq = (int)s.Hq; d.Hkv = (int)s.Hkv; d.hd = (int)s.hd;
+  d.q_stride_t = q.stride; d.k_stride_t = k.stride; d.v_stride_t = v.stride;
+  d.o_stride_t = s.Hq * s.hd;
   d.scale = (float)scale;
   w.window = (int)std::min<int64_t>(window, INT_MAX);
   w.sinks = (int)std::min<int64_t>(sinks, INT_MAX);
-  w.dtype = q.scalar_type() == at::kBFloat16 ? 1 : 0;
+  w.dtype = type == at::kBFloat16 ? 1 : 0;
   return w;
 }
 
-std::vector<Tensor> window_attn_fwd(const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window, int64_t sinks,
-                                    double scale) {
-  TORCH_CHECK(q_.is_cuda(), "titb200 window_attention: CUDA tensors");
-  window_check(q_, k_, v_, window, sinks);
-  c10::cuda::CUDAGuard guard(q_.device());
-  Tensor q = in_place_or_copy(q_), k = in_place_or_copy(k_), v = in_place_or_copy(v_);
-  const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), hd = q.size(3);
-  Tensor o = at::empty({B, T, Hq, hd}, q.options());
-  Tensor lse = at::empty({B, Hq, T}, q.options().dtype(at::kFloat));
-  TitbWindowDesc w = window_desc(q, k, v, window, sinks, scale);
-  w.attn.o = o.data_ptr(); w.attn.lse = lse.data_ptr<float>(); w.attn.o_stride_t = Hq * hd;
+// {o [B, T, Hq, hd], lse fp32 [B, Hq, T]}
+std::pair<Tensor, Tensor> window_forward(const Shape& s, Rows q, Rows k, Rows v, const at::TensorOptions& opt, int64_t window,
+                                         int64_t sinks, double scale) {
+  Tensor o = at::empty({s.B, s.T, s.Hq, s.hd}, opt);
+  Tensor lse = at::empty({s.B, s.Hq, s.T}, opt.dtype(at::kFloat));
+  TitbWindowDesc w = window_desc(s, q, k, v, o.scalar_type(), window, sinks, scale);
+  w.attn.o = o.data_ptr(); w.attn.lse = lse.data_ptr<float>();
   check(titb_window_attn_fwd(&w, at::cuda::getCurrentCUDAStream().stream()), "window_attention");
   return {o, lse};
 }
 
-// Gradients are written into dq / dk / dv, views of the layouts that attn_bwd takes, or into fresh tensors.
-std::vector<Tensor> window_attn_bwd(const Tensor& d_o_, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& o,
-                                    const Tensor& lse, int64_t window, int64_t sinks, double scale,
-                                    const c10::optional<Tensor>& dq_, const c10::optional<Tensor>& dk_,
-                                    const c10::optional<Tensor>& dv_) {
-  window_check(q_, k_, v_, window, sinks);
-  TORCH_CHECK(d_o_.sizes() == q_.sizes() && d_o_.scalar_type() == q_.scalar_type() && d_o_.device() == q_.device(),
+void window_backward(const Shape& s, const Tensor& d_o_, Rows q, Rows k, Rows v, const Tensor& o, const Tensor& lse, Rows dq, Rows dk,
+                     Rows dv, int64_t window, int64_t sinks, double scale) {
+  TORCH_CHECK(d_o_.sizes() == o.sizes() && d_o_.scalar_type() == o.scalar_type() && d_o_.device() == o.device(),
               "titb200 window_attention: the gradient must look like the output");
-  c10::cuda::CUDAGuard guard(q_.device());
-  Tensor q = in_place_or_copy(q_), k = in_place_or_copy(k_), v = in_place_or_copy(v_), d_o = in_place_or_copy(d_o_);
-  const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), hd = q.size(3), Hkv = k.size(2);
-  Tensor dq = dq_.has_value() && dq_->defined() ? *dq_ : at::empty({B, T, Hq, hd}, q.options());
-  Tensor dk = dk_.has_value() && dk_->defined() ? *dk_ : at::empty({B, T, Hkv, hd}, q.options());
-  Tensor dv = dv_.has_value() && dv_->defined() ? *dv_ : at::empty({B, T, Hkv, hd}, q.options());
-  TORCH_CHECK(addressable(dq) && addressable(dk) && addressable(dv), "titb200 window_attention: bad gradient views");
-  Tensor delta = at::empty({B, Hq, T}, q.options().dtype(at::kFloat));
-  TitbWindowDesc w = window_desc(q, k, v, window, sinks, scale);
+  const Tensor d_o = in_place_or_copy(d_o_);
+  TitbWindowDesc w = window_desc(s, q, k, v, o.scalar_type(), window, sinks, scale);
   TitbAttnDesc& d = w.attn;
-  d.o = o.data_ptr(); d.lse = lse.data_ptr<float>(); d.o_stride_t = token_stride(o);
-  d.d_o = d_o.data_ptr(); d.dq = dq.data_ptr(); d.dk = dk.data_ptr(); d.dv = dv.data_ptr();
-  d.delta = delta.data_ptr<float>();
-  d.do_stride_t = token_stride(d_o); d.dq_stride_t = token_stride(dq); d.dk_stride_t = token_stride(dk); d.dv_stride_t = token_stride(dv);
-  Tensor work = at::empty({titb_window_attn_bwd_workspace(&w)}, q.options().dtype(at::kFloat));
-  w.workspace = work.data_ptr<float>();
+  d.o = o.data_ptr(); d.lse = lse.data_ptr<float>();
+  d.d_o = d_o.data_ptr(); d.do_stride_t = token_stride(d_o);
+  d.dq = dq.ptr; d.dk = dk.ptr; d.dv = dv.ptr;
+  d.dq_stride_t = dq.stride; d.dk_stride_t = dk.stride; d.dv_stride_t = dv.stride;
+  // one scratch buffer: delta, to a multiple of four floats, and the kernels' workspace
+  const int64_t n_delta = (s.B * s.Hq * s.T + 3) / 4 * 4;
+  Tensor scratch = at::empty({n_delta + titb_window_attn_bwd_workspace(&w)}, o.options().dtype(at::kFloat));
+  d.delta = scratch.data_ptr<float>();
+  w.workspace = d.delta + n_delta;
   check(titb_window_attn_bwd(&w, at::cuda::getCurrentCUDAStream().stream()), "window_attention backward");
-  return {dq, dk, dv};
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients of a backward pass that is itself recorded: usable as values, an error where they are differentiated.
+variable_list first_order_only(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads) g = g.detach().set_requires_grad(true);   // the error node is attached to inputs that require one
+  auto error = std::make_shared<torch::autograd::DelayedError>("titb200 window_attention has no second derivative",
+                                                               static_cast<int64_t>(grads.size()));
+  return (*error)(std::move(grads));
+}
+
+// The autograd functions are C++ ones: forward and backward through a Python one took 97 us of host time, which is more than
+// the kernels run on a few hundred tokens; 75 us now, most of it the autograd engine.
+struct WindowAttention : public torch::autograd::Function<WindowAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window, int64_t sinks,
+                        double scale) {
+    c10::cuda::CUDAGuard guard(q_.device());
+    const Tensor q = in_place_or_copy(q_), k = in_place_or_copy(k_), v = in_place_or_copy(v_);
+    const Shape s{q.size(0), q.size(1), q.size(2), k.size(2), q.size(3)};
+    auto [o, lse] = window_forward(s, rows_of(q), rows_of(k), rows_of(v), q.options(), window, sinks, scale);
+    ctx->save_for_backward({q, k, v, o, lse});
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    ctx->saved_data["scale"] = scale;
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2];
+    c10::cuda::CUDAGuard guard(q.device());
+    const Shape s{q.size(0), q.size(1), q.size(2), k.size(2), q.size(3)};
+    at::AutoDispatchBelowADInplaceOrView below;
+    Tensor dq = at::empty({s.B, s.T, s.Hq, s.hd}, q.options()), dk = at::empty({s.B, s.T, s.Hkv, s.hd}, q.options()),
+           dv = at::empty({s.B, s.T, s.Hkv, s.hd}, q.options());
+    window_backward(s, grads[0], rows_of(q), rows_of(k), rows_of(v), saved[3], saved[4], rows_of(dq), rows_of(dk), rows_of(dv),
+                    ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble());
+    grads = first_order_only({dq, dk, dv});
+    return {grads[0], grads[1], grads[2], Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// Over a fused projection buffer [B, T, (Hq + 2 Hkv) * hd]: q, k and v are read in place, the gradient has the same layout.
+struct WindowAttentionQKV : public torch::autograd::Function<WindowAttentionQKV> {
+  static std::array<Rows, 3> parts(const Tensor& qkv, const Shape& s) {
+    char* p = static_cast<char*>(qkv.data_ptr());
+    const int64_t row = s.hd * qkv.element_size(), stride = (s.Hq + 2 * s.Hkv) * s.hd;
+    return {Rows{p, stride}, Rows{p + s.Hq * row, stride}, Rows{p + (s.Hq + s.Hkv) * row, stride}};
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& qkv_, int64_t Hq, int64_t Hkv, int64_t window, int64_t sinks, double scale) {
+    c10::cuda::CUDAGuard guard(qkv_.device());
+    Tensor qkv = qkv_.contiguous();
+    if (reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16) qkv = qkv.clone();
+    const Shape s{qkv.size(0), qkv.size(1), Hq, Hkv, qkv.size(2) / (Hq + 2 * Hkv)};
+    const auto in = parts(qkv, s);
+    auto [o, lse] = window_forward(s, in[0], in[1], in[2], qkv.options(), window, sinks, scale);
+    ctx->save_for_backward({qkv, o, lse});
+    ctx->saved_data["Hq"] = Hq;
+    ctx->saved_data["Hkv"] = Hkv;
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    ctx->saved_data["scale"] = scale;
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor& qkv = saved[0];
+    c10::cuda::CUDAGuard guard(qkv.device());
+    const int64_t Hq = ctx->saved_data["Hq"].toInt(), Hkv = ctx->saved_data["Hkv"].toInt();
+    const Shape s{qkv.size(0), qkv.size(1), Hq, Hkv, qkv.size(2) / (Hq + 2 * Hkv)};
+    at::AutoDispatchBelowADInplaceOrView below;
+    Tensor dqkv = at::empty_like(qkv);
+    const auto in = parts(qkv, s), out = parts(dqkv, s);
+    window_backward(s, grads[0], in[0], in[1], in[2], saved[1], saved[2], out[0], out[1], out[2], ctx->saved_data["window"].toInt(),
+                    ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble());
+    grads = first_order_only({dqkv});
+    return {grads[0], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale) {
+  window_check(q, k, v, window, sinks);
+  TORCH_CHECK(q.is_cuda(), "titb200 window_attention: CUDA tensors");
+  return WindowAttention::apply(q, k, v, window, sinks, scale);
+}
+
+void qkv_check(const Tensor& qkv, int64_t Hq, int64_t Hkv) {
+  TORCH_CHECK(qkv.dim() == 3 && Hq > 0 && Hkv > 0 && qkv.size(2) > 0 && qkv.size(2) % (Hq + 2 * Hkv) == 0,
+              "titb200 window_attention: a projection of shape ", qkv.sizes(), " does not hold ", Hq, " + 2 * ", Hkv, " heads");
+}
+Tensor window_attention_qkv(const Tensor& qkv, int64_t Hq, int64_t Hkv, int64_t window, int64_t sinks, double scale) {
+  qkv_check(qkv, Hq, Hkv);
+  TORCH_CHECK(qkv.is_cuda(), "titb200 window_attention: CUDA tensors");
+  TORCH_CHECK(Hq % Hkv == 0, "titb200 window_attention: Hq must be a multiple of Hkv");
+  limits_check(qkv, qkv.size(0), qkv.size(1), Hq, qkv.size(2) / (Hq + 2 * Hkv), window, sinks);
+  return WindowAttentionQKV::apply(qkv, Hq, Hkv, window, sinks, scale);
 }
 }  // namespace
 
@@ -164,8 +265,7 @@ void bind_attention(pybind11::module_& m) {
   m.def("attn_bwd", &attn_bwd, py::arg("d_o"), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("o"), py::arg("lse"),
         py::arg("scale"), py::arg("dq") = py::none(), py::arg("dk") = py::none(), py::arg("dv") = py::none());
   m.def("window_check", &window_check);
-  m.def("window_attn_fwd", &window_attn_fwd);
-  m.def("window_attn_bwd", &window_attn_bwd, py::arg("d_o"), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("o"),
-        py::arg("lse"), py::arg("window"), py::arg("sinks"), py::arg("scale"), py::arg("dq") = py::none(),
-        py::arg("dk") = py::none(), py::arg("dv") = py::none());
+  m.def("window_qkv_check", &qkv_check);
+  m.def("window_attention", &window_attention);
+  m.def("window_attention_qkv", &window_attention_qkv);
 }

@@ -25,7 +25,6 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from .._lib import C
 
@@ -745,44 +744,6 @@ def window_attention_ref(q, k, v, window: Optional[int], sinks: int = 0, scale=N
     return (att @ vf).transpose(1, 2).to(q.dtype)
 
 
-class _WindowAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, window, sinks, scale):
-        o, lse = C.window_attn_fwd(q, k, v, window, sinks, scale)
-        ctx.save_for_backward(q, k, v, o, lse)
-        ctx.args = (window, sinks, scale)
-        return o
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, do):
-        q, k, v, o, lse = ctx.saved_tensors
-        dq, dk, dv = C.window_attn_bwd(do, q, k, v, o, lse, *ctx.args)
-        return dq, dk, dv, None, None, None
-
-
-class _WindowAttentionQKVFn(torch.autograd.Function):
-    """Over a fused projection buffer, as _AttentionQKVFn."""
-
-    @staticmethod
-    def forward(ctx, qkv, Hq, Hkv, hd, window, sinks, scale):
-        qkv = qkv.contiguous()
-        o, lse = C.window_attn_fwd(*_AttentionQKVFn._views(qkv, Hq, Hkv, hd), window, sinks, scale)
-        ctx.save_for_backward(qkv, o, lse)
-        ctx.args = (Hq, Hkv, hd, window, sinks, scale)
-        return o
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, do):
-        qkv, o, lse = ctx.saved_tensors
-        Hq, Hkv, hd, window, sinks, scale = ctx.args
-        dqkv = torch.empty_like(qkv)
-        C.window_attn_bwd(do, *_AttentionQKVFn._views(qkv, Hq, Hkv, hd), o, lse, window, sinks, scale,
-                          *_AttentionQKVFn._views(dqkv, Hq, Hkv, hd))
-        return dqkv, None, None, None, None, None, None
-
-
 def window_attention(q, k, v, window: Optional[int], sinks: int = 0, scale: Optional[float] = None):
     """Causal self-attention over a bounded context: query i sees key j when ``j <= i`` and (``i - j < window`` or
     ``j < sinks``), i.e. the last ``window`` positions, its own among them, and the first ``sinks`` of the sequence.
@@ -795,7 +756,7 @@ def window_attention(q, k, v, window: Optional[int], sinks: int = 0, scale: Opti
     if not q.is_cuda:
         C.window_check(q, k, v, _window_arg(window), sinks)
         return window_attention_ref(q, k, v, window, sinks, scale)
-    return _call(_WindowAttentionFn, q, k, v, _window_arg(window), sinks, scale)
+    return C.window_attention(q, k, v, _window_arg(window), sinks, scale)
 
 
 def window_attention_qkv(qkv, n_head: int, n_kv_head: Optional[int] = None, window: Optional[int] = None, sinks: int = 0,
@@ -803,13 +764,12 @@ def window_attention_qkv(qkv, n_head: int, n_kv_head: Optional[int] = None, wind
     """:func:`window_attention` on a fused QKV projection [B, T, (Hq + 2 Hkv) * hd] -> [B, T, Hq, hd]."""
     Hq = n_head
     Hkv = n_kv_head if n_kv_head is not None else n_head
+    if not qkv.is_cuda:
+        C.window_qkv_check(qkv, Hq, Hkv)
     hd = qkv.shape[-1] // (Hq + 2 * Hkv)
-    if qkv.dim() != 3 or hd * (Hq + 2 * Hkv) != qkv.shape[-1]:
-        raise RuntimeError(f"titb200 window_attention: a projection of shape {tuple(qkv.shape)} does not hold "
-                           f"{Hq} + 2 * {Hkv} heads")
-    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    scale = scale if scale is not None else 1.0 / math.sqrt(max(hd, 1))
     if qkv.is_cuda:
-        return _call(_WindowAttentionQKVFn, qkv, Hq, Hkv, hd, _window_arg(window), sinks, scale)
+        return C.window_attention_qkv(qkv, Hq, Hkv, _window_arg(window), sinks, scale)
     B, T, _ = qkv.shape
     q, k, v = (t.reshape(B, T, -1, hd) for t in qkv.split((Hq * hd, Hkv * hd, Hkv * hd), dim=-1))
     return window_attention(q, k, v, window, sinks, scale)
