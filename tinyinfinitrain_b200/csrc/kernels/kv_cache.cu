@@ -339,40 +339,54 @@ __device__ __forceinline__ void finish_item(const PagedArgs& p, int b, int item,
   __syncthreads();
 }
 
-// One CTA per CTA of the main kernel: the item that began in that one's run and went on behind it.
+// One CTA per CTA of the main kernel: the item that began in that one's run and went on behind it.  A warp takes a head's maxima
+// and denominators, a lane a part's, and leaves the parts' weights in shared memory; then a thread adds four elements of the
+// parts, eight loads in flight (a sequence alone on the card has some fifty parts to a head: with two dependent passes over them
+// the join took 14 of 99 us).
 template <typename T, int HG>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs p) {
+  extern __shared__ float weight[];   // [HG][parts]
+  __shared__ float inv[HG];
   dependency_wait();
   const CacheArgs& c = p.c;
   const int4 join = p.joins[blockIdx.x];   // sequence, item, last CTA, in use
   if (!join.w) return;
   const int G = c.Hq / c.Hkv, hgroups = (G + HG - 1) / HG, hk = join.y / hgroups, g0 = join.y % hgroups * HG, ng = min(HG, G - g0);
   const long long size = slot_floats<HG>(c);
-  const float* first = p.parts + (blockIdx.x * 2LL + 1) * size;
-  const float* rest = p.parts + (blockIdx.x + 1) * 2LL * size;
-  const int n_rest = join.z - blockIdx.x;
+  const int parts = join.z - blockIdx.x + 1, lane = threadIdx.x & 31;
+  const auto part = [&](int r) { return p.parts + ((blockIdx.x + r) * 2LL + (r == 0 ? 1 : 0)) * size; };
+  for (int g = threadIdx.x >> 5; g < ng; g += 4) {
+    float top = -INFINITY, sum = 0.f;
+    for (int r = lane; r < parts; r += 32) {
+      const float m = part(r)[HG * c.hd + g];
+      weight[g * parts + r] = m;
+      top = fmaxf(top, m);
+    }
+    top = warp_max(top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    for (int r = lane; r < parts; r += 32) {
+      const float f = exp2f(weight[g * parts + r] - ref);
+      weight[g * parts + r] = f;
+      sum = fmaf(part(r)[HG * (c.hd + 1) + g], f, sum);
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) inv[g] = sum == 0.f ? 0.f : 1.f / sum;
+  }
+  __syncthreads();
   for (int i = threadIdx.x; i < ng * (c.hd / 4); i += blockDim.x) {
     const int g = i / (c.hd / 4), d = i % (c.hd / 4) * 4;
-    const int at_m = HG * c.hd + g, at_l = HG * (c.hd + 1) + g, at_o = g * c.hd + d;
-    float top = first[at_m];
-    for (int r = 0; r < n_rest; ++r) top = fmaxf(top, rest[r * 2 * size + at_m]);
-    const float ref = top == -INFINITY ? 0.f : top;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-    auto add = [&](const float* s) {
-      const float f = exp2f(s[at_m] - ref);
-      const float4 x = *reinterpret_cast<const float4*>(s + at_o);
-      sum = fmaf(s[at_l], f, sum);
+#pragma unroll 8
+    for (int r = 0; r < parts; ++r) {
+      const float f = weight[g * parts + r];
+      const float4 x = *reinterpret_cast<const float4*>(part(r) + g * c.hd + d);
       acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y);
       acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
-    };
-    add(first);
-    for (int r = 0; r < n_rest; ++r) add(rest + r * 2 * size);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    }
     T* dst = static_cast<T*>(p.o) + (static_cast<long long>(join.x) * c.Hq + hk * G + g0 + g) * c.hd + d;
     Pack<T, 4> o;
-    o.v[0] = from_f32<T>(acc.x * inv); o.v[1] = from_f32<T>(acc.y * inv);
-    o.v[2] = from_f32<T>(acc.z * inv); o.v[3] = from_f32<T>(acc.w * inv);
+    o.v[0] = from_f32<T>(acc.x * inv[g]); o.v[1] = from_f32<T>(acc.y * inv[g]);
+    o.v[2] = from_f32<T>(acc.z * inv[g]); o.v[3] = from_f32<T>(acc.w * inv[g]);
     *reinterpret_cast<Pack<T, 4>*>(dst) = o;
   }
 }
@@ -536,7 +550,8 @@ template <int HD>
 struct PagedMma {
   static constexpr int kKeys = 2048 / HD;              // rows of a warp's step: 4 KB of keys and 4 KB of values
   static constexpr int kTile = 4 * kKeys;              // of a CTA's
-  static constexpr int kStages = 3;
+  static constexpr int kCtas = HD == 64 ? 3 : 2;        // that share an SM
+  static constexpr int kStages = HD == 64 ? 2 : 3;
   static constexpr int kStepBytes = 2 * kKeys * HD * 2;
   static constexpr int kMeta = 4 * kStages * kStepBytes;
   static constexpr int kStat = kMeta + 4 * kStages * 16;
@@ -547,8 +562,13 @@ struct PagedMma {
 // inside an item), multiplies them with the item's queries, keeps its own maximum, sum and output, and meets the others at
 // the item's end.  The rows are swizzled (16-byte unit u of row r at u ^ (r & 7)), so that both the plain and the transposing
 // matrix loads are free of bank conflicts.  UPPER: more than eight query heads in an item.
+// Bound by memory: the cache is read once, and mma.sync, which pads the heads to 16 rows, needs a fifth of its rate for it.  Next
+// to that counts the latency of a step's instructions, with eight to twelve warps on an SM: hd 64 is better off with three CTAs
+// and two stages (192 sequences, window 1024 of up to 32768, 32 / 8 heads: 69 us, 5.6 TB/s; two CTAs and three stages 79 us),
+// hd 128 the other way round (131071 positions, 32 / 8 heads: 94 us, 5.7 TB/s; 102 us).  64 sequences of up to 8192 positions, 32 / 8
+// heads of 128: 97 us, 6.0 TB/s.  The first kernel, one CTA an item on the CUDA cores: 293 us, 21 ms, 1.35 ms.
 template <int HD, bool UPPER>
-__global__ void __launch_bounds__(kPagedThreads) paged_mma_kernel(const PagedArgs p) {
+__global__ void __launch_bounds__(kPagedThreads, PagedMma<HD>::kCtas) paged_mma_kernel(const PagedArgs p) {
   using Cfg = PagedMma<HD>;
   constexpr int KEYS = Cfg::kKeys, STAGES = Cfg::kStages, HG = kMmaHeads;
   constexpr int kUnits = HD / 8, kRowsPerCopy = 32 / kUnits, kCopies = KEYS / kRowsPerCopy;
@@ -799,8 +819,8 @@ static PagedPlan paged_plan(const TitbCacheDesc* d) {
   const long long tiles = ((held < seen ? held : seen) + tile - 1) / tile;
   const int G = d->Hq / d->Hkv;
   const long long items = static_cast<long long>(d->B) * d->Hkv * ((G + plan.heads - 1) / plan.heads);
-  // two CTAs of the matrix kernel fit on an SM (99 KB of shared memory each), four of the other (registers)
-  const long long most = device_sm_count() * (plan.mma ? 2LL : 4LL);
+  // what fits on an SM: shared memory decides for the matrix kernel, registers for the other
+  const long long most = device_sm_count() * static_cast<long long>(!plan.mma ? 4 : d->hd == 64 ? PagedMma<64>::kCtas : PagedMma<128>::kCtas);
   plan.ctas = static_cast<int>(tiles == 0 ? 1 : items > most / tiles ? most : items * tiles);
   plan.join = tiles > 1;   // otherwise every item is one tile
   return plan;
@@ -881,5 +901,5 @@ TITB_API int titb_paged_attention(const TitbCacheDesc* d, const void* q, long lo
   }
   if (rc != 0 || !plan.join) return rc;
   auto join = d->dtype == 0 ? paged_join_kernel<float, kPagedHeads> : plan.mma ? paged_join_kernel<bf16, kMmaHeads> : paged_join_kernel<bf16, kPagedHeads>;
-  return static_cast<int>(launch_dependent(join, dim3(plan.ctas), dim3(128), 0, st, a));
+  return static_cast<int>(launch_dependent(join, dim3(plan.ctas), dim3(128), plan.heads * plan.ctas * 4, st, a));
 }
