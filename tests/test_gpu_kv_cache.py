@@ -277,6 +277,36 @@ def test_pages_outside_the_cache_are_reported_and_not_followed():
             check_device_status()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_caches_without_pages_and_tables_without_entries(dtype):
+    """Nothing can be held: positions are reported, sequences of length 0 are served."""
+    q = torch.ones(2, 2, 64, device=DEV, dtype=dtype)
+    zero, some = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([0, 0], [0, 3]))
+    for n_pages, width in ((0, 2), (4, 0), (0, 0)):
+        kc, vc = (torch.zeros(n_pages, 1, 4, 64, device=DEV, dtype=dtype) for _ in range(2))
+        table = torch.zeros(2, width, dtype=torch.int32, device=DEV)
+        assert not ops.paged_attention(q, kc, vc, table, zero).any()
+        check_device_status()
+        assert not ops.paged_attention(q, kc, vc, table, some).any()
+        with pytest.raises(RuntimeError, match="status 4"):
+            check_device_status()
+        ops.cache_append(torch.ones(2, 1, 4 * 64, device=DEV, dtype=dtype), kc, vc, table, zero, 2, 1)
+        with pytest.raises(RuntimeError, match="status 4"):
+            check_device_status()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_empty_batches(dtype):
+    kc, vc = (torch.zeros(4, 1, 4, 64, device=DEV, dtype=dtype) for _ in range(2))
+    table, none = torch.zeros(0, 3, dtype=torch.int32, device=DEV), torch.zeros(0, dtype=torch.int32, device=DEV)
+    assert ops.paged_attention(torch.zeros(0, 2, 64, device=DEV, dtype=dtype), kc, vc, table, none).shape == (0, 2, 64)
+    for B, T in ((0, 3), (1, 0)):
+        q, k = ops.cache_append(torch.zeros(B, T, 4 * 64, device=DEV, dtype=dtype), kc, vc, table.new_zeros(B, 3), none.new_zeros(B), 2,
+                                1, theta=1e4, return_k=True)
+        assert q.shape == (B, T, 2, 64) and k.shape == (B, T, 1, 64)
+    check_device_status()
+
+
 def test_infinite_and_undefined_rows_that_nobody_sees():
     for fill in (float("nan"), float("inf"), torch.finfo(BF).min):
         kc, vc, table, rows = _cache([130, 5], 2, 64, 16, BF, fill=fill, seed=2)

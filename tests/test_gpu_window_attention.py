@@ -158,6 +158,11 @@ def test_refusals():
     for args in bad:
         with pytest.raises(RuntimeError, match="titb200 window_attention"):
             ops.window_attention(*args)
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(RuntimeError, match="scale"):
+            ops.window_attention(q, k, v, 4, scale=scale)
+        with pytest.raises(RuntimeError, match="scale"):
+            ops.window_attention_qkv(_fused(q, k, v), 4, 2, 4, scale=scale)
     with pytest.raises(RuntimeError, match="head_dim"):
         ops.window_attention(*(torch.zeros(1, 4, 2, 136, device=DEV, dtype=BF),) * 3, 4)
     with pytest.raises(RuntimeError, match="does not hold"):

@@ -119,6 +119,9 @@ def test_refusals():
                  (q[0], kc, vc, table, n), (q, kc, vc, table, n, 0), (q, kc, vc, table, n, 4, -1)):
         with pytest.raises(RuntimeError, match="titb200 paged_attention"):
             ops.paged_attention(*args)
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(RuntimeError, match="scale"):
+            ops.paged_attention(q, kc, vc, table, n, scale=scale)
     for args, kw in (((qkv, kc, vc, table, n, 4, 1), {}), ((qkv, kc, vc, table, n, 3, 2), {}), ((qkv[0], kc, vc, table, n, 4, 2), {}),
                      ((qkv, kc, vc, table, n.float(), 4, 2), {}), ((qkv, kc, vc, table, n, 4, 2), {"theta": -1.0}),
                      ((qkv, kc, vc, table, n, 4, 2), {"theta": 0.0}), ((qkv, kc, vc, table, n, 4, 2), {"theta": float("inf")}),

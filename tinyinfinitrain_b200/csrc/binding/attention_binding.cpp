@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <array>
 #include <climits>
+#include <cmath>
 
 #include "kernels/api.h"
 
@@ -72,7 +73,8 @@ std::vector<Tensor> attn_bwd(const Tensor& d_o_, const Tensor& q_, const Tensor&
 }
 
 // ---- window and sinks
-void limits_check(const Tensor& t, int64_t B, int64_t T, int64_t Hq, int64_t hd, int64_t window, int64_t sinks) {
+void limits_check(const Tensor& t, int64_t B, int64_t T, int64_t Hq, int64_t hd, int64_t window, int64_t sinks, double scale) {
+  TORCH_CHECK(scale > 0.0 && std::isfinite(scale), "titb200 window_attention: scale must be positive, got ", scale);
   TORCH_CHECK(window >= 1, "titb200 window_attention: window must be at least 1, got ", window);
   TORCH_CHECK(sinks >= 0, "titb200 window_attention: sinks must not be negative, got ", sinks);
   if (!t.is_cuda()) return;
@@ -81,7 +83,7 @@ void limits_check(const Tensor& t, int64_t B, int64_t T, int64_t Hq, int64_t hd,
   TORCH_CHECK(hd > 0 && hd <= 128 && hd % 8 == 0, "titb200 window_attention: head_dim must be a multiple of 8 up to 128, got ", hd);
   TORCH_CHECK(T <= 32 * 32767LL && B * Hq < (1LL << 31), "titb200 window_attention: too many tokens or heads");
 }
-void window_check(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks) {
+void window_check(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale) {
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "titb200 window_attention: q [B, T, Hq, hd], k and v [B, T, Hkv, hd]");
   TORCH_CHECK(k.sizes() == v.sizes(), "titb200 window_attention: k and v must have the same shape");
   TORCH_CHECK(q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3),
@@ -89,7 +91,7 @@ void window_check(const Tensor& q, const Tensor& k, const Tensor& v, int64_t win
   TORCH_CHECK(k.size(2) > 0 && q.size(2) % k.size(2) == 0, "titb200 window_attention: Hq must be a multiple of Hkv");
   TORCH_CHECK(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type() && q.device() == k.device() &&
                   q.device() == v.device(), "titb200 window_attention: q, k and v must share dtype and device");
-  limits_check(q, q.size(0), q.size(1), q.size(2), q.size(3), window, sinks);
+  limits_check(q, q.size(0), q.size(1), q.size(2), q.size(3), window, sinks, scale);
 }
 
 // Elements between the tokens of a [B, T, H, hd] view, taken from a dimension that has more than one entry.
@@ -242,7 +244,7 @@ struct WindowAttentionQKV : public torch::autograd::Function<WindowAttentionQKV>
 };
 
 Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale) {
-  window_check(q, k, v, window, sinks);
+  window_check(q, k, v, window, sinks, scale);
   TORCH_CHECK(q.is_cuda(), "titb200 window_attention: CUDA tensors");
   return WindowAttention::apply(q, k, v, window, sinks, scale);
 }
@@ -255,7 +257,7 @@ Tensor window_attention_qkv(const Tensor& qkv, int64_t Hq, int64_t Hkv, int64_t 
   qkv_check(qkv, Hq, Hkv);
   TORCH_CHECK(qkv.is_cuda(), "titb200 window_attention: CUDA tensors");
   TORCH_CHECK(Hq % Hkv == 0, "titb200 window_attention: Hq must be a multiple of Hkv");
-  limits_check(qkv, qkv.size(0), qkv.size(1), Hq, qkv.size(2) / (Hq + 2 * Hkv), window, sinks);
+  limits_check(qkv, qkv.size(0), qkv.size(1), Hq, qkv.size(2) / (Hq + 2 * Hkv), window, sinks, scale);
   return WindowAttentionQKV::apply(qkv, Hq, Hkv, window, sinks, scale);
 }
 }  // namespace

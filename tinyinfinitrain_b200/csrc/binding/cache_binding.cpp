@@ -115,7 +115,8 @@ py::object cache_append(const Tensor& qkv_, Tensor& k_cache, Tensor& v_cache, co
 }
 
 void paged_check(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& lengths,
-                 int64_t window, int64_t sinks) {
+                 int64_t window, int64_t sinks, double scale) {
+  TORCH_CHECK(scale > 0.0 && std::isfinite(scale), "titb200 paged_attention: scale must be positive, got ", scale);
   forward_only("paged_attention", {&q, &k_cache, &v_cache});
   TORCH_CHECK(q.dim() == 3 && k_cache.dim() == 4, "titb200 paged_attention: q [B, Hq, hd], caches [pages, Hkv, page_size, hd]");
   cache_check("paged_attention", q, k_cache, v_cache, table, lengths, q.size(0), q.size(1), k_cache.size(1), q.size(2), window,
@@ -125,7 +126,7 @@ void paged_check(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, 
 Tensor paged_attention(const Tensor& q_, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& lengths,
                        int64_t window, int64_t sinks, double scale) {
   TORCH_CHECK(q_.is_cuda(), "titb200 paged_attention: CUDA tensors");
-  paged_check(q_, k_cache, v_cache, table, lengths, window, sinks);
+  paged_check(q_, k_cache, v_cache, table, lengths, window, sinks, scale);
   c10::cuda::CUDAGuard guard(q_.device());
   const int64_t align = 16 / q_.element_size();
   const bool usable = q_.stride(2) == 1 && q_.stride(1) == q_.size(2) && q_.stride(0) % align == 0 &&

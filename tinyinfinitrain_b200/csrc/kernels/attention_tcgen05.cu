@@ -107,10 +107,10 @@ struct FwdCfg {
   static constexpr int kP = kV + kStages * kTileBytes;
   static constexpr int kBar = kP + (WIN ? 0 : kBlk * kBlk * 2);   // WIN: P lies in tensor memory
   static constexpr int kSmem = kBar + 128;
-  // S: [0, kKeys)  O: [kColO, kColO + HD); WIN: P takes 32 columns, at 64 beside O of 128, else in a second allocation
+  // S: [0, kKeys)  O: [kColO, kColO + HD); WIN: P takes 32 columns, over S (kAlias) or at 64
+  static constexpr bool kAlias = WIN && HD == 64;
   static constexpr int kColO = HD == 128 ? 128 : kKeys;
-  static constexpr int kTmemCols = WIN && HD == 64 ? 128 : 256;
-  static constexpr int kTmemColsP = WIN && HD == 64 ? 32 : 0;
+  static constexpr int kTmemCols = kAlias ? 128 : 256;
 };
 
 // Forward pipeline.  Per key block j the CTA runs
@@ -133,9 +133,14 @@ struct FwdCfg {
 // block on either border of what the rows see is masked by a 128-bit mask per row, built from the row's two ranges of keys.
 // Up to kSinkCols sinks that lie before the window are a block of kSinkCols keys.  The few blocks of such a CTA do not hide its
 // set-up and its chain of dependent steps (S, maximum, exponentials, P, P V), so kCtas CTAs share the SM, with 64 keys a step
-// and P in tensor memory, as the A operand of P V: 48 or 96 KB of shared memory and 160 or 256 columns to a CTA.
+// and P in tensor memory, as the A operand of P V: 48 or 96 KB of shared memory and 128 or 256 columns to a CTA.  At hd 64 P
+// lies over S and S(j+1) is issued behind P(j) V(j), which costs nothing beside two other CTAs (columns of its own, in a
+// second allocation, were as fast).
 // Measured (B200): hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: one CTA an SM 254 us, two with 128 keys a step, P over S
-// and S(j+1) issued behind P(j) V(j) 182 us, now TODO; hd 64, 1 x 1999, 32 / 8 heads, window 512: 29, 26, TODO us.
+// and S(j+1) issued behind P(j) V(j) 182 us, as it is 165 us (790 TFLOP/s of what the rows see); hd 64, 1 x 1999, 32 / 8 heads,
+// window 512: 29 us before, 26 us.  A step of 64 keys takes 1660 cycles (hd 128) and 2140 (hd 64, three CTAs), 920 and 1060 of
+// them for the exponentials; a quarter of those on the multiply-add pipe changed nothing.  Set-up, first loads and output
+// take another 8000 and 5500 cycles of a CTA.
 template <int HD, bool WIN>
 __global__ void __launch_bounds__(kAttnThreads, FwdCfg<HD, WIN>::kCtas)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -156,7 +161,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   uint64_t* s_free = bars + 12;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
   volatile uint32_t* abort_flag = tmem_slot + 1;
-  uint32_t* tmem_slot_p = tmem_slot + 2;
 
   const int warp = ptx::warp_index(), lane = threadIdx.x & 31;
   const int nqb = (p.T + kBlk - 1) / kBlk;
@@ -193,7 +197,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   }
   if (warp == 1) {
     ptx::tmem_alloc(tmem_slot, Cfg::kTmemCols);
-    if (Cfg::kTmemColsP) ptx::tmem_alloc(tmem_slot_p, Cfg::kTmemColsP);
     ptx::tmem_relinquish();
   }
   ptx::tc_fence_before_sync();
@@ -203,7 +206,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   dependency_wait();
   dependents_launch();
   const uint32_t tS = tmem_base, tO = tmem_base + Cfg::kColO;
-  const uint32_t tP = Cfg::kTmemColsP ? *tmem_slot_p : tmem_base + 64;   // WIN
+  const uint32_t tP = Cfg::kAlias ? tS : tmem_base + 64;   // WIN
   const bool bad_align = (*abort_flag != 0);
 
   if (bad_align) {
@@ -258,7 +261,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         issue_s(0);
       }
       for (int j = 0; j < nblk && ok; ++j) {
-        if (j + 1 < nblk) {
+        if (!Cfg::kAlias && j + 1 < nblk) {
           // S(j+1) goes into the score columns as soon as S(j) has been copied to registers
           if (!ptx::mbar_wait(&k_full[(j + 1) % S], ((j + 1) / S) & 1, abort_flag)) break;
           if (!ptx::mbar_wait(s_free, j & 1, abort_flag)) break;
@@ -281,6 +284,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         }
         ptx::tc_commit(o_full);
         ptx::tc_commit(&v_empty[j % S]);
+        if (Cfg::kAlias && j + 1 < nblk) {
+          // products run in the order of their issue: P(j) V(j) has read P before S(j+1) takes its columns
+          if (!ptx::mbar_wait(&k_full[(j + 1) % S], ((j + 1) / S) & 1, abort_flag)) break;
+          ptx::tc_fence_after_sync();
+          issue_s(j + 1);
+        }
       }
     }
   } else {
@@ -297,7 +306,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       if (!ptx::mbar_wait_warp(s_full, j & 1, abort_flag)) { ok = false; break; }
       ptx::tc_fence_after_sync();
       // Moves the reference maximum, and O with it, when a block's maximum exceeds it by too much.
-      bool waited_o = (j == 0);
+      bool waited_o = Cfg::kAlias || j == 0;   // kAlias: S(j) was issued behind the product before
       auto settle = [&](float m_blk) {
         if (j == 0) {
           m_ref = m_blk;
@@ -490,7 +499,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   if (warp == 1) {
     __syncwarp();
     ptx::tmem_dealloc(tmem_base, Cfg::kTmemCols);
-    if (Cfg::kTmemColsP) ptx::tmem_dealloc(*tmem_slot_p, Cfg::kTmemColsP);
   }
   if (threadIdx.x == 0 && *abort_flag) atomicExch(p.status, kStatusMbarTimeout);
 }

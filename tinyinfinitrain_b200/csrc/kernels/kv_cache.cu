@@ -36,7 +36,8 @@ struct CacheArgs {
 static CacheArgs cache_args(const TitbCacheDesc* d) {
   CacheArgs a{};
   a.k_cache = d->k_cache; a.v_cache = d->v_cache;
-  a.page_table = d->page_table; a.table_stride = d->table_stride; a.table_width = d->table_width;
+  a.page_table = d->page_table; a.table_stride = d->table_stride;
+  a.table_width = d->n_pages > 0 ? d->table_width : 0;   // without pages no entry leads anywhere
   a.n_pages = d->n_pages; a.page_size = d->page_size;
   a.B = d->B; a.Hq = d->Hq; a.Hkv = d->Hkv; a.hd = d->hd;
   a.window = d->window; a.sinks = d->sinks;

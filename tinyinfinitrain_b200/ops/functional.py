@@ -754,7 +754,7 @@ def window_attention(q, k, v, window: Optional[int], sinks: int = 0, scale: Opti
     hd = q.shape[-1]
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
     if not q.is_cuda:
-        C.window_check(q, k, v, _window_arg(window), sinks)
+        C.window_check(q, k, v, _window_arg(window), sinks, scale)
         return window_attention_ref(q, k, v, window, sinks, scale)
     return C.window_attention(q, k, v, _window_arg(window), sinks, scale)
 
@@ -878,9 +878,9 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, window: Optional[i
     A page number or length outside the cache raises IndexError on the CPU; on the GPU it is not followed, and
     ``parallel.health.check_device_status()`` raises."""
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])
-    args = (q, k_cache, v_cache, page_table, lengths, _window_arg(window), sinks)
+    args = (q, k_cache, v_cache, page_table, lengths, _window_arg(window), sinks, scale)
     if q.is_cuda:
-        return C.paged_attention(*args, scale)
+        return C.paged_attention(*args)
     C.paged_attention_check(*args)
     return paged_attention_ref(q, k_cache, v_cache, page_table, lengths, window, sinks, scale)
 
