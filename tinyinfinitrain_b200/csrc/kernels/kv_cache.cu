@@ -449,23 +449,30 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
       fresh = false;
     }
     const PageMap map = c.map(walk.b);
-    for (int r = 0; r < kPagedTile / kGroups; r += kBatch) {
-      long long row[kBatch];
-      Pack<T, VN> kx[kBatch], vx[kBatch];
+    // the rows of a batch are looked up under the loads of the batch before
+    int next[kBatch];
+    auto look_up = [&](int r) {
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         const int v = walk.t * kPagedTile + (r + u) * kGroups + grp;
-        row[u] = v < walk.seen.n ? map.row(walk.seen.pos(v), c.Hkv, hk) : -1;
-        if (v < walk.seen.n && row[u] < 0) atomicExch(c.status, kStatusBadPage);
+        next[u] = v < walk.seen.n ? static_cast<int>(map.row(walk.seen.pos(v), c.Hkv, hk)) : -1;
+        if (v < walk.seen.n && next[u] < 0) atomicExch(c.status, kStatusBadPage);
       }
+    };
+    look_up(0);
+    for (int r = 0; r < kPagedTile / kGroups; r += kBatch) {
+      int row[kBatch];
+      Pack<T, VN> kx[kBatch], vx[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
+        row[u] = next[u];
         kx[u] = vx[u] = Pack<T, VN>{};
         if (row[u] >= 0 && in_head) {
-          kx[u] = ld128(static_cast<const T*>(c.k_cache) + row[u] * c.hd + d0);
-          vx[u] = ld128(static_cast<const T*>(c.v_cache) + row[u] * c.hd + d0);
+          kx[u] = ld128(static_cast<const T*>(c.k_cache) + static_cast<long long>(row[u]) * c.hd + d0);
+          vx[u] = ld128(static_cast<const T*>(c.v_cache) + static_cast<long long>(row[u]) * c.hd + d0);
         }
       }
+      if (r + kBatch < kPagedTile / kGroups) look_up(r + kBatch);
 #pragma unroll
       for (int g = 0; g < HG; ++g) {
         if (g0 + g >= G) break;
@@ -636,10 +643,28 @@ __global__ void __launch_bounds__(kPagedThreads, PagedMma<HD>::kCtas) paged_mma_
   const float sc = p.scale * 1.4426950408889634f;
   const int gr = lane >> 2, tq = lane & 3;
 
+  // An item's queries, and nothing accumulated: before the wait for its first rows.
+  auto begin_item = [&](int b, int item) {
+    const int hk = item / hgroups, g0 = item % hgroups * HG;
+    const bf16* src = static_cast<const bf16*>(p.q) + b * p.q_stride_b + static_cast<long long>(hk * G + g0) * HD + tq * 2;
+    const bool lo = g0 + gr < G, hi = UPPER && g0 + gr + 8 < G;
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k) {
+      q[k][0] = lo ? *reinterpret_cast<const uint32_t*>(src + gr * HD + k * 16) : 0u;
+      q[k][2] = lo ? *reinterpret_cast<const uint32_t*>(src + gr * HD + k * 16 + 8) : 0u;
+      q[k][1] = hi ? *reinterpret_cast<const uint32_t*>(src + (gr + 8) * HD + k * 16) : 0u;
+      q[k][3] = hi ? *reinterpret_cast<const uint32_t*>(src + (gr + 8) * HD + k * 16 + 8) : 0u;
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+    m0 = m1 = -INFINITY;
+    l0 = l1 = 0.f;
+  };
+
   look_up();
+  begin_item(ahead.b, ahead.item);
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) copy_step();
-  bool fresh = true;
   for (int it = 0; it < run.n; ++it) {
     copy_wait<STAGES - 2>();
     __syncwarp();
@@ -647,23 +672,6 @@ __global__ void __launch_bounds__(kPagedThreads, PagedMma<HD>::kCtas) paged_mma_
     const int st = it % STAGES;
     const int4 info = meta[st];
     const uint32_t real = static_cast<uint32_t>(info.x);
-    if (fresh) {
-      fresh = false;
-      const int hk = info.z / hgroups, g0 = info.z % hgroups * HG;
-      const bf16* src = static_cast<const bf16*>(p.q) + info.y * p.q_stride_b + static_cast<long long>(hk * G + g0) * HD + tq * 2;
-      const bool lo = g0 + gr < G, hi = UPPER && g0 + gr + 8 < G;
-#pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        q[k][0] = lo ? *reinterpret_cast<const uint32_t*>(src + gr * HD + k * 16) : 0u;
-        q[k][2] = lo ? *reinterpret_cast<const uint32_t*>(src + gr * HD + k * 16 + 8) : 0u;
-        q[k][1] = hi ? *reinterpret_cast<const uint32_t*>(src + (gr + 8) * HD + k * 16) : 0u;
-        q[k][3] = hi ? *reinterpret_cast<const uint32_t*>(src + (gr + 8) * HD + k * 16 + 8) : 0u;
-      }
-#pragma unroll
-      for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
-      m0 = m1 = -INFINITY;
-      l0 = l1 = 0.f;
-    }
     if (real != 0) {
       const uint32_t kb = smem_addr(ring + st * Cfg::kStepBytes), vb = kb + KEYS * HD * 2;
       float s[KEYS / 8][4];
@@ -773,7 +781,10 @@ __global__ void __launch_bounds__(kPagedThreads, PagedMma<HD>::kCtas) paged_mma_
       finish_item<bf16, HG, 4>(p, info.y, info.z, item_ends && !began_before, began_before,
                                reinterpret_cast<const float*>(smem + st * Cfg::kStepBytes), STAGES * Cfg::kStepBytes / 4, HD, sm_m, sm_l);
       began_before = false;
-      fresh = true;
+      if (it + 1 < run.n) {   // whose rows are on their way
+        const int4 next = meta[(it + 1) % STAGES];
+        begin_item(next.y, next.z);
+      }
     }
   }
 }
