@@ -8,9 +8,9 @@ n e times the sum of their absolute values.
 * O = P V, P rounded to the tensors' type before the product, O rounded:
   |dO| <= u |O| + (u + E_i + n e) (P |V|)
 * dV = P^T dO, the same: u |dV| + P'^T |dO| with P' = (u + E_i + n e) P
-* dS = scale P (dP - D), rounded; dP = dO V^T is off by hd e (|dO| |V|^T), D = rowsum(dO O) by (u + hd e) rowsum|dO O| because O
-  is the rounded one (and O's own error):
-  |d dS| <= (u + E_i + 4 e) |dS| + scale P (hd e |dO||V|^T + |dO|.(|d O|) + hd e |dO|.|O|)
+* dS = scale P (dP - D), rounded; dP = dO V^T is off by hd e (|dO| |V|^T), D = rowsum(dO O) by hd e rowsum|dO O| and O's own error,
+  of which the rounding counts with u^2: what it leaves is kept, rounded itself:
+  |d dS| <= (u + E_i + 4 e) |dS| + scale P (hd e |dO||V|^T + |dO|.(|d O| - u |O| + u^2 |O|) + hd e |dO|.|O|)
 * dQ = dS K and dK = dS^T Q: u |dQ| + (|d dS| + n e |dS|) |K|, and so for dK.
 """
 import math
@@ -61,7 +61,7 @@ def attention64(q, k, v, do, mask, scale=None):
     delta = (g * o).sum(-1, keepdim=True)
     ds = scale * p * (dp - delta)
     ds_err = (u + row + 4 * E) * ds.abs() + scale * p * (
-        hd * E * (g.abs() @ vr.abs().transpose(2, 3)) + (g.abs() * o_err).sum(-1, keepdim=True)
+        hd * E * (g.abs() @ vr.abs().transpose(2, 3)) + (g.abs() * (o_err - (u - u * u) * o.abs())).sum(-1, keepdim=True)
         + hd * E * (g.abs() * o.abs()).sum(-1, keepdim=True))
     ds_all = ds_err + (n + G * T) * E * ds.abs()
     dq, dk = ds @ kr, share(ds.transpose(2, 3) @ q)

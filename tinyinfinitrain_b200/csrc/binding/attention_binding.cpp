@@ -133,25 +133,31 @@ TitbWindowDesc window_desc(const Shape& s, Rows q, Rows k, Rows v, at::ScalarTyp
   return w;
 }
 
-// {o [B, T, Hq, hd], lse fp32 [B, Hq, T]}
-std::pair<Tensor, Tensor> window_forward(const Shape& s, Rows q, Rows k, Rows v, const at::TensorOptions& opt, int64_t window,
-                                         int64_t sinks, double scale) {
+// {o [B, T, Hq, hd], lse fp32 [B, Hq, T], what the rounding of o left (bf16, when a backward pass may follow)}
+std::array<Tensor, 3> window_forward(const Shape& s, Rows q, Rows k, Rows v, const at::TensorOptions& opt, int64_t window,
+                                     int64_t sinks, double scale, bool training) {
   Tensor o = at::empty({s.B, s.T, s.Hq, s.hd}, opt);
   Tensor lse = at::empty({s.B, s.Hq, s.T}, opt.dtype(at::kFloat));
   TitbWindowDesc w = window_desc(s, q, k, v, o.scalar_type(), window, sinks, scale);
   w.attn.o = o.data_ptr(); w.attn.lse = lse.data_ptr<float>();
+  Tensor o_lo;
+  if (training && w.dtype == 1) {
+    o_lo = at::empty_like(o);
+    w.o_lo = o_lo.data_ptr();
+  }
   check(titb_window_attn_fwd(&w, at::cuda::getCurrentCUDAStream().stream()), "window_attention");
-  return {o, lse};
+  return {o, lse, o_lo};
 }
 
-void window_backward(const Shape& s, const Tensor& d_o_, Rows q, Rows k, Rows v, const Tensor& o, const Tensor& lse, Rows dq, Rows dk,
-                     Rows dv, int64_t window, int64_t sinks, double scale) {
+void window_backward(const Shape& s, const Tensor& d_o_, Rows q, Rows k, Rows v, const Tensor& o, const Tensor& lse, const Tensor& o_lo,
+                     Rows dq, Rows dk, Rows dv, int64_t window, int64_t sinks, double scale) {
   TORCH_CHECK(d_o_.sizes() == o.sizes() && d_o_.scalar_type() == o.scalar_type() && d_o_.device() == o.device(),
               "titb200 window_attention: the gradient must look like the output");
   const Tensor d_o = in_place_or_copy(d_o_);
   TitbWindowDesc w = window_desc(s, q, k, v, o.scalar_type(), window, sinks, scale);
   TitbAttnDesc& d = w.attn;
   d.o = o.data_ptr(); d.lse = lse.data_ptr<float>();
+  w.o_lo = o_lo.defined() ? o_lo.data_ptr() : nullptr;
   d.d_o = d_o.data_ptr(); d.do_stride_t = token_stride(d_o);
   d.dq = dq.ptr; d.dk = dk.ptr; d.dv = dv.ptr;
   d.dq_stride_t = dq.stride; d.dk_stride_t = dk.stride; d.dv_stride_t = dv.stride;
@@ -179,12 +185,12 @@ variable_list first_order_only(variable_list grads) {
 // the kernels run on a few hundred tokens; 75 us now, most of it the autograd engine.
 struct WindowAttention : public torch::autograd::Function<WindowAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window, int64_t sinks,
-                        double scale) {
+                        double scale, bool training) {
     c10::cuda::CUDAGuard guard(q_.device());
     const Tensor q = in_place_or_copy(q_), k = in_place_or_copy(k_), v = in_place_or_copy(v_);
     const Shape s{q.size(0), q.size(1), q.size(2), k.size(2), q.size(3)};
-    auto [o, lse] = window_forward(s, rows_of(q), rows_of(k), rows_of(v), q.options(), window, sinks, scale);
-    ctx->save_for_backward({q, k, v, o, lse});
+    auto [o, lse, o_lo] = window_forward(s, rows_of(q), rows_of(k), rows_of(v), q.options(), window, sinks, scale, training);
+    ctx->save_for_backward({q, k, v, o, lse, o_lo});
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
     ctx->saved_data["scale"] = scale;
@@ -198,10 +204,10 @@ struct WindowAttention : public torch::autograd::Function<WindowAttention> {
     at::AutoDispatchBelowADInplaceOrView below;
     Tensor dq = at::empty({s.B, s.T, s.Hq, s.hd}, q.options()), dk = at::empty({s.B, s.T, s.Hkv, s.hd}, q.options()),
            dv = at::empty({s.B, s.T, s.Hkv, s.hd}, q.options());
-    window_backward(s, grads[0], rows_of(q), rows_of(k), rows_of(v), saved[3], saved[4], rows_of(dq), rows_of(dk), rows_of(dv),
+    window_backward(s, grads[0], rows_of(q), rows_of(k), rows_of(v), saved[3], saved[4], saved[5], rows_of(dq), rows_of(dk), rows_of(dv),
                     ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble());
     grads = first_order_only({dq, dk, dv});
-    return {grads[0], grads[1], grads[2], Tensor(), Tensor(), Tensor()};
+    return {grads[0], grads[1], grads[2], Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -212,14 +218,15 @@ struct WindowAttentionQKV : public torch::autograd::Function<WindowAttentionQKV>
     const int64_t row = s.hd * qkv.element_size(), stride = (s.Hq + 2 * s.Hkv) * s.hd;
     return {Rows{p, stride}, Rows{p + s.Hq * row, stride}, Rows{p + (s.Hq + s.Hkv) * row, stride}};
   }
-  static Tensor forward(AutogradContext* ctx, const Tensor& qkv_, int64_t Hq, int64_t Hkv, int64_t window, int64_t sinks, double scale) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& qkv_, int64_t Hq, int64_t Hkv, int64_t window, int64_t sinks, double scale,
+                        bool training) {
     c10::cuda::CUDAGuard guard(qkv_.device());
     Tensor qkv = qkv_.contiguous();
     if (reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16) qkv = qkv.clone();
     const Shape s{qkv.size(0), qkv.size(1), Hq, Hkv, qkv.size(2) / (Hq + 2 * Hkv)};
     const auto in = parts(qkv, s);
-    auto [o, lse] = window_forward(s, in[0], in[1], in[2], qkv.options(), window, sinks, scale);
-    ctx->save_for_backward({qkv, o, lse});
+    auto [o, lse, o_lo] = window_forward(s, in[0], in[1], in[2], qkv.options(), window, sinks, scale, training);
+    ctx->save_for_backward({qkv, o, lse, o_lo});
     ctx->saved_data["Hq"] = Hq;
     ctx->saved_data["Hkv"] = Hkv;
     ctx->saved_data["window"] = window;
@@ -236,17 +243,18 @@ struct WindowAttentionQKV : public torch::autograd::Function<WindowAttentionQKV>
     at::AutoDispatchBelowADInplaceOrView below;
     Tensor dqkv = at::empty_like(qkv);
     const auto in = parts(qkv, s), out = parts(dqkv, s);
-    window_backward(s, grads[0], in[0], in[1], in[2], saved[1], saved[2], out[0], out[1], out[2], ctx->saved_data["window"].toInt(),
+    window_backward(s, grads[0], in[0], in[1], in[2], saved[1], saved[2], saved[3], out[0], out[1], out[2], ctx->saved_data["window"].toInt(),
                     ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble());
     grads = first_order_only({dqkv});
-    return {grads[0], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return {grads[0], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
 Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, int64_t sinks, double scale) {
   window_check(q, k, v, window, sinks, scale);
   TORCH_CHECK(q.is_cuda(), "titb200 window_attention: CUDA tensors");
-  return WindowAttention::apply(q, k, v, window, sinks, scale);
+  const bool training = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+  return WindowAttention::apply(q, k, v, window, sinks, scale, training);
 }
 
 void qkv_check(const Tensor& qkv, int64_t Hq, int64_t Hkv) {
@@ -258,7 +266,7 @@ Tensor window_attention_qkv(const Tensor& qkv, int64_t Hq, int64_t Hkv, int64_t 
   TORCH_CHECK(qkv.is_cuda(), "titb200 window_attention: CUDA tensors");
   TORCH_CHECK(Hq % Hkv == 0, "titb200 window_attention: Hq must be a multiple of Hkv");
   limits_check(qkv, qkv.size(0), qkv.size(1), Hq, qkv.size(2) / (Hq + 2 * Hkv), window, sinks, scale);
-  return WindowAttentionQKV::apply(qkv, Hq, Hkv, window, sinks, scale);
+  return WindowAttentionQKV::apply(qkv, Hq, Hkv, window, sinks, scale, at::GradMode::is_enabled() && qkv.requires_grad());
 }
 }  // namespace
 

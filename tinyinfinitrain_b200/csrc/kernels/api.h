@@ -286,10 +286,13 @@ TITB_API int titb_attn_bwd(const TitbAttnDesc* d, cudaStream_t stream);
 // Causal attention over a window and sinks: query i sees key j when j <= i and (i - j < window or j < sinks).  window >= 1,
 // sinks >= 0.  dtype 0 (fp32) or 1 (bf16) for q .. dv; hd a multiple of 8 up to 128.  `attn.dq_accum` is not used: the backward
 // pass takes a workspace of titb_window_attn_bwd_workspace() floats, 16-byte aligned.
+// o_lo (may be null): what the rounding of a bf16 o left, bf16 like o.  The forward pass writes it, the backward pass takes
+// delta = rowsum(dO (o + o_lo)): with few visible keys dP - delta is small beside both, and o's rounding alone would show.
 struct TitbWindowDesc {
   TitbAttnDesc attn;
   int window, sinks, dtype;
   float* workspace;
+  void* o_lo;
 };
 TITB_API long long titb_window_attn_bwd_workspace(const TitbWindowDesc* d);
 TITB_API int titb_window_attn_fwd(const TitbWindowDesc* d, cudaStream_t stream);

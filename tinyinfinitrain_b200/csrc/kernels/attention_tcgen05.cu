@@ -80,6 +80,7 @@ struct AttnArgs {
   int* status;
   // window attention: query i sees key j <= i when i - j < window or j < sinks (both at most T)
   int window, sinks;
+  bf16* o_lo;   // what the rounding of o left, or null
   // its backward pass: key blocks that hold sinks, the query blocks that one of their CTAs takes, and the CTAs of a block
   int sink_blocks, sink_step, sink_parts;
   float* sink_part;  // fp32 [sink_parts][B][sink_blocks][Hkv][dK, dV][kBlk][hd]
@@ -299,7 +300,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
     const uint32_t lane_sel = static_cast<uint32_t>(quad * 32) << 16;
     const float sc = p.scale * kLog2e;
     constexpr float kLazy = 8.f;   // log2 of the largest P value tolerated before the reference maximum moves
-    float m_ref = -INFINITY, l = 0.f;
+    float m_ref = -INFINITY, l = 0.f, l_used = 0.f;
     uint8_t* p_smem = smem + Cfg::kP;
     bool ok = true;
     for (int j = 0; j < nblk; ++j) {
@@ -330,6 +331,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           }
           ptx::tmem_st_wait();
           l *= alpha;
+          l_used *= alpha;
           if (need) m_ref = m_blk;
         }
         return true;
@@ -350,7 +352,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         }
         if (!settle(top * sc)) { ok = false; break; }
         const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
-        float rs0 = 0.f, rs1 = 0.f;
+        float rs0 = 0.f, rs1 = 0.f, ru0 = 0.f, ru1 = 0.f;
 #pragma unroll
         for (int e = 0; e < kSinkCols; e += 2) {
           const float p0 = ex2(fmaf(__uint_as_float(r[e]), sc, neg)), p1 = ex2(fmaf(__uint_as_float(r[e + 1]), sc, neg));
@@ -358,8 +360,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           rs1 += p1;
           pk[e >> 1] = pack_bf16x2(p0, p1);
           pk[8 + (e >> 1)] = 0u;
+          ru0 += __uint_as_float(pk[e >> 1] << 16);
+          ru1 += __uint_as_float(pk[e >> 1] & 0xffff0000u);
         }
         l += rs0 + rs1;
+        l_used += ru0 + ru1;
         if (!waited_o && !ptx::mbar_wait_warp(o_full, (j - 1) & 1, abort_flag)) { ok = false; break; }
         ptx::tmem_st16(tP + lane_sel, pk);
         ptx::tmem_st_wait();
@@ -409,7 +414,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       const float m_blk = (KB == 128 ? fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[KB / 32 - 2], mx[KB / 32 - 1])) : fmaxf(mx[0], mx[1])) * sc;
       if (!settle(m_blk)) { ok = false; break; }
       const float neg = WIN && m_ref == -INFINITY ? 0.f : -m_ref;   // a row may see nothing of its first blocks
-      float rs0 = 0.f, rs1 = 0.f;
+      float rs0 = 0.f, rs1 = 0.f, ru0 = 0.f, ru1 = 0.f;
       auto exp_chunk = [&](uint32_t (&r)[32], int c) {
         uint32_t pk[16];
 #pragma unroll
@@ -420,6 +425,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           p1 = ex2(p1);
           add2(rs0, rs1, rs0, rs1, p0, p1);
           pk[e >> 1] = pack_bf16x2(p0, p1);
+          // O is divided by the sum of what the product takes: the error that P's rounding leaves in it is then in proportion to
+          // v_j - O, and in delta to dP_j - delta, which counts where a row sees few keys
+          if (WIN) add2(ru0, ru1, ru0, ru1, __uint_as_float(pk[e >> 1] << 16), __uint_as_float(pk[e >> 1] & 0xffff0000u));
         }
         if (c == 0 && !waited_o) {
           // P(j-1) V(j-1) must have finished reading the P buffer before it is overwritten
@@ -439,6 +447,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
 #pragma unroll
       for (int c = 1; c < KB / 32; ++c) exp_chunk(r[c], c);
       l += rs0 + rs1;
+      l_used += ru0 + ru1;
       if constexpr (WIN) ptx::tmem_st_wait();
       else ptx::fence_proxy_async_smem();
       ptx::tc_fence_before_sync();
@@ -448,9 +457,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
     if (ok) ok = ptx::mbar_wait_warp(o_full, (nblk - 1) & 1, abort_flag);
     if (ok) {
       ptx::tc_fence_after_sync();
-      const float inv = 1.f / l;
+      const float inv = 1.f / (WIN ? l_used : l);
       bf16* dst = p.o + (static_cast<long long>(b) * p.T + q_idx) * p.o_stride_t + h * HD;
-      uint8_t* q_smem = smem + Cfg::kQ;   // WIN: no product reads Q any more
+      // WIN: no product reads Q or K any more; the rounded rows go there, and what the rounding left
+      uint8_t* q_smem = smem + Cfg::kQ;
+      uint8_t* lo_smem = smem + Cfg::kK;
+      static_assert(!WIN || Cfg::kStages * Cfg::kTileBytes >= Cfg::kQBytes, "room for a tile of rows");
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t r[32];
@@ -465,6 +477,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
             u.z = pack_bf16x2(__uint_as_float(r[d + 4]) * inv, __uint_as_float(r[d + 5]) * inv);
             u.w = pack_bf16x2(__uint_as_float(r[d + 6]) * inv, __uint_as_float(r[d + 7]) * inv);
             *reinterpret_cast<uint4*>(q_smem + swz_off(row, c * 4 + d / 8)) = u;
+            if (p.o_lo) {
+              uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack_bf16x2(fmaf(__uint_as_float(r[d + 2 * e]), inv, -__uint_as_float(w[e] << 16)),
+                                   fmaf(__uint_as_float(r[d + 2 * e + 1]), inv, -__uint_as_float(w[e] & 0xffff0000u)));
+              *reinterpret_cast<uint4*>(lo_smem + swz_off(row, c * 4 + d / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
         } else if (q_idx < p.T) {
 #pragma unroll
@@ -484,9 +504,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
 #pragma unroll 4
         for (int i = lane; i < 32 * (HD / 8); i += 32) {
           const int r = quad * 32 + i / (HD / 8), u = i % (HD / 8);
-          if (q0 + r < p.T)
-            *reinterpret_cast<uint4*>(p.o + (static_cast<long long>(b) * p.T + q0 + r) * p.o_stride_t + h * HD + u * 8) =
-                *reinterpret_cast<const uint4*>(q_smem + swz_off(r, u));
+          if (q0 + r < p.T) {
+            const long long at = (static_cast<long long>(b) * p.T + q0 + r) * p.o_stride_t + h * HD + u * 8;
+            *reinterpret_cast<uint4*>(p.o + at) = *reinterpret_cast<const uint4*>(q_smem + swz_off(r, u));
+            if (p.o_lo) *reinterpret_cast<uint4*>(p.o_lo + at) = *reinterpret_cast<const uint4*>(lo_smem + swz_off(r, u));
+          }
         }
       }
       if (q_idx < p.T)
@@ -965,10 +987,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   if (threadIdx.x == 0 && *abort_flag) atomicExch(p.status, kStatusMbarTimeout);
 }
 
-// delta[b,h,t] = sum_d dO[b,t,h,d] * O[b,t,h,d], and the fp32 dQ accumulator starts at zero.  hd / 8 neighbouring lanes
+// delta[b,h,t] = sum_d dO[b,t,h,d] * O[b,t,h,d] (WIN: with what O's rounding left), and the fp32 dQ accumulator starts at zero.  hd / 8 neighbouring lanes
 // share a (b,t,h) row, 16 bytes of each operand per lane, so that every access of a warp is whole lines.
-template <int HD>
-__global__ void attn_delta_kernel(const bf16* __restrict__ d_o, const bf16* __restrict__ o, float* __restrict__ delta,
+template <int HD, bool WIN>
+__global__ void attn_delta_kernel(const bf16* __restrict__ d_o, const bf16* __restrict__ o, const bf16* __restrict__ o_lo, float* __restrict__ delta,
                                   float* __restrict__ dq_accum, int B, int T, int H, long long do_stride_t, long long o_stride_t) {
   dependents_launch();
   constexpr int L = HD / 8;
@@ -986,6 +1008,11 @@ __global__ void attn_delta_kernel(const bf16* __restrict__ d_o, const bf16* __re
       const float2 a0 = unpack_bf16x2(ua.x), a1 = unpack_bf16x2(ua.y), a2 = unpack_bf16x2(ua.z), a3 = unpack_bf16x2(ua.w);
       const float2 c0 = unpack_bf16x2(uc.x), c1 = unpack_bf16x2(uc.y), c2 = unpack_bf16x2(uc.z), c3 = unpack_bf16x2(uc.w);
       s = a0.x * c0.x + a0.y * c0.y + a1.x * c1.x + a1.y * c1.y + a2.x * c2.x + a2.y * c2.y + a3.x * c3.x + a3.y * c3.y;
+      if (WIN && o_lo) {
+        const uint4 ul = *reinterpret_cast<const uint4*>(o_lo + bt * o_stride_t + h * HD + d);
+        const float2 l0 = unpack_bf16x2(ul.x), l1 = unpack_bf16x2(ul.y), l2 = unpack_bf16x2(ul.z), l3 = unpack_bf16x2(ul.w);
+        s += a0.x * l0.x + a0.y * l0.y + a1.x * l1.x + a1.y * l1.y + a2.x * l2.x + a2.y * l2.y + a3.x * l3.x + a3.y * l3.y;
+      }
       float4* acc = reinterpret_cast<float4*>(dq_accum + i * HD + d);
       acc[0] = make_float4(0.f, 0.f, 0.f, 0.f);
       acc[1] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1067,7 +1094,7 @@ static bool attn_check(const TitbAttnDesc* d) {
 }
 
 template <int HD, bool WIN = false>
-static int attn_fwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 0, int sinks = 0) {
+static int attn_fwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 0, int sinks = 0, void* o_lo = nullptr) {
   using Cfg = FwdCfg<HD, WIN>;
   static bool attr_set[64] = {false};
   int dev = 0;
@@ -1088,7 +1115,7 @@ static int attn_fwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 
   AttnArgs a{};
   a.B = d->B; a.T = d->T; a.Hq = d->Hq; a.Hkv = d->Hkv; a.hd = HD;
   a.scale = d->scale;
-  a.window = window; a.sinks = sinks;
+  a.window = window; a.sinks = sinks; a.o_lo = static_cast<bf16*>(o_lo);
   a.o = static_cast<bf16*>(d->o); a.lse = d->lse; a.o_stride_t = d->o_stride_t;
   a.status = titb_status_ptr();
   dim3 grid(static_cast<unsigned>(d->Hq) * d->B, (d->T + kBlk - 1) / kBlk);
@@ -1112,7 +1139,8 @@ static SinkSplit sink_split(const TitbAttnDesc& d, int window, int sinks) {
 }
 
 template <int HD, bool WIN = false>
-static int attn_bwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 0, int sinks = 0, float* sink_part = nullptr) {
+static int attn_bwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 0, int sinks = 0, float* sink_part = nullptr,
+                           const void* o_lo = nullptr) {
   using Cfg = BwdCfg<HD>;
   static bool attr_set[64] = {false};
   int dev = 0;
@@ -1133,8 +1161,8 @@ static int attn_bwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 
     return TITB_ERR_TENSOR_MAP;
   const long long nrows = static_cast<long long>(d->B) * d->T * d->Hq;
   const long long delta_blocks = (nrows * (HD / 8) + 255) / 256, delta_max = device_sm_count() * 16LL;
-  attn_delta_kernel<HD><<<static_cast<int>(delta_blocks < delta_max ? delta_blocks : delta_max), 256, 0, st>>>(
-      static_cast<const bf16*>(d->d_o), static_cast<const bf16*>(d->o), d->delta, d->dq_accum, d->B, d->T, d->Hq,
+  attn_delta_kernel<HD, WIN><<<static_cast<int>(delta_blocks < delta_max ? delta_blocks : delta_max), 256, 0, st>>>(
+      static_cast<const bf16*>(d->d_o), static_cast<const bf16*>(d->o), static_cast<const bf16*>(o_lo), d->delta, d->dq_accum, d->B, d->T, d->Hq,
       d->do_stride_t, d->o_stride_t);
   AttnArgs a{};
   a.B = d->B; a.T = d->T; a.Hq = d->Hq; a.Hkv = d->Hkv; a.hd = HD;
@@ -1165,12 +1193,12 @@ static int attn_bwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 
 }
 
 // bf16 window attention, hd 64 or 128 (window_attention.cu checks the operands); window and sinks at most T.
-int window_tc_fwd(const TitbAttnDesc* d, int window, int sinks, cudaStream_t st) {
-  return d->hd == 64 ? attn_fwd_launch<64, true>(d, st, window, sinks) : attn_fwd_launch<128, true>(d, st, window, sinks);
+int window_tc_fwd(const TitbAttnDesc* d, int window, int sinks, void* o_lo, cudaStream_t st) {
+  return d->hd == 64 ? attn_fwd_launch<64, true>(d, st, window, sinks, o_lo) : attn_fwd_launch<128, true>(d, st, window, sinks, o_lo);
 }
-int window_tc_bwd(const TitbAttnDesc* d, int window, int sinks, float* sink_part, cudaStream_t st) {
-  return d->hd == 64 ? attn_bwd_launch<64, true>(d, st, window, sinks, sink_part)
-                     : attn_bwd_launch<128, true>(d, st, window, sinks, sink_part);
+int window_tc_bwd(const TitbAttnDesc* d, int window, int sinks, float* sink_part, const void* o_lo, cudaStream_t st) {
+  return d->hd == 64 ? attn_bwd_launch<64, true>(d, st, window, sinks, sink_part, o_lo)
+                     : attn_bwd_launch<128, true>(d, st, window, sinks, sink_part, o_lo);
 }
 long long window_tc_sink_floats(const TitbAttnDesc* d, int window, int sinks) {
   const SinkSplit s = sink_split(*d, window, sinks);

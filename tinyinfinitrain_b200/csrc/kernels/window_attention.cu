@@ -18,8 +18,8 @@
 namespace titb {
 
 // bf16 heads of 64 and 128 (attention_tcgen05.cu)
-int window_tc_fwd(const TitbAttnDesc* d, int window, int sinks, cudaStream_t st);
-int window_tc_bwd(const TitbAttnDesc* d, int window, int sinks, float* sink_part, cudaStream_t st);
+int window_tc_fwd(const TitbAttnDesc* d, int window, int sinks, void* o_lo, cudaStream_t st);
+int window_tc_bwd(const TitbAttnDesc* d, int window, int sinks, float* sink_part, const void* o_lo, cudaStream_t st);
 long long window_tc_sink_floats(const TitbAttnDesc* d, int window, int sinks);
 
 constexpr int kWinThreads = 128;   // 8 x 16 threads of 4 x 4 scores
@@ -32,6 +32,7 @@ constexpr int kWeightPitch = kWinRows + 4;
 struct WinArgs {
   const void *q, *k, *v, *d_o;
   void *o, *dq, *dk, *dv;
+  bf16* o_lo;   // what the rounding of a bf16 o left, or null
   float *lse, *delta;
   int B, T, Hq, Hkv, hd, window, sinks;
   float scale;
@@ -225,6 +226,13 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
     if (tx == 0 && i < p.T) p.lse[(static_cast<long long>(b) * p.Hq + h) * p.T + i] = m[r] + logf(l[r]);
   }
   store_rows<T, HD>(static_cast<T*>(p.o) + row0 * p.o_st + h * p.hd, p.o_st, q0, p.T, p.hd, acc, ty, tx);
+  if (sizeof(T) == 2 && p.o_lo) {
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[e / 4][e % 4][r] -= to_f32(from_f32<T>(acc[e / 4][e % 4][r]));
+    store_rows<bf16, HD>(p.o_lo + row0 * p.o_st + h * p.hd, p.o_st, q0, p.T, p.hd, acc, ty, tx);
+  }
 }
 
 template <int HD>
@@ -262,6 +270,10 @@ __global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p)
     for (int c = 0; c < HD / 64; ++c) {
       const float4 a = load4(d_o, i, p.do_st, c * 64 + tx * 4, p.T, p.hd), x = load4(o, i, p.o_st, c * 64 + tx * 4, p.T, p.hd);
       s += a.x * x.x + a.y * x.y + a.z * x.z + a.w * x.w;
+      if (sizeof(T) == 2 && p.o_lo) {
+        const float4 y = load4(static_cast<const bf16*>(p.o_lo) + row0 * p.o_st + h * p.hd, i, p.o_st, c * 64 + tx * 4, p.T, p.hd);
+        s += a.x * y.x + a.y * y.y + a.z * y.z + a.w * y.w;
+      }
     }
     delta[r] = half_warp_sum(s);
     lse[r] = i < p.T ? p.lse[stat0 + i] : 0.f;
@@ -419,7 +431,7 @@ static WinArgs win_args(const TitbWindowDesc* w) {
   a.q = d.q; a.k = d.k; a.v = d.v; a.o = d.o; a.lse = d.lse;
   a.d_o = d.d_o; a.dq = d.dq; a.dk = d.dk; a.dv = d.dv; a.delta = d.delta;
   a.B = d.B; a.T = d.T; a.Hq = d.Hq; a.Hkv = d.Hkv; a.hd = d.hd; a.scale = d.scale;
-  a.window = window_of(w); a.sinks = sinks_of(w);
+  a.window = window_of(w); a.sinks = sinks_of(w); a.o_lo = static_cast<bf16*>(w->o_lo);
   a.q_st = d.q_stride_t; a.k_st = d.k_stride_t; a.v_st = d.v_stride_t; a.o_st = d.o_stride_t;
   a.do_st = d.do_stride_t; a.dq_st = d.dq_stride_t; a.dk_st = d.dk_stride_t; a.dv_st = d.dv_stride_t;
   return a;
@@ -461,6 +473,7 @@ static int win_check(const TitbWindowDesc* w, bool backward) {
   if (static_cast<long long>(d.Hq) * d.B > 0x7fffffffLL || (d.T + kWinRows - 1LL) / kWinRows > 32767) return TITB_ERR_SHAPE;
   const int mask = w->dtype == 1 ? 7 : 3;
   auto bad = [&](const void* p, long long st) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0 || (st & mask) != 0; };
+  if (reinterpret_cast<uintptr_t>(w->o_lo) & 15) return TITB_ERR_ALIGNMENT;
   if (bad(d.q, d.q_stride_t) || bad(d.k, d.k_stride_t) || bad(d.v, d.v_stride_t) || bad(d.o, d.o_stride_t))
     return TITB_ERR_ALIGNMENT;
   if (backward && (bad(d.d_o, d.do_stride_t) || bad(d.dq, d.dq_stride_t) || bad(d.dk, d.dk_stride_t) || bad(d.dv, d.dv_stride_t)))
@@ -476,7 +489,7 @@ TITB_API int titb_window_attn_fwd(const TitbWindowDesc* w, cudaStream_t st) {
   (void)cudaGetLastError();
   if (w->attn.B <= 0 || w->attn.T <= 0 || w->attn.Hq <= 0) return 0;
   if (const int rc = win_check(w, false)) return rc;
-  if (on_tensor_cores(w)) return window_tc_fwd(&w->attn, window_of(w), sinks_of(w), st);
+  if (on_tensor_cores(w)) return window_tc_fwd(&w->attn, window_of(w), sinks_of(w), w->o_lo, st);
   if (w->dtype == 1) return w->attn.hd <= 64 ? win_fwd<bf16, 64>(w, st) : win_fwd<bf16, 128>(w, st);
   return w->attn.hd <= 64 ? win_fwd<float, 64>(w, st) : win_fwd<float, 128>(w, st);
 }
@@ -489,7 +502,7 @@ TITB_API int titb_window_attn_bwd(const TitbWindowDesc* w, cudaStream_t st) {
     TitbAttnDesc d = w->attn;
     d.dq_accum = w->workspace;
     float* sink_part = w->workspace + static_cast<long long>(d.B) * d.T * d.Hq * d.hd;
-    return window_tc_bwd(&d, window_of(w), sinks_of(w), sink_part, st);
+    return window_tc_bwd(&d, window_of(w), sinks_of(w), sink_part, w->o_lo, st);
   }
   if (w->dtype == 1) return w->attn.hd <= 64 ? win_bwd<bf16, 64>(w, st) : win_bwd<bf16, 128>(w, st);
   return w->attn.hd <= 64 ? win_bwd<float, 64>(w, st) : win_bwd<float, 128>(w, st);
