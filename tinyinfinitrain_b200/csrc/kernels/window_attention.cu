@@ -22,9 +22,10 @@ int window_tc_fwd(const TitbAttnDesc* d, int window, int sinks, void* o_lo, cuda
 int window_tc_bwd(const TitbAttnDesc* d, int window, int sinks, float* sink_part, const void* o_lo, cudaStream_t st);
 long long window_tc_sink_floats(const TitbAttnDesc* d, int window, int sinks);
 
-constexpr int kWinThreads = 128;   // 8 x 16 threads of 4 x 4 scores
+constexpr int kWinThreads = 128;   // 8 x 16 threads of 4 x 2 scores
 constexpr int kWinRows = 32;       // rows of the tile that a CTA owns
-constexpr int kWinStep = 64;       // rows of the other operand that arrive at a time
+constexpr int kWinStep = 32;       // rows of the other operand that arrive at a time, while those before are multiplied
+constexpr int kCols = kWinStep / 16;
 // Tiles are [rows][HD + 4], weights [step row][kWeightPitch]: odd numbers of 16-byte units, so that rows that neighbouring lanes
 // read or write lie in different banks.
 constexpr int kWeightPitch = kWinRows + 4;
@@ -74,6 +75,37 @@ __device__ __forceinline__ void load_tile(const T* base, long long stride, int t
   }
 }
 
+// The same while the CTA computes on: fp32 rows are copied asynchronously (wait_tiles ends the wait for all but the copies that
+// were issued last), bf16 rows have to be converted on their way.
+template <typename T, int HD>
+__device__ __forceinline__ void fetch_tile(const T* base, long long stride, int t0, int n_rows, int hd, float* tile) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll 8
+    for (int i = threadIdx.x; i < kWinStep * HD / 4; i += kWinThreads) {
+      const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+      const bool real = t0 + r < n_rows && d < hd;
+      const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(tile + r * (HD + 4) + d));
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
+                   "l"(base + (real ? (t0 + r) * stride + d : 0LL)), "r"(real ? 16 : 0)
+                   : "memory");
+    }
+  } else {
+    load_tile<T, HD, kWinStep>(base, stride, t0, n_rows, hd, tile);
+  }
+}
+// 32 floats from element t0 on; zeros past the sequence.
+__device__ __forceinline__ void fetch_row(const float* base, int t0, int n, float* row, int lane) {
+  const bool real = t0 + lane < n;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(row + lane))),
+               "l"(base + (real ? t0 + lane : 0)), "r"(real ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void commit_tiles() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void wait_tiles() {
+  asm volatile("cp.async.wait_group 1;" ::: "memory");
+  __syncthreads();
+}
+
 __device__ __forceinline__ float half_warp_max(float v) {
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -88,19 +120,19 @@ __device__ __forceinline__ float half_warp_sum(float v) {
 // acc[r][c] = own row ty * 4 + r times step row tx + 16 c.  Even and odd elements of the head are summed apart, two to an
 // instruction.
 template <int HD>
-__device__ __forceinline__ void scores(float (&acc)[4][4], const float* own, const float* step, int ty, int tx) {
-  float even[4][4] = {}, odd[4][4] = {};
+__device__ __forceinline__ void scores(float (&acc)[4][kCols], const float* own, const float* step, int ty, int tx) {
+  float even[4][kCols] = {}, odd[4][kCols] = {};
 #pragma unroll 4
   for (int d = 0; d < HD; d += 4) {
-    float4 a[4], b[4];
+    float4 a[4], b[kCols];
 #pragma unroll
     for (int r = 0; r < 4; ++r) a[r] = *reinterpret_cast<const float4*>(own + (ty * 4 + r) * (HD + 4) + d);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) b[c] = *reinterpret_cast<const float4*>(step + (tx + 16 * c) * (HD + 4) + d);
+    for (int c = 0; c < kCols; ++c) b[c] = *reinterpret_cast<const float4*>(step + (tx + 16 * c) * (HD + 4) + d);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < kCols; ++c) {
         fma2(even[r][c], odd[r][c], a[r].x, a[r].y, b[c].x, b[c].y, even[r][c], odd[r][c]);
         fma2(even[r][c], odd[r][c], a[r].z, a[r].w, b[c].z, b[c].w, even[r][c], odd[r][c]);
       }
@@ -108,12 +140,12 @@ __device__ __forceinline__ void scores(float (&acc)[4][4], const float* own, con
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc[r][c] = even[r][c] + odd[r][c];
+    for (int c = 0; c < kCols; ++c) acc[r][c] = even[r][c] + odd[r][c];
 }
 // w ([step row][own row]) <- s
-__device__ __forceinline__ void store_weights(float* w, const float (&s)[4][4], int ty, int tx) {
+__device__ __forceinline__ void store_weights(float* w, const float (&s)[4][kCols], int ty, int tx) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+  for (int c = 0; c < kCols; ++c)
     *reinterpret_cast<float4*>(w + (tx + 16 * c) * kWeightPitch + ty * 4) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
 }
 // acc[r] += sum over the step's rows n of w[n][own row ty * 4 + r] times elements 64 c + 4 tx .. of row n; two rows to an
@@ -155,7 +187,8 @@ __device__ __forceinline__ void store_rows(T* base, long long stride, int t0, in
 
 template <int HD>
 struct WinFwdSmem {
-  static constexpr int kQ = 0, kK = kQ + kWinRows * (HD + 4), kV = kK + kWinStep * (HD + 4), kP = kV + kWinStep * (HD + 4);
+  static constexpr int kTile = kWinStep * (HD + 4);   // K and V in two buffers each
+  static constexpr int kQ = 0, kK = kQ + kWinRows * (HD + 4), kV = kK + 2 * kTile, kP = kV + 2 * kTile;
   static constexpr int kBytes = (kP + kWinStep * kWeightPitch) * 4;
 };
 
@@ -182,20 +215,27 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
   const int first = max(0, q0 - p.window + 1) / kWinStep, last = min(q0 + kWinRows, p.T) - 1;
   const int sink_steps = min((p.sinks + kWinStep - 1) / kWinStep, first);
   const int n_steps = sink_steps + last / kWinStep - first + 1;
+  const auto key0 = [&](int it) { return (it < sink_steps ? it : first + it - sink_steps) * kWinStep; };
+  const auto fetch = [&](int it) {
+    if (it < n_steps) {
+      fetch_tile<T, HD>(k, p.k_st, key0(it), p.T, p.hd, Ks + (it & 1) * Sm::kTile);
+      fetch_tile<T, HD>(v, p.v_st, key0(it), p.T, p.hd, Vs + (it & 1) * Sm::kTile);
+    }
+    commit_tiles();
+  };
+  fetch(0);
   for (int it = 0; it < n_steps; ++it) {
-    const int k0 = (it < sink_steps ? it : first + it - sink_steps) * kWinStep;
-    __syncthreads();
-    load_tile<T, HD, kWinStep>(k, p.k_st, k0, p.T, p.hd, Ks);
-    load_tile<T, HD, kWinStep>(v, p.v_st, k0, p.T, p.hd, Vs);
-    __syncthreads();
-    float s[4][4];
-    scores<HD>(s, Qs, Ks, ty, tx);
+    const int k0 = key0(it);
+    fetch(it + 1);
+    wait_tiles();
+    float s[4][kCols];
+    scores<HD>(s, Qs, Ks + (it & 1) * Sm::kTile, ty, tx);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = q0 + ty * 4 + r;
       float top = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < kCols; ++c) {
         s[r][c] = win_visible(i, k0 + tx + 16 * c, p.window, p.sinks) ? s[r][c] * p.scale : -INFINITY;
         top = fmaxf(top, s[r][c]);
       }
@@ -204,7 +244,7 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
       const float keep = expf(m[r] - ref);
       float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < kCols; ++c) {
         s[r][c] = expf(s[r][c] - ref);
         sum += s[r][c];
       }
@@ -215,7 +255,8 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
     }
     store_weights(Ps, s, ty, tx);
     __syncthreads();
-    accumulate<HD>(acc, Ps, Vs, ty, tx);
+    accumulate<HD>(acc, Ps, Vs + (it & 1) * Sm::kTile, ty, tx);
+    __syncthreads();
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -237,8 +278,8 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
 
 template <int HD>
 struct WinDqSmem {
-  static constexpr int kQ = 0, kDO = kQ + kWinRows * (HD + 4), kK = kDO + kWinRows * (HD + 4), kV = kK + kWinStep * (HD + 4),
-                       kDS = kV + kWinStep * (HD + 4);
+  static constexpr int kTile = kWinStep * (HD + 4);
+  static constexpr int kQ = 0, kDO = kQ + kWinRows * (HD + 4), kK = kDO + kWinRows * (HD + 4), kV = kK + 2 * kTile, kDS = kV + 2 * kTile;
   static constexpr int kBytes = (kDS + kWinStep * kWeightPitch) * 4;
 };
 
@@ -283,35 +324,44 @@ __global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p)
   const int first = max(0, q0 - p.window + 1) / kWinStep, last = min(q0 + kWinRows, p.T) - 1;
   const int sink_steps = min((p.sinks + kWinStep - 1) / kWinStep, first);
   const int n_steps = sink_steps + last / kWinStep - first + 1;
+  const auto key0 = [&](int it) { return (it < sink_steps ? it : first + it - sink_steps) * kWinStep; };
+  const auto fetch = [&](int it) {
+    if (it < n_steps) {
+      fetch_tile<T, HD>(k, p.k_st, key0(it), p.T, p.hd, Ks + (it & 1) * Sm::kTile);
+      fetch_tile<T, HD>(v, p.v_st, key0(it), p.T, p.hd, Vs + (it & 1) * Sm::kTile);
+    }
+    commit_tiles();
+  };
+  fetch(0);
   for (int it = 0; it < n_steps; ++it) {
-    const int k0 = (it < sink_steps ? it : first + it - sink_steps) * kWinStep;
-    __syncthreads();
-    load_tile<T, HD, kWinStep>(k, p.k_st, k0, p.T, p.hd, Ks);
-    load_tile<T, HD, kWinStep>(v, p.v_st, k0, p.T, p.hd, Vs);
-    __syncthreads();
-    float s[4][4], dp[4][4];
-    scores<HD>(s, Qs, Ks, ty, tx);
-    scores<HD>(dp, Ds, Vs, ty, tx);
+    const int k0 = key0(it);
+    fetch(it + 1);
+    wait_tiles();
+    float s[4][kCols], dp[4][kCols];
+    scores<HD>(s, Qs, Ks + (it & 1) * Sm::kTile, ty, tx);
+    scores<HD>(dp, Ds, Vs + (it & 1) * Sm::kTile, ty, tx);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < kCols; ++c) {
         const int i = q0 + ty * 4 + r;
         const bool see = i < p.T && win_visible(i, k0 + tx + 16 * c, p.window, p.sinks);
         s[r][c] = see ? expf(s[r][c] * p.scale - lse[r]) * (dp[r][c] - delta[r]) * p.scale : 0.f;
       }
     store_weights(Ss, s, ty, tx);
     __syncthreads();
-    accumulate<HD>(acc, Ss, Ks, ty, tx);
+    accumulate<HD>(acc, Ss, Ks + (it & 1) * Sm::kTile, ty, tx);
+    __syncthreads();
   }
   store_rows<T, HD>(static_cast<T*>(p.dq) + row0 * p.dq_st + h * p.hd, p.dq_st, q0, p.T, p.hd, acc, ty, tx);
 }
 
 template <int HD>
 struct WinDkvSmem {
-  static constexpr int kK = 0, kV = kK + kWinRows * (HD + 4), kQ = kV + kWinRows * (HD + 4), kDO = kQ + kWinStep * (HD + 4),
-                       kP = kDO + kWinStep * (HD + 4), kDS = kP + kWinStep * kWeightPitch;
-  static constexpr int kBytes = (kDS + kWinStep * kWeightPitch) * 4;
+  static constexpr int kTile = kWinStep * (HD + 4);
+  static constexpr int kK = 0, kV = kK + kWinRows * (HD + 4), kQ = kV + kWinRows * (HD + 4), kDO = kQ + 2 * kTile, kP = kDO + 2 * kTile,
+                       kDS = kP + kWinStep * kWeightPitch, kStat = kDS + kWinStep * kWeightPitch;   // lse and delta, two buffers
+  static constexpr int kBytes = (kStat + 4 * kWinStep) * 4;
 };
 
 // One CTA per 32 keys of a kv head, over the query heads that share it; reads the delta that window_dq_kernel wrote.  The
@@ -320,7 +370,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p) {
   using Sm = WinDkvSmem<HD>;
   extern __shared__ __align__(16) float sm[];
-  float *Ks = sm + Sm::kK, *Vs = sm + Sm::kV, *Qs = sm + Sm::kQ, *Ds = sm + Sm::kDO, *Ps = sm + Sm::kP, *Ss = sm + Sm::kDS;
+  float *Ks = sm + Sm::kK, *Vs = sm + Sm::kV, *Qs = sm + Sm::kQ, *Ds = sm + Sm::kDO, *Ps = sm + Sm::kP, *Ss = sm + Sm::kDS, *stat = sm + Sm::kStat;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int hk = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv, G = p.Hq / p.Hkv;
   const int n_sink_ctas = p.sink_tiles * p.sink_parts, y = blockIdx.y;
@@ -338,27 +388,35 @@ __global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p
   load_tile<T, HD, kWinRows>(static_cast<const T*>(p.k) + row0 * p.k_st + hk * p.hd, p.k_st, k0, p.T, p.hd, Ks);
   load_tile<T, HD, kWinRows>(static_cast<const T*>(p.v) + row0 * p.v_st + hk * p.hd, p.v_st, k0, p.T, p.hd, Vs);
   float dk[HD / 64][4][4] = {}, dv[HD / 64][4][4] = {};
-  for (int it = 0; it < G * n_steps; ++it) {
-    const int h = hk * G + it / n_steps, q0 = (first + it % n_steps) * kWinStep;
-    const long long stat0 = (static_cast<long long>(b) * p.Hq + h) * p.T;
-    __syncthreads();
-    load_tile<T, HD, kWinStep>(static_cast<const T*>(p.q) + row0 * p.q_st + h * p.hd, p.q_st, q0, p.T, p.hd, Qs);
-    load_tile<T, HD, kWinStep>(static_cast<const T*>(p.d_o) + row0 * p.do_st + h * p.hd, p.do_st, q0, p.T, p.hd, Ds);
-    float lse[4], delta[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int i = q0 + tx + 16 * c;
-      lse[c] = i < p.T ? p.lse[stat0 + i] : 0.f;
-      delta[c] = i < p.T ? p.delta[stat0 + i] : 0.f;
+  const int n_all = G * n_steps;
+  const auto fetch = [&](int it) {
+    if (it < n_all) {
+      const int h = hk * G + it / n_steps, q0 = (first + it % n_steps) * kWinStep, buf = it & 1;
+      const long long stat0 = (static_cast<long long>(b) * p.Hq + h) * p.T;
+      fetch_tile<T, HD>(static_cast<const T*>(p.q) + row0 * p.q_st + h * p.hd, p.q_st, q0, p.T, p.hd, Qs + buf * Sm::kTile);
+      fetch_tile<T, HD>(static_cast<const T*>(p.d_o) + row0 * p.do_st + h * p.hd, p.do_st, q0, p.T, p.hd, Ds + buf * Sm::kTile);
+      if (threadIdx.x < 32) fetch_row(p.lse + stat0, q0, p.T, stat + buf * 2 * kWinStep, threadIdx.x);
+      else if (threadIdx.x < 64) fetch_row(p.delta + stat0, q0, p.T, stat + buf * 2 * kWinStep + kWinStep, threadIdx.x - 32);
     }
-    __syncthreads();
-    float s[4][4], dp[4][4];
-    scores<HD>(s, Ks, Qs, ty, tx);
-    scores<HD>(dp, Vs, Ds, ty, tx);
+    commit_tiles();
+  };
+  fetch(0);
+  for (int it = 0; it < n_all; ++it) {
+    const int q0 = (first + it % n_steps) * kWinStep, buf = it & 1;
+    fetch(it + 1);
+    wait_tiles();
+    float s[4][kCols], dp[4][kCols], lse[kCols], delta[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      lse[c] = stat[buf * 2 * kWinStep + tx + 16 * c];
+      delta[c] = stat[buf * 2 * kWinStep + kWinStep + tx + 16 * c];
+    }
+    scores<HD>(s, Ks, Qs + buf * Sm::kTile, ty, tx);
+    scores<HD>(dp, Vs, Ds + buf * Sm::kTile, ty, tx);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < kCols; ++c) {
         const int i = q0 + tx + 16 * c, j = k0 + ty * 4 + r;
         const bool see = i < p.T && win_visible(i, j, p.window, p.sinks);
         const float prob = see ? expf(s[r][c] * p.scale - lse[c]) : 0.f;
@@ -368,8 +426,9 @@ __global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p
     store_weights(Ps, s, ty, tx);
     store_weights(Ss, dp, ty, tx);
     __syncthreads();
-    accumulate<HD>(dv, Ps, Ds, ty, tx);
-    accumulate<HD>(dk, Ss, Qs, ty, tx);
+    accumulate<HD>(dv, Ps, Ds + buf * Sm::kTile, ty, tx);
+    accumulate<HD>(dk, Ss, Qs + buf * Sm::kTile, ty, tx);
+    __syncthreads();
   }
   if (part == 0) {   // holds all queries that see keys of the tile that are no sinks
     store_rows<T, HD>(static_cast<T*>(p.dk) + row0 * p.dk_st + hk * p.hd, p.dk_st, k0, p.T, p.hd, dk, ty, tx);
