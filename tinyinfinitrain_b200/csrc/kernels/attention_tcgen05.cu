@@ -138,7 +138,7 @@ struct FwdCfg {
 // lies over S and S(j+1) is issued behind P(j) V(j), which costs nothing beside two other CTAs (columns of its own, in a
 // second allocation, were as fast).
 // Measured (B200): hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: one CTA an SM 254 us, two with 128 keys a step, P over S
-// and S(j+1) issued behind P(j) V(j) 182 us, as it is 165 us (790 TFLOP/s of what the rows see); hd 64, 1 x 1999, 32 / 8 heads,
+// and S(j+1) issued behind P(j) V(j) 182 us, as it is 165 us (790 TFLOP/s of what the rows see; 178 us where a backward pass follows); hd 64, 1 x 1999, 32 / 8 heads,
 // window 512: 29 us before, 26 us.  A step of 64 keys takes 1660 cycles (hd 128) and 2140 (hd 64, three CTAs), 920 and 1060 of
 // them for the exponentials; a quarter of those on the multiply-add pipe changed nothing.  Set-up, first loads and output
 // take another 8000 and 5500 cycles of a CTA.

@@ -199,6 +199,7 @@ class GPT2(nn.Module):
         if cache is not None:
             assert targets is None, "a cache is for generating text: there is no loss"
             return self._forward_cached(idx, cache, counts)
+        assert counts is None, "counts go with a cache"
         tr = self.transformer
         x = ops.embedding(idx, tr["wte"].weight, tr["wpe"].weight)
         for block in tr["h"]:
