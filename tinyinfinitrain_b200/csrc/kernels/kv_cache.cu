@@ -82,61 +82,68 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) cache_append_kern
   constexpr int U = 2;
   __shared__ __align__(16) float sin_of[kAppendTokens][kMaxHalf], cos_of[kAppendTokens][kMaxHalf];
   __shared__ long long row_of[kAppendTokens];   // of the cache, of kv head 0 (the others follow page_size rows apart); -1: none
+  __shared__ long long src_of[kAppendTokens];   // of the projection
   dependency_wait();
   dependents_launch();
   const CacheArgs& c = p.c;
   const int half = c.hd / 2, chunks = half / V, heads = c.Hq + 2 * c.Hkv, rotated = p.rotate ? c.Hq + c.Hkv : 0;
   const int h0 = blockIdx.y * p.per, nh = min(p.per, heads - h0);
-  const int bt0 = blockIdx.x * p.tokens, nt = min(p.tokens, c.B * p.T - bt0), n = nt * nh * chunks;
-  Pack<T, V> lo[U], hi[U];
-  int k[U], h[U], i[U];
-  auto load = [&](int x) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int y = x + u * kAppendThreads, z = y / chunks;
-      i[u] = (y - z * chunks) * V;
-      k[u] = z / nh;
-      h[u] = h0 + z - k[u] * nh;
-      if (y >= n || (h[u] < c.Hq && !p.q_out)) {
-        k[u] = -1;
-        continue;
-      }
-      const int b = (bt0 + k[u]) / p.T, t = bt0 + k[u] - b * p.T;
-      const T* src = static_cast<const T*>(p.qkv) + b * p.stride_b + t * p.stride_t + static_cast<long long>(h[u]) * c.hd + i[u];
-      lo[u] = *reinterpret_cast<const Pack<T, V>*>(src);
-      hi[u] = *reinterpret_cast<const Pack<T, V>*>(src + half);
-    }
-  };
-  load(threadIdx.x);   // on their way while the angles are taken
-  if (h0 < rotated)
-    for (int x = threadIdx.x; x < nt * half; x += kAppendThreads) {
-      const int kk = x / half, e = x - kk * half, b = (bt0 + kk) / p.T, t = bt0 + kk - b * p.T;
-      rope_sincos(static_cast<int>(static_cast<long long>(p.starts[b]) + t), p.turns[e], sin_of[kk][e], cos_of[kk][e]);
-    }
-  if (threadIdx.x >= kAppendThreads - kAppendTokens) {
-    const int kk = kAppendThreads - 1 - threadIdx.x;
-    if (kk < nt && h0 + nh > c.Hq) {
+  const int bt0 = blockIdx.x * p.tokens, nt = min(p.tokens, c.B * p.T - bt0);
+  if (threadIdx.x < kAppendTokens) {
+    const int kk = threadIdx.x;
+    if (kk < nt) {
       const int b = (bt0 + kk) / p.T, t = bt0 + kk - b * p.T;
+      src_of[kk] = b * p.stride_b + t * p.stride_t;
       const int start = p.starts[b], count = p.counts ? min(p.counts[b], p.T) : p.T;
       const long long pos = static_cast<long long>(start) + t;
       long long row = -1;
-      if (t < count && (pos >= static_cast<long long>(start) + count - c.window || pos < c.sinks)) {
+      if (h0 + nh > c.Hq && t < count && (pos >= static_cast<long long>(start) + count - c.window || pos < c.sinks)) {
         if (pos <= 0x7fffffffLL) row = c.map(b).row(static_cast<int>(pos), c.Hkv, 0);
         if (row < 0) atomicExch(c.status, kStatusBadPage);
       }
       row_of[kk] = row;
     }
   }
+  if (h0 < rotated)
+    for (int x = threadIdx.x; x < nt * half; x += kAppendThreads) {
+      const int kk = x / half, e = x - kk * half, b = (bt0 + kk) / p.T, t = bt0 + kk - b * p.T;
+      rope_sincos(static_cast<int>(static_cast<long long>(p.starts[b]) + t), p.turns[e], sin_of[kk][e], cos_of[kk][e]);
+    }
   __syncthreads();
-  for (int x = threadIdx.x; x < n;) {
+  // a thread stays at its place in the heads and steps from head to head: (token, head) pairs in a row, `lanes` at a time
+  const int lanes = kAppendThreads / chunks, i = static_cast<int>(threadIdx.x) % chunks * V;
+  int h = static_cast<int>(threadIdx.x) / chunks, k = 0;
+  if (h >= lanes) return;   // what does not fill a row of chunks
+  const auto settle = [&]() {
+    while (h >= nh) {
+      h -= nh;
+      ++k;
+    }
+  };
+  settle();
+  while (k < nt) {
+    Pack<T, V> lo[U], hi[U];
+    int ku[U], hu[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (k[u] < 0) continue;
-      if (h[u] < rotated) {
+      ku[u] = k < nt && (h0 + h >= c.Hq || p.q_out) ? k : -1;
+      hu[u] = h0 + h;
+      if (ku[u] >= 0) {
+        const T* src = static_cast<const T*>(p.qkv) + src_of[k] + static_cast<long long>(hu[u]) * c.hd + i;
+        lo[u] = *reinterpret_cast<const Pack<T, V>*>(src);
+        hi[u] = *reinterpret_cast<const Pack<T, V>*>(src + half);
+      }
+      h += lanes;
+      settle();
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (ku[u] < 0) continue;
+      if (hu[u] < rotated) {
 #pragma unroll
         for (int e = 0; e < V; e += 4) {
-          const float4 sn = *reinterpret_cast<const float4*>(&sin_of[k[u]][i[u] + e]);
-          const float4 cs = *reinterpret_cast<const float4*>(&cos_of[k[u]][i[u] + e]);
+          const float4 sn = *reinterpret_cast<const float4*>(&sin_of[ku[u]][i + e]);
+          const float4 cs = *reinterpret_cast<const float4*>(&cos_of[ku[u]][i + e]);
           const float s4[4] = {sn.x, sn.y, sn.z, sn.w}, c4[4] = {cs.x, cs.y, cs.z, cs.w};
 #pragma unroll
           for (int f = 0; f < 4; ++f) {
@@ -147,21 +154,19 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) cache_append_kern
         }
       }
       auto put = [&](void* base, long long r) {
-        T* dst = static_cast<T*>(base) + r * c.hd + i[u];
+        T* dst = static_cast<T*>(base) + r * c.hd + i;
         *reinterpret_cast<Pack<T, V>*>(dst) = lo[u];
         *reinterpret_cast<Pack<T, V>*>(dst + half) = hi[u];
       };
-      if (h[u] < c.Hq) {
-        put(p.q_out, static_cast<long long>(bt0 + k[u]) * c.Hq + h[u]);
+      if (hu[u] < c.Hq) {
+        put(p.q_out, static_cast<long long>(bt0 + ku[u]) * c.Hq + hu[u]);
         continue;
       }
-      const bool key = h[u] < c.Hq + c.Hkv;
-      const int hk = h[u] - c.Hq - (key ? 0 : c.Hkv);
-      if (key && p.k_out) put(p.k_out, static_cast<long long>(bt0 + k[u]) * c.Hkv + hk);
-      if (row_of[k[u]] >= 0) put(key ? c.k_cache : c.v_cache, row_of[k[u]] + static_cast<long long>(hk) * c.page_size);
+      const bool key = hu[u] < c.Hq + c.Hkv;
+      const int hk = hu[u] - c.Hq - (key ? 0 : c.Hkv);
+      if (key && p.k_out) put(p.k_out, static_cast<long long>(bt0 + ku[u]) * c.Hkv + hk);
+      if (row_of[ku[u]] >= 0) put(key ? c.k_cache : c.v_cache, row_of[ku[u]] + static_cast<long long>(hk) * c.page_size);
     }
-    x += U * kAppendThreads;
-    if (x < n) load(x);
   }
 }
 
