@@ -572,6 +572,8 @@ struct BwdCfg {
 // WIN: a window and sinks.  A block of keys meets the query blocks up to its last key's window.  A block that holds sinks meets
 // all later ones, which would make its CTA the last by far: its query blocks are split over sink_parts CTAs, which leave
 // fp32 sums of the sinks' rows that attn_window_finish_kernel adds in order.
+// Measured: hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: 396 us, 1070 TFLOP/s of the tiles it visits, an eighth of them
+// masked and a tenth for the sinks; the same parts as above bound it.
 template <int HD, bool WIN>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,

@@ -74,7 +74,9 @@ __device__ __forceinline__ void rope_sincos(int pos, double turns, float& sn, fl
 // A CTA takes up to kAppendTokens tokens and `per` of their heads.  The sines and cosines of its tokens go to shared memory once
 // (their 64-bit reduction costs more than a head's bytes), then a thread moves V neighbouring elements of both halves of a
 // head at a time, two of them in flight.  Bound by memory.  Before, every thread took the angles of eight heads of its own:
-// 112 registers, 13 warps on an SM, 31 us for 2 x 1999 tokens, 32 / 8 heads of 128 (106 MB); now 25 us (4.3 TB/s).
+// 112 registers, 13 warps on an SM, 31 us for 2 x 1999 tokens, 32 / 8 heads of 128 (106 MB); now 23.5 us (4.5 TB/s).  Asking
+// for the rows ahead of the angles (prefetch to the L2) did not help.  64 single tokens: 5 us, of which the launch, positions,
+// page table and angles one behind the other are most.
 constexpr int kAppendTokens = 8, kAppendThreads = 256, kAppendCtas = 4;   // the last: CTAs of an SM
 
 template <typename T, int V>
@@ -409,7 +411,10 @@ __device__ __forceinline__ void note_join(const PagedArgs& p, const Run& run, co
 }
 
 // ---- any head size, fp32 arithmetic on the CUDA cores.  L lanes hold a row (16 bytes each); every group of L lanes takes rows
-// of its own, kBatch at a time, and keeps its own running maximum, sum and output.
+// of its own, kBatch at a time, and keeps its own running maximum, sum and output.  Serves fp32 caches, whose products the
+// matrix instructions would round, and head sizes that those do not take.  Four query heads share a row's loads: more would
+// cost the registers that keep 16 warps on an SM.  Bound by the latency of page table and rows on short caches: 4 sequences of 777
+// positions, 12 heads of 64: 12 us with the join (90 us as one CTA an item).
 constexpr int kPagedHeads = 4;   // query heads that share the loads of a pass over the cache
 constexpr int kPagedTile = 64;
 

@@ -10,6 +10,10 @@
 // and those from its first query's window to its own; a tile of keys meets the query tiles up to its last key's window, or
 // all later ones when a sink lies in it.  All arithmetic is fp32.  The backward pass takes the scores twice, once per key tile
 // (dK, dV) and once per query tile (delta, dQ), so that every sum has one owner and a fixed order: no atomics.
+// Bound by the reads of shared memory: two 16-byte reads feed eight packed multiply-adds (70 % of what the SM can read; a layout
+// with half as many distinct words a read changed nothing), and by tiles that are half masked where the window is short.
+// Measured (B200), 2 x 512 tokens, 12 heads of 64, window 128, sinks 2, forward and backward of one pass: 64 x 64 tiles 230 us, 32
+// rows a CTA 156, packed products 130, 32 x 32 tiles in two buffers 114 us (30 + 42 + 47 us and the join of 4).
 #include <cuda_runtime.h>
 
 #include "api.h"
