@@ -232,3 +232,57 @@ def test_without_gradients_and_for_some_inputs_only():
     o.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         o.backward(do)
+
+
+@pytest.mark.parametrize("fill", [float("nan"), float("inf"), -float("inf"), 3e38])
+@pytest.mark.parametrize("dtype,hd", [(BF, 64), (BF, 128), (F32, 64), (F32, 128), (BF, 40)])
+@pytest.mark.parametrize("T,window,first,last", [(300, 40, 50, 250), (1100, 130, 300, 900)])
+def test_what_a_row_does_not_see_may_be_anything(T, window, first, last, dtype, hd, fill):
+    """Positions before `first` and from `last` on hold NaN, infinities or numbers whose products overflow, in q, k, v and the
+    gradient.  Rows of o and dQ whose window holds none of them, and rows of dK and dV that no such query sees, are what the
+    positions between them give by themselves."""
+    q, k, v, do = _inputs(2, T, 4, 2, hd, dtype, seed=T)
+    for t in (q, k, v, do):
+        t[:, :first] = fill
+        t[:, last:] = fill
+    got = _run(q, k, v, do, window, 0, fused=False)
+    lo, hi = first + window, last - window
+    inner = [t[:, first:last] for t in (q, k, v, do)]
+    want = attention64(*inner, visible(last - first, window, 0))
+    for name, t, rows in zip(("o", "dq", "dk", "dv"), got, (slice(lo, last), slice(lo, last), slice(lo, hi), slice(lo, hi))):
+        value, bound = (x[:, rows.start - first:rows.stop - first] for x in want[name])
+        check(name, t[:, rows], (value, bound))
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF, 64), (BF, 128), (F32, 64)])
+def test_garbage_between_sinks_and_window(dtype, hd):
+    """Garbage in the middle of a sequence: later rows see the sinks before it and the window behind it, and the sinks' gradients
+    come from them alone where the queries beside the garbage have no gradient."""
+    T, window, sinks = 900, 70, 3
+    q, k, v, do = _inputs(1, T, 2, 1, hd, dtype, seed=2)
+    k[:, 200:400], v[:, 200:400] = float("nan"), float("inf")
+    got = _run(q, k, v, do, window, sinks, fused=True)
+    keep = list(range(sinks)) + list(range(400, T))
+    mask = visible(T, window, sinks)[470:][:, keep]
+    n = T - 470
+    want = attention64(q[:, 470:], k[:, keep], v[:, keep], do[:, 470:], mask)
+    check("o", got[0][:, 470:], want["o"])
+    check("dq", got[1][:, 470:], want["dq"])
+    # keys from 470 on are seen by rows from 470 on only
+    check("dk", got[2][:, 470:], tuple(x[:, -n:] for x in want["dk"]))
+    check("dv", got[3][:, 470:], tuple(x[:, -n:] for x in want["dv"]))
+    assert torch.isnan(got[0][:, 250]).all() and torch.isfinite(got[0][:, :200]).all()
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF, 64), (BF, 128), (F32, 64)])
+def test_a_visible_nan_shows(dtype, hd):
+    q, k, v, do = _inputs(1, 300, 2, 1, hd, dtype, seed=2)
+    k[:, 100] = float("nan")
+    o, dq, dk, dv = _run(q, k, v, do, 40, 0, fused=True)
+    assert torch.isnan(o[:, 100:140]).all() and torch.isfinite(o[:, :100]).all() and torch.isfinite(o[:, 140:]).all()
+    assert torch.isnan(dq[:, 100:140]).all() and torch.isfinite(dq[:, :100]).all() and torch.isfinite(dq[:, 140:]).all()
+    assert torch.isnan(dv[:, 61:140]).all() and torch.isfinite(dv[:, :61]).all() and torch.isfinite(dv[:, 140:]).all()
+    v[:, 100] = float("inf")
+    k[:, 100] = 0
+    o = ops.window_attention(q, k, v, 40)
+    assert torch.isinf(o[:, 100:140]).all() and torch.isfinite(o[:, :100]).all() and torch.isfinite(o[:, 140:]).all()

@@ -31,6 +31,7 @@
 
 #include "api.h"
 #include "ptx_sm100.cuh"
+#include "window_rows.cuh"
 
 namespace titb {
 
@@ -86,6 +87,32 @@ struct AttnArgs {
   float* sink_part;  // fp32 [sink_parts][B][sink_blocks][Hkv][dK, dV][kBlk][hd]
 };
 
+// A row of o that is not finite, over visible pairs only.  The call is the kernel's last act and takes its operands from a
+// parameter of their own; that it is there costs 1.1 us of 24 (32 heads of 64, T 1999, window 512), looking for such rows 0.2 of it;
+// from the epilogue, with 32 elements at once (spills at hd 64), 1.3.
+template <int HD>
+__device__ __noinline__ void o_row_again(const WinRows& rows, int b, int h, int i, bf16* o, bf16* o_lo) {
+  const float lse = rows.lse[rows.stat(b, h, i)];
+#pragma unroll 1
+  for (int c = 0; c < HD; c += 16) window_o_again<bf16, 16>(rows, b, h, i, lse, c, o + c, o_lo ? o_lo + c : nullptr);
+}
+
+// Pieces of row j of dK and dV that are not finite, over visible pairs only, from queries [i0, i1).  `sum` is where a part of a
+// sink goes (dK, dV after it), or null.
+template <int HD>
+__device__ __noinline__ void dkv_pieces_again(const WinRows& rows, int b, int hk, int j, int i0, int i1, uint32_t pieces, float* sum,
+                                              bf16* dk, bf16* dv) {
+  for (; pieces; pieces &= pieces - 1) {
+    const int piece = __ffs(pieces) - 1, d0 = piece % (HD / 32) * 32;
+    const bool value = piece < HD / 32;
+#pragma unroll 1
+    for (int d = d0; d < d0 + 32; d += 16) {
+      if (sum) window_dkv_again<bf16, float, 16>(rows, b, hk, j, i0, i1, value, d, sum + (value ? kBlk * HD : 0) + d);
+      else window_dkv_again<bf16, bf16, 16>(rows, b, hk, j, i0, i1, value, d, (value ? dv : dk) + d);
+    }
+  }
+}
+
 // Bits [lo, hi) of a 32-bit word; lo and hi may lie outside it.
 __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
   lo = max(lo, 0);
@@ -138,14 +165,14 @@ struct FwdCfg {
 // lies over S and S(j+1) is issued behind P(j) V(j), which costs nothing beside two other CTAs (columns of its own, in a
 // second allocation, were as fast).
 // Measured (B200): hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: one CTA an SM 254 us, two with 128 keys a step, P over S
-// and S(j+1) issued behind P(j) V(j) 182 us, as it is 165 us (790 TFLOP/s of what the rows see; 178 us where a backward pass follows); hd 64, 1 x 1999, 32 / 8 heads,
-// window 512: 29 us before, 26 us.  A step of 64 keys takes 1660 cycles (hd 128) and 2140 (hd 64, three CTAs), 920 and 1060 of
-// them for the exponentials; a quarter of those on the multiply-add pipe changed nothing.  Set-up, first loads and output
-// take another 8000 and 5500 cycles of a CTA.
+// and S(j+1) issued behind P(j) V(j) 182 us, as it is 165 us (790 TFLOP/s of what the rows see; 180 us where a backward pass
+// follows); hd 64, 1 x 1999, 32 / 8 heads, window 512: 29 us before, 26 us (28 with the call of o_row_again).  A step of 64 keys
+// takes 1660 cycles (hd 128) and 2140 (hd 64, three CTAs), 920 and 1060 of them for the exponentials; a quarter of those on the
+// multiply-add pipe changed nothing.  Set-up, first loads and output take another 8000 and 5500 cycles of a CTA.
 template <int HD, bool WIN>
 __global__ void __launch_bounds__(kAttnThreads, FwdCfg<HD, WIN>::kCtas)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                const __grid_constant__ CUtensorMap tv, const AttnArgs p) {
+                const __grid_constant__ CUtensorMap tv, const AttnArgs p, const __grid_constant__ WinRows rows) {
   using Cfg = FwdCfg<HD, WIN>;
   constexpr int S = Cfg::kStages;
   constexpr int KB = Cfg::kKeys;
@@ -209,6 +236,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   const uint32_t tS = tmem_base, tO = tmem_base + Cfg::kColO;
   const uint32_t tP = Cfg::kAlias ? tS : tmem_base + 64;   // WIN
   const bool bad_align = (*abort_flag != 0);
+  int again_row = -1;   // WIN: this thread's row, if it is not finite
 
   if (bad_align) {
     // fall through to the common exit
@@ -463,6 +491,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       uint8_t* q_smem = smem + Cfg::kQ;
       uint8_t* lo_smem = smem + Cfg::kK;
       static_assert(!WIN || Cfg::kStages * Cfg::kTileBytes >= Cfg::kQBytes, "room for a tile of rows");
+      uint32_t probe = 0;
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t r[32];
@@ -477,6 +506,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
             u.z = pack_bf16x2(__uint_as_float(r[d + 4]) * inv, __uint_as_float(r[d + 5]) * inv);
             u.w = pack_bf16x2(__uint_as_float(r[d + 6]) * inv, __uint_as_float(r[d + 7]) * inv);
             *reinterpret_cast<uint4*>(q_smem + swz_off(row, c * 4 + d / 8)) = u;
+            probe_finite(probe, u.x); probe_finite(probe, u.y); probe_finite(probe, u.z); probe_finite(probe, u.w);
             if (p.o_lo) {
               uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -500,16 +530,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       }
       if constexpr (WIN) {
         // a warp's rows leave as whole rows: a store of one unit per row and lane would take a transaction for each
-        __syncwarp();
+        const bool again = q_idx < p.T && probe != 0;   // not finite
+        const uint32_t skip = __ballot_sync(0xffffffffu, again);
 #pragma unroll 4
         for (int i = lane; i < 32 * (HD / 8); i += 32) {
           const int r = quad * 32 + i / (HD / 8), u = i % (HD / 8);
-          if (q0 + r < p.T) {
+          if (q0 + r < p.T && !(skip >> (r & 31) & 1u)) {
             const long long at = (static_cast<long long>(b) * p.T + q0 + r) * p.o_stride_t + h * HD + u * 8;
             *reinterpret_cast<uint4*>(p.o + at) = *reinterpret_cast<const uint4*>(q_smem + swz_off(r, u));
             if (p.o_lo) *reinterpret_cast<uint4*>(p.o_lo + at) = *reinterpret_cast<const uint4*>(lo_smem + swz_off(r, u));
           }
         }
+        if (again) again_row = q_idx;
       }
       if (q_idx < p.T)
         p.lse[(static_cast<long long>(b) * p.Hq + h) * p.T + q_idx] = (m_ref + log2f(l)) * 0.6931471805599453f;
@@ -523,6 +555,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
     ptx::tmem_dealloc(tmem_base, Cfg::kTmemCols);
   }
   if (threadIdx.x == 0 && *abort_flag) atomicExch(p.status, kStatusMbarTimeout);
+  if (WIN && again_row >= 0) {
+    const long long at = (static_cast<long long>(b) * p.T + again_row) * p.o_stride_t + h * HD;
+    o_row_again<HD>(rows, b, h, again_row, p.o + at, p.o_lo ? p.o_lo + at : nullptr);
+  }
 }
 
 // ------------------------------------------------------------------------ backward
@@ -572,13 +608,13 @@ struct BwdCfg {
 // WIN: a window and sinks.  A block of keys meets the query blocks up to its last key's window.  A block that holds sinks meets
 // all later ones, which would make its CTA the last by far: its query blocks are split over sink_parts CTAs, which leave
 // fp32 sums of the sinks' rows that attn_window_finish_kernel adds in order.
-// Measured: hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: 396 us, 1070 TFLOP/s of the tiles it visits, an eighth of them
-// masked and a tenth for the sinks; the same parts as above bound it.
+// Measured: hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: 401 us (396 without the look for what is not finite),
+// 1070 TFLOP/s of the tiles it visits, an eighth of them masked and a tenth for the sinks; the same parts as above bound it.
 template <int HD, bool WIN>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                 const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
-                const __grid_constant__ CUtensorMap tdq, const AttnArgs p) {
+                const __grid_constant__ CUtensorMap tdq, const AttnArgs p, const __grid_constant__ WinRows rows) {
   using Cfg = BwdCfg<HD>;
   constexpr int DS = Cfg::kDoStages;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -652,6 +688,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   dependency_wait();
   dependents_launch();
   const bool bad_align = (*abort_flag != 0);
+  uint32_t again = 0;   // WIN: pieces of 32 elements of this thread's row that are not finite, a bit each
 
   if (bad_align) {
     // fall through to the common exit
@@ -958,6 +995,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           uint32_t r[32];
           ptx::tmem_ld32(tmem_base + col + lane_sel + c * 32, r);
           ptx::tmem_ld_wait();
+          if (WIN) {
+            float probe = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) probe_finite(probe, __uint_as_float(r[e]));
+            if (probe != 0.f) again |= 1u << (which * (HD / 32) + c);
+          }
           if (sink_cta && p.sink_parts > 1 && kv_idx < p.sinks) {
             float* sum = p.sink_part + ((((static_cast<long long>(part) * p.B + b) * p.sink_blocks + jb) * p.Hkv + hk) * 2 + 1 - which) * (kBlk * HD) +
                          row * HD + c * 32;
@@ -987,6 +1030,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
     ptx::tmem_dealloc(tmem_base, Cfg::kTmemCols);
   }
   if (threadIdx.x == 0 && *abort_flag) atomicExch(p.status, kStatusMbarTimeout);
+  const int again_j = jb * kBlk + warp % 4 * 32 + lane;
+  const bool again_part = sink_cta && p.sink_parts > 1 && again_j < p.sinks;
+  if (WIN && again && again_j < p.T && (again_part || part == 0)) {
+    const long long bt = static_cast<long long>(b) * p.T + again_j;
+    float* sum = p.sink_part + (((static_cast<long long>(part) * p.B + b) * p.sink_blocks + jb) * p.Hkv + hk) * 2 * (kBlk * HD) +
+                 (again_j - jb * kBlk) * HD;
+    dkv_pieces_again<HD>(rows, b, hk, again_j, ib * kBlk, (ib + nq) * kBlk, again, again_part ? sum : nullptr,
+                         p.dk + bt * p.dk_stride_t + hk * HD, p.dv + bt * p.dv_stride_t + hk * HD);
+  }
 }
 
 // delta[b,h,t] = sum_d dO[b,t,h,d] * O[b,t,h,d] (WIN: with what O's rounding left), and the fp32 dQ accumulator starts at zero.  hd / 8 neighbouring lanes
@@ -1046,15 +1098,33 @@ __global__ void attn_dq_convert_kernel(const float* __restrict__ acc, bf16* __re
   }
 }
 
+// What of a thread's dq (below) is not finite, over visible pairs only.  It starts over, since a call within the loop below took
+// registers from it.
+template <int HD>
+__device__ __noinline__ void dq_again(const WinRows& rows, const float* acc, long long n_sink, long long n, bf16* dq, long long dq_stride_t) {
+  const int wv = rows.Hq * HD / 8;
+  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+    if (i < n_sink) continue;
+    const long long bt = (i - n_sink) / wv;
+    const int c = static_cast<int>(i - n_sink - bt * wv) * 8;
+    float probe = 0.f;
+    for (int e = 0; e < 8; ++e) probe_finite(probe, acc[bt * wv * 8 + c + e]);
+    if (probe != 0.f)
+      window_dq_again<bf16, 8>(rows, static_cast<int>(bt / rows.T), c / HD, static_cast<int>(bt % rows.T), c % HD, dq + bt * dq_stride_t + c);
+  }
+}
+
 // The end of the backward pass of window attention: dq from its accumulator, and dK and dV of the sinks, whose parts are
 // added in order.
 template <int HD>
-__global__ void attn_window_finish_kernel(const AttnArgs p, bf16* __restrict__ dq, long long dq_stride_t) {
+__global__ void __launch_bounds__(256, 6) attn_window_finish_kernel(const AttnArgs p, const __grid_constant__ WinRows rows, bf16* __restrict__ dq,
+                                                                 long long dq_stride_t) {
   dependents_launch();
   const int width = p.Hq * HD, wv = width / 8, nqb = (p.T + kBlk - 1) / kBlk;
   const long long n_dq = static_cast<long long>(p.B) * p.T * wv;
   const long long n_sink = p.sink_parts > 1 ? static_cast<long long>(p.B) * p.sinks * p.Hkv * 2 * (HD / 4) : 0;
   const long long part_size = static_cast<long long>(p.B) * p.sink_blocks * p.Hkv * 2 * kBlk * HD;
+  float probe = 0.f;
   for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n_sink + n_dq; i += (long long)gridDim.x * blockDim.x) {
     if (i < n_sink) {
       const int d = static_cast<int>(i % (HD / 4)) * 4;
@@ -1083,7 +1153,10 @@ __global__ void attn_window_finish_kernel(const AttnArgs p, bf16* __restrict__ d
     u.x = pack_bf16x2(f0.x, f0.y); u.y = pack_bf16x2(f0.z, f0.w);
     u.z = pack_bf16x2(f1.x, f1.y); u.w = pack_bf16x2(f1.z, f1.w);
     *reinterpret_cast<uint4*>(dq + bt * dq_stride_t + c) = u;
+    probe_finite(probe, f0.x); probe_finite(probe, f0.y); probe_finite(probe, f0.z); probe_finite(probe, f0.w);
+    probe_finite(probe, f1.x); probe_finite(probe, f1.y); probe_finite(probe, f1.z); probe_finite(probe, f1.w);
   }
+  if (probe != 0.f) dq_again<HD>(rows, p.dq_accum, n_sink, n_sink + n_dq, dq, dq_stride_t);
 }
 
 static bool attn_check(const TitbAttnDesc* d) {
@@ -1121,7 +1194,7 @@ static int attn_fwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 
   a.o = static_cast<bf16*>(d->o); a.lse = d->lse; a.o_stride_t = d->o_stride_t;
   a.status = titb_status_ptr();
   dim3 grid(static_cast<unsigned>(d->Hq) * d->B, (d->T + kBlk - 1) / kBlk);
-  launch_dependent(attn_fwd_kernel<HD, WIN>, grid, kAttnThreads, Cfg::kSmem, st, tq, tk, tv, a);
+  launch_dependent(attn_fwd_kernel<HD, WIN>, grid, kAttnThreads, Cfg::kSmem, st, tq, tk, tv, a, window_rows(*d, window, sinks));
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -1177,17 +1250,17 @@ static int attn_bwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 
   if (WIN) {
     const SinkSplit split = sink_split(*d, window, sinks);
     a.window = window; a.sinks = sinks;
-    a.sink_blocks = split.blocks; a.sink_step = split.step; a.sink_parts = split.parts; a.sink_part = sink_part;
+      a.sink_blocks = split.blocks; a.sink_step = split.step; a.sink_parts = split.parts; a.sink_part = sink_part;
     jobs += split.blocks * (split.parts - 1);
   }
   dim3 grid(static_cast<unsigned>(d->Hkv) * d->B, jobs);
-  launch_dependent(attn_bwd_kernel<HD, WIN>, grid, kBwdThreads, Cfg::kSmem, st, tq, tk, tv, tdo, tdq, a);
+  launch_dependent(attn_bwd_kernel<HD, WIN>, grid, kBwdThreads, Cfg::kSmem, st, tq, tk, tv, tdo, tdq, a, window_rows(*d, window, sinks));
   const long long bt = static_cast<long long>(d->B) * d->T;
   const int width = d->Hq * HD;
   int cb = static_cast<int>((bt * (width / 8) + 255) / 256);
   if (cb > device_sm_count() * 8) cb = device_sm_count() * 8;
   if (WIN) {
-    attn_window_finish_kernel<HD><<<cb, 256, 0, st>>>(a, static_cast<bf16*>(d->dq), d->dq_stride_t);
+    attn_window_finish_kernel<HD><<<cb, 256, 0, st>>>(a, window_rows(*d, window, sinks), static_cast<bf16*>(d->dq), d->dq_stride_t);
     return static_cast<int>(cudaGetLastError());
   }
   attn_dq_convert_kernel<<<cb, 256, 0, st>>>(d->dq_accum, static_cast<bf16*>(d->dq), bt, width, d->dq_stride_t);

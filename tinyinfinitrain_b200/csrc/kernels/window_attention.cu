@@ -13,11 +13,13 @@
 // Bound by the reads of shared memory: two 16-byte reads feed eight packed multiply-adds (70 % of what the SM can read; a layout
 // with half as many distinct words a read changed nothing), and by tiles that are half masked where the window is short.
 // Measured (B200), 2 x 512 tokens, 12 heads of 64, window 128, sinks 2, forward and backward of one pass: 64 x 64 tiles 230 us, 32
-// rows a CTA 156, packed products 130, 32 x 32 tiles in two buffers 114 us (30 + 42 + 47 us and the join of 4).
+// rows a CTA 156, packed products 130, 32 x 32 tiles in two buffers 114 us, with the look for what is not
+// finite 117 (32 + 43 + 47 us and the join of 4).
 #include <cuda_runtime.h>
 
 #include "api.h"
 #include "common.cuh"
+#include "window_rows.cuh"
 
 namespace titb {
 
@@ -190,6 +192,14 @@ __device__ __forceinline__ void store_rows(T* base, long long stride, int t0, in
 }
 
 template <int HD>
+__device__ __forceinline__ bool piece_finite(const float (&acc)[HD / 64][4][4], int c, int r) {
+  float probe = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) probe_finite(probe, acc[c][e][r]);
+  return probe == 0.f;
+}
+
+template <int HD>
 struct WinFwdSmem {
   static constexpr int kTile = kWinStep * (HD + 4);   // K and V in two buffers each
   static constexpr int kQ = 0, kK = kQ + kWinRows * (HD + 4), kV = kK + 2 * kTile, kP = kV + 2 * kTile;
@@ -198,7 +208,7 @@ struct WinFwdSmem {
 
 // One CTA per 32 queries of a head.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p) {
+__global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p, const __grid_constant__ WinRows rows) {
   using Sm = WinFwdSmem<HD>;
   extern __shared__ __align__(16) float sm[];
   float *Qs = sm + Sm::kQ, *Ks = sm + Sm::kK, *Vs = sm + Sm::kV, *Ps = sm + Sm::kP;
@@ -278,6 +288,17 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
       for (int r = 0; r < 4; ++r) acc[e / 4][e % 4][r] -= to_f32(from_f32<T>(acc[e / 4][e % 4][r]));
     store_rows<bf16, HD>(p.o_lo + row0 * p.o_st + h * p.hd, p.o_st, q0, p.T, p.hd, acc, ty, tx);
   }
+#pragma unroll
+  for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = q0 + ty * 4 + r, d = c * 64 + tx * 4;
+      if (i < p.T && d < p.hd && !piece_finite<HD>(acc, c, r)) {
+        const long long at = (row0 + i) * p.o_st + h * p.hd + d;
+        window_o_again<T, 4>(rows, b, h, i, m[r] + logf(l[r]), d, static_cast<T*>(p.o) + at,
+                             sizeof(T) == 2 && p.o_lo ? p.o_lo + at : nullptr);
+      }
+    }
 }
 
 template <int HD>
@@ -289,7 +310,7 @@ struct WinDqSmem {
 
 // One CTA per 32 queries of a head: delta, then dQ.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p) {
+__global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p, const __grid_constant__ WinRows rows) {
   using Sm = WinDqSmem<HD>;
   extern __shared__ __align__(16) float sm[];
   float *Qs = sm + Sm::kQ, *Ds = sm + Sm::kDO, *Ks = sm + Sm::kK, *Vs = sm + Sm::kV, *Ss = sm + Sm::kDS;
@@ -358,6 +379,15 @@ __global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p)
     __syncthreads();
   }
   store_rows<T, HD>(static_cast<T*>(p.dq) + row0 * p.dq_st + h * p.hd, p.dq_st, q0, p.T, p.hd, acc, ty, tx);
+  __syncthreads();   // delta is read again
+#pragma unroll
+  for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = q0 + ty * 4 + r, d = c * 64 + tx * 4;
+      if (i < p.T && d < p.hd && !piece_finite<HD>(acc, c, r))
+        window_dq_again<T, 4>(rows, b, h, i, d, static_cast<T*>(p.dq) + (row0 + i) * p.dq_st + h * p.hd + d);
+    }
 }
 
 template <int HD>
@@ -371,7 +401,7 @@ struct WinDkvSmem {
 // One CTA per 32 keys of a kv head, over the query heads that share it; reads the delta that window_dq_kernel wrote.  The
 // query steps of a tile that holds sinks reach to the end of the sequence and are split over sink_parts CTAs.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p) {
+__global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p, const __grid_constant__ WinRows rows) {
   using Sm = WinDkvSmem<HD>;
   extern __shared__ __align__(16) float sm[];
   float *Ks = sm + Sm::kK, *Vs = sm + Sm::kV, *Qs = sm + Sm::kQ, *Ds = sm + Sm::kDO, *Ps = sm + Sm::kP, *Ss = sm + Sm::kDS, *stat = sm + Sm::kStat;
@@ -438,10 +468,32 @@ __global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p
     store_rows<T, HD>(static_cast<T*>(p.dk) + row0 * p.dk_st + hk * p.hd, p.dk_st, k0, p.T, p.hd, dk, ty, tx);
     store_rows<T, HD>(static_cast<T*>(p.dv) + row0 * p.dv_st + hk * p.hd, p.dv_st, k0, p.T, p.hd, dv, ty, tx);
   }
+  const int i0 = first * kWinStep, i1 = (first + n_steps) * kWinStep;
+#pragma unroll
+  for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int j = k0 + ty * 4 + r, d = c * 64 + tx * 4;
+      if (part != 0 || j >= p.T || d >= p.hd) continue;
+      if (!piece_finite<HD>(dk, c, r))
+        window_dkv_again<T, T, 4>(rows, b, hk, j, i0, i1, false, d, static_cast<T*>(p.dk) + (row0 + j) * p.dk_st + hk * p.hd + d);
+      if (!piece_finite<HD>(dv, c, r))
+        window_dkv_again<T, T, 4>(rows, b, hk, j, i0, i1, true, d, static_cast<T*>(p.dv) + (row0 + j) * p.dv_st + hk * p.hd + d);
+    }
   if (sink_cta && p.sink_parts > 1) {
     float* sum = p.sink_part + (((static_cast<long long>(part) * p.B + b) * p.sink_tiles + tile) * p.Hkv + hk) * 2 * kWinRows * p.hd;
     store_rows<float, HD>(sum, p.hd, 0, p.sinks - k0, p.hd, dk, ty, tx);
     store_rows<float, HD>(sum + kWinRows * p.hd, p.hd, 0, p.sinks - k0, p.hd, dv, ty, tx);
+#pragma unroll
+    for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = k0 + ty * 4 + r, d = c * 64 + tx * 4;
+        if (j >= p.sinks || d >= p.hd) continue;
+        float* at = sum + (j - k0) * p.hd + d;
+        if (!piece_finite<HD>(dk, c, r)) window_dkv_again<T, float, 4>(rows, b, hk, j, i0, i1, false, d, at);
+        if (!piece_finite<HD>(dv, c, r)) window_dkv_again<T, float, 4>(rows, b, hk, j, i0, i1, true, d, at + kWinRows * p.hd);
+      }
   }
 }
 
@@ -501,28 +553,30 @@ static WinArgs win_args(const TitbWindowDesc* w) {
 }
 
 template <typename K>
-static cudaError_t win_launch(K kernel, const WinArgs& a, int heads, int jobs, int smem, cudaStream_t st) {
+static cudaError_t win_launch(K kernel, const WinArgs& a, const WinRows& rows, int heads, int jobs, int smem, cudaStream_t st) {
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<dim3(static_cast<unsigned>(heads) * a.B, jobs), kWinThreads, smem, st>>>(a);
+  kernel<<<dim3(static_cast<unsigned>(heads) * a.B, jobs), kWinThreads, smem, st>>>(a, rows);
   return cudaGetLastError();
 }
 
 template <typename T, int HD>
 static int win_fwd(const TitbWindowDesc* w, cudaStream_t st) {
   const WinArgs a = win_args(w);
-  return static_cast<int>(win_launch(window_fwd_kernel<T, HD>, a, a.Hq, (a.T + kWinRows - 1) / kWinRows, WinFwdSmem<HD>::kBytes, st));
+  return static_cast<int>(win_launch(window_fwd_kernel<T, HD>, a, window_rows(w->attn, a.window, a.sinks), a.Hq,
+                                     (a.T + kWinRows - 1) / kWinRows, WinFwdSmem<HD>::kBytes, st));
 }
 template <typename T, int HD>
 static int win_bwd(const TitbWindowDesc* w, cudaStream_t st) {
   WinArgs a = win_args(w);
+  const WinRows rows = window_rows(w->attn, a.window, a.sinks);
   const WinSplit split = win_split(w->attn, a.window, a.sinks);
   a.sink_tiles = split.tiles; a.sink_step = split.step; a.sink_parts = split.parts;
   a.sink_part = w->workspace;
   const int tiles = (a.T + kWinRows - 1) / kWinRows;
-  cudaError_t e = win_launch(window_dq_kernel<T, HD>, a, a.Hq, tiles, WinDqSmem<HD>::kBytes, st);
+  cudaError_t e = win_launch(window_dq_kernel<T, HD>, a, rows, a.Hq, tiles, WinDqSmem<HD>::kBytes, st);
   if (e != cudaSuccess) return static_cast<int>(e);
-  e = win_launch(window_dkv_kernel<T, HD>, a, a.Hkv, tiles + split.tiles * (split.parts - 1), WinDkvSmem<HD>::kBytes, st);
+  e = win_launch(window_dkv_kernel<T, HD>, a, rows, a.Hkv, tiles + split.tiles * (split.parts - 1), WinDkvSmem<HD>::kBytes, st);
   if (e != cudaSuccess || split.tiles == 0 || split.parts == 1) return static_cast<int>(e);
   const long long n = win_part_floats(w->attn, split) / split.parts, most = device_sm_count() * 8LL;
   window_join_kernel<T><<<static_cast<int>((n + 255) / 256 < most ? (n + 255) / 256 : most), 256, 0, st>>>(a);

@@ -749,8 +749,7 @@ def window_attention(q, k, v, window: Optional[int], sinks: int = 0, scale: Opti
     ``j < sinks``), i.e. the last ``window`` positions, its own among them, and the first ``sinks`` of the sequence.
 
     Shapes and layouts as in :func:`causal_attention`; ``window=None`` is no bound.  float32 or bfloat16; on the GPU a head
-    size that is a multiple of 8 up to 128.  q, k and v have to be finite: inside a tile of 128 positions a key's or value's
-    NaN or infinity reaches queries that do not see it."""
+    size that is a multiple of 8 up to 128, and there NaN and infinities reach only the rows that see them."""
     hd = q.shape[-1]
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
     if not q.is_cuda:
