@@ -53,6 +53,14 @@ def test_an_idle_sequence_stays_as_it_is():
     assert cache.lengths.tolist() == [6, 3] and torch.equal(held, cache.k[:, cache.page_table[1].long()])
 
 
+def test_counts_outside_the_tokens_at_hand():
+    for model in _models(0, 0):
+        idx = torch.randint(0, 97, (2, 5))
+        caches = [model.new_cache(2, page_size=4) for _ in range(2)]
+        a, b = (model(idx, cache=c, counts=torch.tensor(n, dtype=torch.int32)) for c, n in zip(caches, ([9, -4], [5, 0])))
+        assert torch.equal(a, b) and caches[0].lengths.tolist() == [5, 0]
+
+
 def test_training_with_a_window_differs_and_runs():
     torch.manual_seed(1)
     idx = torch.randint(0, 97, (2, 20))

@@ -62,7 +62,8 @@ class PagedKVCache:
 
     def begin(self, idx: torch.Tensor, counts: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Called by a model before its layers: the positions of the new tokens idx [batch, T], int64 [batch, T].  ``counts``
-        (int32 [batch]): how many of the T tokens of a sequence are real, the others being padding behind them."""
+        (int32 [batch]): how many of the T tokens of a sequence are real, the others being padding behind them; a count outside
+        0 .. T is taken as the nearer of the two."""
         B, T = idx.shape
         if B != self.batch:
             raise ValueError(f"PagedKVCache: a batch of {B} for a cache of {self.batch} sequences")
@@ -72,6 +73,8 @@ class PagedKVCache:
             raise ValueError("PagedKVCache: several tokens at once go into an empty cache only; reset() it, or feed them one by one")
         if counts is not None and (counts.dtype != torch.int32 or counts.shape != (B,) or counts.device != self.lengths.device):
             raise ValueError(f"PagedKVCache: counts must be an int32 tensor of {B} elements on {self.lengths.device}")
+        if counts is not None:
+            counts = counts.clamp(0, T)     # a larger one would count rows that no token was written to
         self._starts, self._counts = self.lengths, counts
         self._ends = self.lengths + (T if counts is None else counts)
         return self.lengths[:, None].long() + torch.arange(T, device=idx.device)
