@@ -386,6 +386,25 @@ def test_captured_and_replayed_with_other_lengths(dtype, hd):
             check("o", o, _expect(q, [(k[:m], v[:m]) for (k, v), m in zip(rows, now)], now, None, 0))
 
 
+def test_a_write_counts_as_one():
+    """Autograd refuses a cache that it has kept and that tokens were appended to; in inference mode there is nothing to count."""
+    kc, vc = (torch.zeros(2, 2, 16, 64, device=DEV) for _ in range(2))
+    table, lengths = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([[0, 1]], [3]))
+    w = torch.ones(64, device=DEV, requires_grad=True)
+    y = (kc * w).sum()
+    ops.cache_append(torch.zeros(1, 1, 8 * 64, device=DEV), kc, vc, table, lengths, 4, 2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        qkv = torch.randn(1, 1, 8 * 64, device=DEV)
+        a, b = torch.zeros_like(kc), torch.zeros_like(vc)
+        out = ops.cache_append(qkv, a, b, table, lengths, 4, 2, theta=1e4)
+        got = ops.paged_attention(out[:, 0], a, b, table, lengths + 1, window=1)
+        assert torch.equal(got[0], qkv[0, 0, 6 * 64:].view(2, 64).repeat_interleave(2, 0))
+        q = torch.randn(1, 5, 2, 64, device=DEV)
+        assert torch.equal(ops.window_attention(q, q, q, 1), q)
+
+
 def test_results_do_not_change_from_run_to_run():
     kc, vc, table, _ = _cache([5000, 100, 7, 900], 2, 128, 64, BF, fill=0.0)
     q = torch.randn(4, 8, 128, device=DEV).to(BF)

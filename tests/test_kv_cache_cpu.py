@@ -129,6 +129,14 @@ def test_refusals():
                      ((qkv, kc.double(), vc.double(), table, n, 4, 2), {})):
         with pytest.raises(RuntimeError, match="titb200 cache_append"):
             ops.cache_append(*args, **kw)
+    with pytest.raises(RuntimeError, match="share memory"):
+        ops.cache_append(qkv, kc, kc, table, n, 4, 2)
+    both = torch.zeros(3 * kc.shape[0], *kc.shape[1:])
+    with pytest.raises(RuntimeError, match="share memory"):
+        ops.cache_append(qkv, both[:kc.shape[0]], both[1:1 + kc.shape[0]], table, n, 4, 2)
+    for scale in (1e-60, 1e60):     # zero and infinity in 32 bits
+        with pytest.raises(RuntimeError, match="scale"):
+            ops.paged_attention(q, kc, vc, table, n, scale=scale)
     with pytest.raises(RuntimeError, match="no gradient"):
         ops.paged_attention(q.requires_grad_(), kc, vc, table, n)
     with pytest.raises(RuntimeError, match="no gradient"):

@@ -68,7 +68,7 @@ def test_refusals():
                  (q, k[:, :, :1], v, 4, 0), (q[:, :, :3], k, v, 4, 0), (q[0], k[0], v[0], 4, 0)):
         with pytest.raises(RuntimeError, match="titb200 window_attention"):
             ops.window_attention(*args)
-    for scale in (0.0, -1.0, float("inf"), float("nan")):
+    for scale in (0.0, -1.0, float("inf"), float("nan"), 1e-60, 1e60):
         with pytest.raises(RuntimeError, match="scale"):
             ops.window_attention(q, k, v, 4, scale=scale)
     with pytest.raises(RuntimeError, match="does not hold"):

@@ -74,7 +74,8 @@ std::vector<Tensor> attn_bwd(const Tensor& d_o_, const Tensor& q_, const Tensor&
 
 // ---- window and sinks
 void limits_check(const Tensor& t, int64_t B, int64_t T, int64_t Hq, int64_t hd, int64_t window, int64_t sinks, double scale) {
-  TORCH_CHECK(scale > 0.0 && std::isfinite(scale), "titb200 window_attention: scale must be positive, got ", scale);
+  const float scale32 = static_cast<float>(scale);   // what the kernels take
+  TORCH_CHECK(scale32 > 0.f && std::isfinite(scale32), "titb200 window_attention: scale must be positive, got ", scale);
   TORCH_CHECK(window >= 1, "titb200 window_attention: window must be at least 1, got ", window);
   TORCH_CHECK(sinks >= 0, "titb200 window_attention: sinks must not be negative, got ", sinks);
   if (!t.is_cuda()) return;

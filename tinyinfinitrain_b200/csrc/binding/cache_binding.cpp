@@ -72,6 +72,9 @@ void append_check(const Tensor& qkv, const Tensor& k_cache, const Tensor& v_cach
               "titb200 cache_append: a projection of width ", qkv.size(2), " does not hold ", n_head, " + 2 * ", n_kv_head,
               " heads of the cache's size");
   cache_check("cache_append", qkv, k_cache, v_cache, table, starts, qkv.size(0), n_head, n_kv_head, k_cache.size(3), window, sinks);
+  const char *ck = static_cast<const char*>(k_cache.data_ptr()), *cv = static_cast<const char*>(v_cache.data_ptr());
+  const int64_t held = k_cache.numel() * k_cache.element_size();
+  TORCH_CHECK(held == 0 || ck + held <= cv || cv + held <= ck, "titb200 cache_append: k_cache and v_cache share memory");
   if (counts.has_value())
     TORCH_CHECK(counts->dim() == 1 && counts->size(0) == qkv.size(0) && counts->scalar_type() == at::kInt && counts->is_contiguous() &&
                     counts->device() == qkv.device(),
@@ -102,6 +105,8 @@ py::object cache_append(const Tensor& qkv_, Tensor& k_cache, Tensor& v_cache, co
                           counts.has_value() ? counts->data_ptr<int>() : nullptr, theta, q.defined() ? q.data_ptr() : nullptr,
                           k.defined() ? k.data_ptr() : nullptr, at::cuda::getCurrentCUDAStream().stream()),
         "cache_append");
+  for (const Tensor* c : {&k_cache, &v_cache})   // so that autograd sees the write where it has kept the cache
+    if (!c->is_inference()) c->unsafeGetTensorImpl()->bump_version();
   if (theta == 0.0) {
     const auto view = [&](int64_t first, int64_t heads) {
       return qkv_.as_strided({B, T, heads, hd}, {qkv_.stride(0), qkv_.stride(1), hd * qkv_.stride(2), qkv_.stride(2)},
@@ -116,7 +121,8 @@ py::object cache_append(const Tensor& qkv_, Tensor& k_cache, Tensor& v_cache, co
 
 void paged_check(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& lengths,
                  int64_t window, int64_t sinks, double scale) {
-  TORCH_CHECK(scale > 0.0 && std::isfinite(scale), "titb200 paged_attention: scale must be positive, got ", scale);
+  const float scale32 = static_cast<float>(scale);   // what the kernels take
+  TORCH_CHECK(scale32 > 0.f && std::isfinite(scale32), "titb200 paged_attention: scale must be positive, got ", scale);
   forward_only("paged_attention", {&q, &k_cache, &v_cache});
   TORCH_CHECK(q.dim() == 3 && k_cache.dim() == 4, "titb200 paged_attention: q [B, Hq, hd], caches [pages, Hkv, page_size, hd]");
   cache_check("paged_attention", q, k_cache, v_cache, table, lengths, q.size(0), q.size(1), k_cache.size(1), q.size(2), window,
