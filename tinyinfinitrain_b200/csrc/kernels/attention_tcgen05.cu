@@ -135,7 +135,8 @@ struct FwdCfg {
   static constexpr int kP = kV + kStages * kTileBytes;
   static constexpr int kBar = kP + (WIN ? 0 : kBlk * kBlk * 2);   // WIN: P lies in tensor memory
   static constexpr int kSmem = kBar + 128;
-  // S: [0, kKeys)  O: [kColO, kColO + HD); WIN: P takes 32 columns, over S (kAlias) or at 64
+  // S: [0, kKeys)  O: [kColO, kColO + HD); WIN: P takes 32 columns and what its rounding left 32 more, over S (kAlias) or
+  // from 64 on
   static constexpr bool kAlias = WIN && HD == 64;
   static constexpr int kColO = HD == 128 ? 128 : kKeys;
   static constexpr int kTmemCols = kAlias ? 128 : 256;
@@ -163,13 +164,16 @@ struct FwdCfg {
 // set-up and its chain of dependent steps (S, maximum, exponentials, P, P V), so kCtas CTAs share the SM, with 64 keys a step
 // and P in tensor memory, as the A operand of P V: 48 or 96 KB of shared memory and 128 or 256 columns to a CTA.  At hd 64 P
 // lies over S and S(j+1) is issued behind P(j) V(j), which costs nothing beside two other CTAs (columns of its own, in a
-// second allocation, were as fast).
+// second allocation, were as fast).  What P's rounding to bf16 left is the A operand of a second product onto the same O:
+// without it the output was off by 0.20 % (0.165 % being its own rounding) and dQ, through delta, by 0.25 % (now 0.235, 0.233
+// being the roundings of dS and of dQ).  LO: a backward pass may follow, and what the rounding of o left is kept for its delta.
 // Measured (B200): hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: one CTA an SM 254 us, two with 128 keys a step, P over S
-// and S(j+1) issued behind P(j) V(j) 182 us, as it is 165 us (790 TFLOP/s of what the rows see; 180 us where a backward pass
-// follows); hd 64, 1 x 1999, 32 / 8 heads, window 512: 29 us before, 26 us (28 with the call of o_row_again).  A step of 64 keys
-// takes 1660 cycles (hd 128) and 2140 (hd 64, three CTAs), 920 and 1060 of them for the exponentials; a quarter of those on the
-// multiply-add pipe changed nothing.  Set-up, first loads and output take another 8000 and 5500 cycles of a CTA.
-template <int HD, bool WIN>
+// and S(j+1) issued behind P(j) V(j) 182 us, with the steps as they are 165 us (790 TFLOP/s of what the rows see), with LO 180,
+// with the second product 197 us; hd 64, 1 x 1999, 32 / 8 heads, window 512: 29 us before, 26 us, 28 with the call of
+// o_row_again, 30 with the second product.  Without that product a step of 64 keys takes 1660 cycles (hd 128) and 2140 (hd 64,
+// three CTAs), 920 and 1060 of them for the exponentials; a quarter of those on the multiply-add pipe changed nothing.  Set-up,
+// first loads and output take another 8000 and 5500 cycles of a CTA.
+template <int HD, bool WIN, bool LO>
 __global__ void __launch_bounds__(kAttnThreads, FwdCfg<HD, WIN>::kCtas)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                 const __grid_constant__ CUtensorMap tv, const AttnArgs p, const __grid_constant__ WinRows rows) {
@@ -311,6 +315,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           else
             ptx::mma_f16_ss(tO, desc_add(p_desc, a_off), desc_add(v_desc, k * 2048), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
         }
+        if constexpr (WIN) {   // what P's rounding left
+#pragma unroll
+          for (int k = 0; k < KB / 16; ++k)
+            if (k < steps) ptx::mma_f16_ts(tO, tP + 32 + k * 8, desc_add(v_desc, k * 2048), idesc_o, 1u);
+        }
         ptx::tc_commit(o_full);
         ptx::tc_commit(&v_empty[j % S]);
         if (Cfg::kAlias && j + 1 < nblk) {
@@ -328,7 +337,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
     const uint32_t lane_sel = static_cast<uint32_t>(quad * 32) << 16;
     const float sc = p.scale * kLog2e;
     constexpr float kLazy = 8.f;   // log2 of the largest P value tolerated before the reference maximum moves
-    float m_ref = -INFINITY, l = 0.f, l_used = 0.f;
+    float m_ref = -INFINITY, l = 0.f;
     uint8_t* p_smem = smem + Cfg::kP;
     bool ok = true;
     for (int j = 0; j < nblk; ++j) {
@@ -359,14 +368,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           }
           ptx::tmem_st_wait();
           l *= alpha;
-          l_used *= alpha;
           if (need) m_ref = m_blk;
         }
         return true;
       };
       if (WIN && j == narrow) {
         // the sinks: all of them lie before the rows' windows
-        uint32_t r[16], pk[16];
+        uint32_t r[16], pk[16], lo[16];
         ptx::tmem_ld16(tS + lane_sel, r);
         ptx::tmem_ld_wait();
         ptx::tc_fence_before_sync();
@@ -380,21 +388,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         }
         if (!settle(top * sc)) { ok = false; break; }
         const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
-        float rs0 = 0.f, rs1 = 0.f, ru0 = 0.f, ru1 = 0.f;
+        float rs0 = 0.f, rs1 = 0.f;
 #pragma unroll
         for (int e = 0; e < kSinkCols; e += 2) {
           const float p0 = ex2(fmaf(__uint_as_float(r[e]), sc, neg)), p1 = ex2(fmaf(__uint_as_float(r[e + 1]), sc, neg));
           rs0 += p0;
           rs1 += p1;
           pk[e >> 1] = pack_bf16x2(p0, p1);
-          pk[8 + (e >> 1)] = 0u;
-          ru0 += __uint_as_float(pk[e >> 1] << 16);
-          ru1 += __uint_as_float(pk[e >> 1] & 0xffff0000u);
+          lo[e >> 1] = pack_bf16x2(p0 - __uint_as_float(pk[e >> 1] << 16), p1 - __uint_as_float(pk[e >> 1] & 0xffff0000u));
+          pk[8 + (e >> 1)] = lo[8 + (e >> 1)] = 0u;
         }
         l += rs0 + rs1;
-        l_used += ru0 + ru1;
         if (!waited_o && !ptx::mbar_wait_warp(o_full, (j - 1) & 1, abort_flag)) { ok = false; break; }
         ptx::tmem_st16(tP + lane_sel, pk);
+        ptx::tmem_st16(tP + 32 + lane_sel, lo);
         ptx::tmem_st_wait();
         ptx::tc_fence_before_sync();
         __syncwarp();
@@ -442,9 +449,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       const float m_blk = (KB == 128 ? fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[KB / 32 - 2], mx[KB / 32 - 1])) : fmaxf(mx[0], mx[1])) * sc;
       if (!settle(m_blk)) { ok = false; break; }
       const float neg = WIN && m_ref == -INFINITY ? 0.f : -m_ref;   // a row may see nothing of its first blocks
-      float rs0 = 0.f, rs1 = 0.f, ru0 = 0.f, ru1 = 0.f;
+      float rs0 = 0.f, rs1 = 0.f;
       auto exp_chunk = [&](uint32_t (&r)[32], int c) {
-        uint32_t pk[16];
+        uint32_t pk[16], lo[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           float p0, p1;
@@ -453,9 +460,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           p1 = ex2(p1);
           add2(rs0, rs1, rs0, rs1, p0, p1);
           pk[e >> 1] = pack_bf16x2(p0, p1);
-          // O is divided by the sum of what the product takes: the error that P's rounding leaves in it is then in proportion to
-          // v_j - O, and in delta to dP_j - delta, which counts where a row sees few keys
-          if (WIN) add2(ru0, ru1, ru0, ru1, __uint_as_float(pk[e >> 1] << 16), __uint_as_float(pk[e >> 1] & 0xffff0000u));
+          if constexpr (WIN) {
+            add2(p0, p1, p0, p1, -__uint_as_float(pk[e >> 1] << 16), -__uint_as_float(pk[e >> 1] & 0xffff0000u));
+            lo[e >> 1] = pack_bf16x2(p0, p1);
+          }
         }
         if (c == 0 && !waited_o) {
           // P(j-1) V(j-1) must have finished reading the P buffer before it is overwritten
@@ -463,6 +471,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         }
         if constexpr (WIN) {
           if (ok) ptx::tmem_st16(tP + lane_sel + c * 16, pk);
+          if (ok) ptx::tmem_st16(tP + 32 + lane_sel + c * 16, lo);
           return;
         }
 #pragma unroll
@@ -475,7 +484,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
 #pragma unroll
       for (int c = 1; c < KB / 32; ++c) exp_chunk(r[c], c);
       l += rs0 + rs1;
-      l_used += ru0 + ru1;
       if constexpr (WIN) ptx::tmem_st_wait();
       else ptx::fence_proxy_async_smem();
       ptx::tc_fence_before_sync();
@@ -485,7 +493,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
     if (ok) ok = ptx::mbar_wait_warp(o_full, (nblk - 1) & 1, abort_flag);
     if (ok) {
       ptx::tc_fence_after_sync();
-      const float inv = 1.f / (WIN ? l_used : l);
+      const float inv = 1.f / l;
       bf16* dst = p.o + (static_cast<long long>(b) * p.T + q_idx) * p.o_stride_t + h * HD;
       // WIN: no product reads Q or K any more; the rounded rows go there, and what the rounding left
       uint8_t* q_smem = smem + Cfg::kQ;
@@ -507,7 +515,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
             u.w = pack_bf16x2(__uint_as_float(r[d + 6]) * inv, __uint_as_float(r[d + 7]) * inv);
             *reinterpret_cast<uint4*>(q_smem + swz_off(row, c * 4 + d / 8)) = u;
             probe_finite(probe, u.x); probe_finite(probe, u.y); probe_finite(probe, u.z); probe_finite(probe, u.w);
-            if (p.o_lo) {
+            if constexpr (LO) {
               uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e)
@@ -538,7 +546,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           if (q0 + r < p.T && !(skip >> (r & 31) & 1u)) {
             const long long at = (static_cast<long long>(b) * p.T + q0 + r) * p.o_stride_t + h * HD + u * 8;
             *reinterpret_cast<uint4*>(p.o + at) = *reinterpret_cast<const uint4*>(q_smem + swz_off(r, u));
-            if (p.o_lo) *reinterpret_cast<uint4*>(p.o_lo + at) = *reinterpret_cast<const uint4*>(lo_smem + swz_off(r, u));
+            if constexpr (LO) *reinterpret_cast<uint4*>(p.o_lo + at) = *reinterpret_cast<const uint4*>(lo_smem + swz_off(r, u));
           }
         }
         if (again) again_row = q_idx;
@@ -557,7 +565,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   if (threadIdx.x == 0 && *abort_flag) atomicExch(p.status, kStatusMbarTimeout);
   if (WIN && again_row >= 0) {
     const long long at = (static_cast<long long>(b) * p.T + again_row) * p.o_stride_t + h * HD;
-    o_row_again<HD>(rows, b, h, again_row, p.o + at, p.o_lo ? p.o_lo + at : nullptr);
+    o_row_again<HD>(rows, b, h, again_row, p.o + at, LO ? p.o_lo + at : nullptr);
   }
 }
 
@@ -608,7 +616,7 @@ struct BwdCfg {
 // WIN: a window and sinks.  A block of keys meets the query blocks up to its last key's window.  A block that holds sinks meets
 // all later ones, which would make its CTA the last by far: its query blocks are split over sink_parts CTAs, which leave
 // fp32 sums of the sinks' rows that attn_window_finish_kernel adds in order.
-// Measured: hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: 401 us (396 without the look for what is not finite),
+// Measured: hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: 400 us (396 without the look for what is not finite),
 // 1070 TFLOP/s of the tiles it visits, an eighth of them masked and a tenth for the sinks; the same parts as above bound it.
 template <int HD, bool WIN>
 __global__ void __launch_bounds__(kBwdThreads, 1)
@@ -1168,7 +1176,7 @@ static bool attn_check(const TitbAttnDesc* d) {
   return true;
 }
 
-template <int HD, bool WIN = false>
+template <int HD, bool WIN = false, bool LO = false>
 static int attn_fwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 0, int sinks = 0, void* o_lo = nullptr) {
   using Cfg = FwdCfg<HD, WIN>;
   static bool attr_set[64] = {false};
@@ -1176,7 +1184,7 @@ static int attn_fwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) dev = 0;
   if (!attr_set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<HD, WIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<HD, WIN, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
     attr_set[dev] = true;
   }
@@ -1194,7 +1202,7 @@ static int attn_fwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 
   a.o = static_cast<bf16*>(d->o); a.lse = d->lse; a.o_stride_t = d->o_stride_t;
   a.status = titb_status_ptr();
   dim3 grid(static_cast<unsigned>(d->Hq) * d->B, (d->T + kBlk - 1) / kBlk);
-  launch_dependent(attn_fwd_kernel<HD, WIN>, grid, kAttnThreads, Cfg::kSmem, st, tq, tk, tv, a, window_rows(*d, window, sinks));
+  launch_dependent(attn_fwd_kernel<HD, WIN, LO>, grid, kAttnThreads, Cfg::kSmem, st, tq, tk, tv, a, window_rows(*d, window, sinks));
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -1269,7 +1277,8 @@ static int attn_bwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 
 
 // bf16 window attention, hd 64 or 128 (window_attention.cu checks the operands); window and sinks at most T.
 int window_tc_fwd(const TitbAttnDesc* d, int window, int sinks, void* o_lo, cudaStream_t st) {
-  return d->hd == 64 ? attn_fwd_launch<64, true>(d, st, window, sinks, o_lo) : attn_fwd_launch<128, true>(d, st, window, sinks, o_lo);
+  if (o_lo) return d->hd == 64 ? attn_fwd_launch<64, true, true>(d, st, window, sinks, o_lo) : attn_fwd_launch<128, true, true>(d, st, window, sinks, o_lo);
+  return d->hd == 64 ? attn_fwd_launch<64, true>(d, st, window, sinks) : attn_fwd_launch<128, true>(d, st, window, sinks);
 }
 int window_tc_bwd(const TitbAttnDesc* d, int window, int sinks, float* sink_part, const void* o_lo, cudaStream_t st) {
   return d->hd == 64 ? attn_bwd_launch<64, true>(d, st, window, sinks, sink_part, o_lo)
