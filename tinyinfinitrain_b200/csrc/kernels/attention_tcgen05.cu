@@ -538,6 +538,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       }
       if constexpr (WIN) {
         // a warp's rows leave as whole rows: a store of one unit per row and lane would take a transaction for each
+        __syncwarp();   // the rows that other lanes have put down are read from here on; the ballot orders no memory
         const bool again = q_idx < p.T && probe != 0;   // not finite
         const uint32_t skip = __ballot_sync(0xffffffffu, again);
 #pragma unroll 4
