@@ -87,39 +87,6 @@ struct AttnArgs {
   float* sink_part;  // fp32 [sink_parts][B][sink_blocks][Hkv][dK, dV][kBlk][hd]
 };
 
-// A row of o that is not finite, over visible pairs only.  The call is the kernel's last act and takes its operands from a
-// parameter of their own; that it is there costs 1.1 us of 24 (32 heads of 64, T 1999, window 512), looking for such rows 0.2 of it;
-// from the epilogue, with 32 elements at once (spills at hd 64), 1.3.
-template <int HD>
-__device__ __noinline__ void o_row_again(const WinRows& rows, int b, int h, int i, bf16* o, bf16* o_lo) {
-  const float lse = rows.lse[rows.stat(b, h, i)];
-#pragma unroll 1
-  for (int c = 0; c < HD; c += 16) window_o_again<bf16, 16>(rows, b, h, i, lse, c, o + c, o_lo ? o_lo + c : nullptr);
-}
-
-// Pieces of row j of dK and dV that are not finite, over visible pairs only, from queries [i0, i1).  `sum` is where a part of a
-// sink goes (dK, dV after it), or null.
-template <int HD>
-__device__ __noinline__ void dkv_pieces_again(const WinRows& rows, int b, int hk, int j, int i0, int i1, uint32_t pieces, float* sum,
-                                              bf16* dk, bf16* dv) {
-  for (; pieces; pieces &= pieces - 1) {
-    const int piece = __ffs(pieces) - 1, d0 = piece % (HD / 32) * 32;
-    const bool value = piece < HD / 32;
-#pragma unroll 1
-    for (int d = d0; d < d0 + 32; d += 16) {
-      if (sum) window_dkv_again<bf16, float, 16>(rows, b, hk, j, i0, i1, value, d, sum + (value ? kBlk * HD : 0) + d);
-      else window_dkv_again<bf16, bf16, 16>(rows, b, hk, j, i0, i1, value, d, (value ? dv : dk) + d);
-    }
-  }
-}
-
-// Bits [lo, hi) of a 32-bit word; lo and hi may lie outside it.
-__device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
-  lo = max(lo, 0);
-  hi = min(hi, 32);
-  return hi <= lo ? 0u : (0xffffffffu >> (32 - (hi - lo))) << lo;
-}
-
 // ------------------------------------------------------------------------- forward
 template <int HD, bool WIN>
 struct FwdCfg {
@@ -169,8 +136,8 @@ struct FwdCfg {
 // being the roundings of dS and of dQ).  LO: a backward pass may follow, and what the rounding of o left is kept for its delta.
 // Measured (B200): hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: one CTA an SM 254 us, two with 128 keys a step, P over S
 // and S(j+1) issued behind P(j) V(j) 182 us, with the steps as they are 165 us (790 TFLOP/s of what the rows see), with LO 180,
-// with the second product 197 us; hd 64, 1 x 1999, 32 / 8 heads, window 512: 29 us before, 26 us, 28 with the call of
-// o_row_again, 30 with the second product.  Without that product a step of 64 keys takes 1660 cycles (hd 128) and 2140 (hd 64,
+// with the second product 197 us; hd 64, 1 x 1999, 32 / 8 heads, window 512: 29 us before, 26 us, 28 with the look
+// for rows that are not finite, 30 with the second product.  Without that product a step of 64 keys takes 1660 cycles (hd 128) and 2140 (hd 64,
 // three CTAs), 920 and 1060 of them for the exponentials; a quarter of those on the multiply-add pipe changed nothing.  Set-up,
 // first loads and output take another 8000 and 5500 cycles of a CTA.
 template <int HD, bool WIN, bool LO>
@@ -240,7 +207,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   const uint32_t tS = tmem_base, tO = tmem_base + Cfg::kColO;
   const uint32_t tP = Cfg::kAlias ? tS : tmem_base + 64;   // WIN
   const bool bad_align = (*abort_flag != 0);
-  int again_row = -1;   // WIN: this thread's row, if it is not finite
+  bool again = false;   // WIN: this thread's row is not finite
 
   if (bad_align) {
     // fall through to the common exit
@@ -538,19 +505,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
       }
       if constexpr (WIN) {
         // a warp's rows leave as whole rows: a store of one unit per row and lane would take a transaction for each
-        __syncwarp();   // the rows that other lanes have put down are read from here on; the ballot orders no memory
-        const bool again = q_idx < p.T && probe != 0;   // not finite
-        const uint32_t skip = __ballot_sync(0xffffffffu, again);
+        __syncwarp();   // the rows that other lanes have put down are read from here on
+        again = q_idx < p.T && probe != 0;
 #pragma unroll 4
         for (int i = lane; i < 32 * (HD / 8); i += 32) {
           const int r = quad * 32 + i / (HD / 8), u = i % (HD / 8);
-          if (q0 + r < p.T && !(skip >> (r & 31) & 1u)) {
+          if (q0 + r < p.T) {
             const long long at = (static_cast<long long>(b) * p.T + q0 + r) * p.o_stride_t + h * HD + u * 8;
             *reinterpret_cast<uint4*>(p.o + at) = *reinterpret_cast<const uint4*>(q_smem + swz_off(r, u));
             if constexpr (LO) *reinterpret_cast<uint4*>(p.o_lo + at) = *reinterpret_cast<const uint4*>(lo_smem + swz_off(r, u));
           }
         }
-        if (again) again_row = q_idx;
       }
       if (q_idx < p.T)
         p.lse[(static_cast<long long>(b) * p.Hq + h) * p.T + q_idx] = (m_ref + log2f(l)) * 0.6931471805599453f;
@@ -564,9 +529,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
     ptx::tmem_dealloc(tmem_base, Cfg::kTmemCols);
   }
   if (threadIdx.x == 0 && *abort_flag) atomicExch(p.status, kStatusMbarTimeout);
-  if (WIN && again_row >= 0) {
-    const long long at = (static_cast<long long>(b) * p.T + again_row) * p.o_stride_t + h * HD;
-    o_row_again<HD>(rows, b, h, again_row, p.o + at, LO ? p.o_lo + at : nullptr);
+  if constexpr (WIN) {
+    // the call is the kernel's last act and takes its operands from a parameter of their own
+    const uint32_t bad = __ballot_sync(0xffffffffu, again);
+    if (bad) {
+      const int i0 = q0 + (warp & 3) * 32;
+      const long long at = (static_cast<long long>(b) * p.T + i0) * p.o_stride_t + h * HD;
+      query_rows_again<bf16, false>(rows, b, h, i0, bad, p.o + at, p.o_stride_t, LO ? p.o_lo + at : nullptr);
+    }
   }
 }
 
@@ -596,6 +566,33 @@ struct BwdCfg {
   static constexpr int kPHalf = kAlias ? 64 : 32;
 };
 
+// Rows of key block jb that are not finite (`found`: bit 0 dV, bit 1 dK; a word for either half of a row), over query blocks
+// ib .. ib + nq - 1.  part: of a block with sinks, else -1.  All warps of the CTA, eight rows at a time.
+template <int HD>
+__device__ __noinline__ void key_tile_again(const AttnArgs& p, const WinRows& rows, const uint32_t* found, int b, int hk, int jb, int part,
+                                            int ib, int nq) {
+  constexpr int kFew = 8;
+  const int lane = threadIdx.x & 31, i0 = ib * kBlk, i1 = (ib + nq) * kBlk;
+#pragma unroll 1
+  for (int x = threadIdx.x >> 5; x < 2 * kBlk / kFew; x += kBwdThreads / 32) {
+    const int which = x / (kBlk / kFew), row0 = x % (kBlk / kFew) * kFew, j0 = jb * kBlk + row0;
+    const uint32_t mine = lane < kFew ? found[row0 + lane] | found[kBlk + row0 + lane] : 0u;
+    const uint32_t bad = __ballot_sync(0xffffffffu, (mine >> which & 1u) && j0 + lane < p.T);
+    const uint32_t in_part = part >= 0 && p.sink_parts > 1 ? bad & bit_range(0, p.sinks - j0) : 0u, whole = part <= 0 ? bad & ~in_part : 0u;
+    if (in_part) {
+      float* sum = p.sink_part + ((((static_cast<long long>(part) * p.B + b) * p.sink_blocks + jb) * p.Hkv + hk) * 2 + 1 - which) * (kBlk * HD) +
+                   row0 * HD;
+      if (which == 0) key_rows_again<bf16, float, true>(rows, b, hk, j0, in_part, i0, i1, sum, HD);
+      else key_rows_again<bf16, float, false>(rows, b, hk, j0, in_part, i0, i1, sum, HD);
+    }
+    if (whole) {
+      const long long bt = static_cast<long long>(b) * p.T + j0;
+      if (which == 0) key_rows_again<bf16, bf16, true>(rows, b, hk, j0, whole, i0, i1, p.dv + bt * p.dv_stride_t + hk * HD, p.dv_stride_t);
+      else key_rows_again<bf16, bf16, false>(rows, b, hk, j0, whole, i0, i1, p.dk + bt * p.dk_stride_t + hk * HD, p.dk_stride_t);
+    }
+  }
+}
+
 // Backward pipeline.  Scores are computed transposed (rows = keys, columns = queries), so that P^T can stay in tensor
 // memory as the A operand of dV and only dS passes through shared memory, stored once and read as the K-major A operand
 // of dK and as the MN-major A operand of dQ.  Per (query head, query block) iteration `it` the MMA warp issues
@@ -623,7 +620,7 @@ template <int HD, bool WIN>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                 const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
-                const __grid_constant__ CUtensorMap tdq, const AttnArgs p, const __grid_constant__ WinRows rows) {
+                const __grid_constant__ CUtensorMap tdq, const __grid_constant__ AttnArgs p, const __grid_constant__ WinRows rows) {
   using Cfg = BwdCfg<HD>;
   constexpr int DS = Cfg::kDoStages;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -697,7 +694,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
   dependency_wait();
   dependents_launch();
   const bool bad_align = (*abort_flag != 0);
-  uint32_t again = 0;   // WIN: pieces of 32 elements of this thread's row that are not finite, a bit each
+  // WIN: which rows are not finite, of either half; over the row statistics, which nobody reads any more when the sums are whole
+  uint32_t* again_rows = reinterpret_cast<uint32_t*>(smem + Cfg::kStat);
+  uint32_t again = 0;   // WIN: of this thread's half of a row, bit 0: dV is not finite, bit 1: dK is not
 
   if (bad_align) {
     // fall through to the common exit
@@ -1008,7 +1007,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
             float probe = 0.f;
 #pragma unroll
             for (int e = 0; e < 32; ++e) probe_finite(probe, __uint_as_float(r[e]));
-            if (probe != 0.f) again |= 1u << (which * (HD / 32) + c);
+            if (probe != 0.f) again |= 1u << which;
           }
           if (sink_cta && p.sink_parts > 1 && kv_idx < p.sinks) {
             float* sum = p.sink_part + ((((static_cast<long long>(part) * p.B + b) * p.sink_blocks + jb) * p.Hkv + hk) * 2 + 1 - which) * (kBlk * HD) +
@@ -1029,25 +1028,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
           }
         }
       }
+      if (WIN) again_rows[half * kBlk + row] = again;
     }
   }
 
   ptx::tc_fence_before_sync();
-  __syncthreads();
+  const bool any_again = WIN ? __syncthreads_or(again) : (__syncthreads(), false);
   if (warp == 13) {
     __syncwarp();
     ptx::tmem_dealloc(tmem_base, Cfg::kTmemCols);
   }
   if (threadIdx.x == 0 && *abort_flag) atomicExch(p.status, kStatusMbarTimeout);
-  const int again_j = jb * kBlk + warp % 4 * 32 + lane;
-  const bool again_part = sink_cta && p.sink_parts > 1 && again_j < p.sinks;
-  if (WIN && again && again_j < p.T && (again_part || part == 0)) {
-    const long long bt = static_cast<long long>(b) * p.T + again_j;
-    float* sum = p.sink_part + (((static_cast<long long>(part) * p.B + b) * p.sink_blocks + jb) * p.Hkv + hk) * 2 * (kBlk * HD) +
-                 (again_j - jb * kBlk) * HD;
-    dkv_pieces_again<HD>(rows, b, hk, again_j, ib * kBlk, (ib + nq) * kBlk, again, again_part ? sum : nullptr,
-                         p.dk + bt * p.dk_stride_t + hk * HD, p.dv + bt * p.dv_stride_t + hk * HD);
-  }
+  if (WIN && any_again && *abort_flag == 0) key_tile_again<HD>(p, rows, again_rows, b, hk, jb, sink_cta ? part : -1, ib, nq);
 }
 
 // delta[b,h,t] = sum_d dO[b,t,h,d] * O[b,t,h,d] (WIN: with what O's rounding left), and the fp32 dQ accumulator starts at zero.  hd / 8 neighbouring lanes
@@ -1070,12 +1062,14 @@ __global__ void attn_delta_kernel(const bf16* __restrict__ d_o, const bf16* __re
       const uint4 uc = *reinterpret_cast<const uint4*>(o + bt * o_stride_t + h * HD + d);
       const float2 a0 = unpack_bf16x2(ua.x), a1 = unpack_bf16x2(ua.y), a2 = unpack_bf16x2(ua.z), a3 = unpack_bf16x2(ua.w);
       const float2 c0 = unpack_bf16x2(uc.x), c1 = unpack_bf16x2(uc.y), c2 = unpack_bf16x2(uc.z), c3 = unpack_bf16x2(uc.w);
-      s = a0.x * c0.x + a0.y * c0.y + a1.x * c1.x + a1.y * c1.y + a2.x * c2.x + a2.y * c2.y + a3.x * c3.x + a3.y * c3.y;
-      if (WIN && o_lo) {
+      float2 c[4] = {c0, c1, c2, c3};
+      if (WIN && o_lo) {   // added to o first: the product with an infinite dO has the sign of their sum
         const uint4 ul = *reinterpret_cast<const uint4*>(o_lo + bt * o_stride_t + h * HD + d);
-        const float2 l0 = unpack_bf16x2(ul.x), l1 = unpack_bf16x2(ul.y), l2 = unpack_bf16x2(ul.z), l3 = unpack_bf16x2(ul.w);
-        s += a0.x * l0.x + a0.y * l0.y + a1.x * l1.x + a1.y * l1.y + a2.x * l2.x + a2.y * l2.y + a3.x * l3.x + a3.y * l3.y;
+        const float2 l[4] = {unpack_bf16x2(ul.x), unpack_bf16x2(ul.y), unpack_bf16x2(ul.z), unpack_bf16x2(ul.w)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { c[e].x += l[e].x; c[e].y += l[e].y; }
       }
+      s = a0.x * c[0].x + a0.y * c[0].y + a1.x * c[1].x + a1.y * c[1].y + a2.x * c[2].x + a2.y * c[2].y + a3.x * c[3].x + a3.y * c[3].y;
       float4* acc = reinterpret_cast<float4*>(dq_accum + i * HD + d);
       acc[0] = make_float4(0.f, 0.f, 0.f, 0.f);
       acc[1] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1107,19 +1101,26 @@ __global__ void attn_dq_convert_kernel(const float* __restrict__ acc, bf16* __re
   }
 }
 
-// What of a thread's dq (below) is not finite, over visible pairs only.  It starts over, since a call within the loop below took
-// registers from it.
+// What of a warp's dq (below) is not finite, over visible pairs only.  It starts over, since a call within the loop below took
+// registers from it.  HD / 8 neighbouring lanes hold a row, and a row lies in one warp: n_sink is a multiple of 32.
 template <int HD>
 __device__ __noinline__ void dq_again(const WinRows& rows, const float* acc, long long n_sink, long long n, bf16* dq, long long dq_stride_t) {
-  const int wv = rows.Hq * HD / 8;
-  for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-    if (i < n_sink) continue;
-    const long long bt = (i - n_sink) / wv;
-    const int c = static_cast<int>(i - n_sink - bt * wv) * 8;
+  constexpr int L = HD / 8;
+  const int wv = rows.Hq * L, lane = threadIdx.x & 31;
+  for (long long i0 = blockIdx.x * (long long)blockDim.x + threadIdx.x - lane; i0 < n; i0 += (long long)gridDim.x * blockDim.x) {
+    if (i0 < n_sink) continue;
     float probe = 0.f;
-    for (int e = 0; e < 8; ++e) probe_finite(probe, acc[bt * wv * 8 + c + e]);
-    if (probe != 0.f)
-      window_dq_again<bf16, 8>(rows, static_cast<int>(bt / rows.T), c / HD, static_cast<int>(bt % rows.T), c % HD, dq + bt * dq_stride_t + c);
+    if (i0 + lane < n)
+      for (int e = 0; e < 8; ++e) probe_finite(probe, acc[(i0 + lane - n_sink) * 8 + e]);
+    const uint32_t bad = __ballot_sync(0xffffffffu, probe != 0.f);
+#pragma unroll 1
+    for (int r = 0; r < 32; r += L) {
+      if (!(bad & bit_range(r, r + L))) continue;
+      const long long bt = (i0 + r - n_sink) / wv;
+      const int h = static_cast<int>(i0 + r - n_sink - bt * wv) / L;
+      query_rows_again<bf16, true>(rows, static_cast<int>(bt / rows.T), h, static_cast<int>(bt % rows.T), 1u, dq + bt * dq_stride_t + h * HD,
+                                   dq_stride_t, nullptr);
+    }
   }
 }
 
@@ -1165,7 +1166,8 @@ __global__ void __launch_bounds__(256, 6) attn_window_finish_kernel(const AttnAr
     probe_finite(probe, f0.x); probe_finite(probe, f0.y); probe_finite(probe, f0.z); probe_finite(probe, f0.w);
     probe_finite(probe, f1.x); probe_finite(probe, f1.y); probe_finite(probe, f1.z); probe_finite(probe, f1.w);
   }
-  if (probe != 0.f) dq_again<HD>(rows, p.dq_accum, n_sink, n_sink + n_dq, dq, dq_stride_t);
+  __syncwarp();   // the rows are read again by lanes other than those that stored them
+  if (__any_sync(0xffffffffu, probe != 0.f)) dq_again<HD>(rows, p.dq_accum, n_sink, n_sink + n_dq, dq, dq_stride_t);
 }
 
 static bool attn_check(const TitbAttnDesc* d) {

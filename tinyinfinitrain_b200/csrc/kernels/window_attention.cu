@@ -199,6 +199,21 @@ __device__ __forceinline__ bool piece_finite(const float (&acc)[HD / 64][4][4], 
   return probe == 0.f;
 }
 
+// The warp's eight rows of a tile (the first is that of its lane 0) that are not finite.
+template <int HD>
+__device__ __forceinline__ uint32_t bad_rows(const float (&acc)[HD / 64][4][4], int hd, int n_rows, int row, int tx) {
+  uint32_t bad = 0u;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    bool mine = false;
+#pragma unroll
+    for (int c = 0; c < HD / 64; ++c) mine = mine || (c * 64 + tx * 4 < hd && !piece_finite<HD>(acc, c, r));
+    const uint32_t votes = __ballot_sync(0xffffffffu, mine && row + r < n_rows);
+    bad |= (votes & 0xffffu ? 1u << r : 0u) | (votes >> 16 ? 1u << (4 + r) : 0u);
+  }
+  return bad;
+}
+
 template <int HD>
 struct WinFwdSmem {
   static constexpr int kTile = kWinStep * (HD + 4);   // K and V in two buffers each
@@ -288,17 +303,12 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
       for (int r = 0; r < 4; ++r) acc[e / 4][e % 4][r] -= to_f32(from_f32<T>(acc[e / 4][e % 4][r]));
     store_rows<bf16, HD>(p.o_lo + row0 * p.o_st + h * p.hd, p.o_st, q0, p.T, p.hd, acc, ty, tx);
   }
-#pragma unroll
-  for (int c = 0; c < HD / 64; ++c)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = q0 + ty * 4 + r, d = c * 64 + tx * 4;
-      if (i < p.T && d < p.hd && !piece_finite<HD>(acc, c, r)) {
-        const long long at = (row0 + i) * p.o_st + h * p.hd + d;
-        window_o_again<T, 4>(rows, b, h, i, m[r] + logf(l[r]), d, static_cast<T*>(p.o) + at,
-                             sizeof(T) == 2 && p.o_lo ? p.o_lo + at : nullptr);
-      }
-    }
+  if (const uint32_t bad = bad_rows<HD>(acc, p.hd, p.T, q0 + ty * 4, tx)) {
+    __syncwarp();   // rows and log-sum-exp are read again by other lanes
+    const int i0 = q0 + static_cast<int>(threadIdx.x >> 5) * 8;
+    const long long at = (row0 + i0) * p.o_st + h * p.hd;
+    query_rows_again<T, false>(rows, b, h, i0, bad, static_cast<T*>(p.o) + at, p.o_st, sizeof(T) == 2 && p.o_lo ? p.o_lo + at : nullptr);
+  }
 }
 
 template <int HD>
@@ -334,12 +344,13 @@ __global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p,
     float s = 0.f;
 #pragma unroll
     for (int c = 0; c < HD / 64; ++c) {
-      const float4 a = load4(d_o, i, p.do_st, c * 64 + tx * 4, p.T, p.hd), x = load4(o, i, p.o_st, c * 64 + tx * 4, p.T, p.hd);
-      s += a.x * x.x + a.y * x.y + a.z * x.z + a.w * x.w;
-      if (sizeof(T) == 2 && p.o_lo) {
+      const float4 a = load4(d_o, i, p.do_st, c * 64 + tx * 4, p.T, p.hd);
+      float4 x = load4(o, i, p.o_st, c * 64 + tx * 4, p.T, p.hd);
+      if (sizeof(T) == 2 && p.o_lo) {   // added to o first: the product with an infinite dO has the sign of their sum
         const float4 y = load4(static_cast<const bf16*>(p.o_lo) + row0 * p.o_st + h * p.hd, i, p.o_st, c * 64 + tx * 4, p.T, p.hd);
-        s += a.x * y.x + a.y * y.y + a.z * y.z + a.w * y.w;
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
       }
+      s += a.x * x.x + a.y * x.y + a.z * x.z + a.w * x.w;
     }
     delta[r] = half_warp_sum(s);
     lse[r] = i < p.T ? p.lse[stat0 + i] : 0.f;
@@ -379,15 +390,11 @@ __global__ void __launch_bounds__(kWinThreads) window_dq_kernel(const WinArgs p,
     __syncthreads();
   }
   store_rows<T, HD>(static_cast<T*>(p.dq) + row0 * p.dq_st + h * p.hd, p.dq_st, q0, p.T, p.hd, acc, ty, tx);
-  __syncthreads();   // delta is read again
-#pragma unroll
-  for (int c = 0; c < HD / 64; ++c)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = q0 + ty * 4 + r, d = c * 64 + tx * 4;
-      if (i < p.T && d < p.hd && !piece_finite<HD>(acc, c, r))
-        window_dq_again<T, 4>(rows, b, h, i, d, static_cast<T*>(p.dq) + (row0 + i) * p.dq_st + h * p.hd + d);
-    }
+  if (const uint32_t bad = bad_rows<HD>(acc, p.hd, p.T, q0 + ty * 4, tx)) {
+    __syncwarp();   // rows and delta are read again by other lanes
+    const int i0 = q0 + static_cast<int>(threadIdx.x >> 5) * 8;
+    query_rows_again<T, true>(rows, b, h, i0, bad, static_cast<T*>(p.dq) + (row0 + i0) * p.dq_st + h * p.hd, p.dq_st, nullptr);
+  }
 }
 
 template <int HD>
@@ -468,32 +475,22 @@ __global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p
     store_rows<T, HD>(static_cast<T*>(p.dk) + row0 * p.dk_st + hk * p.hd, p.dk_st, k0, p.T, p.hd, dk, ty, tx);
     store_rows<T, HD>(static_cast<T*>(p.dv) + row0 * p.dv_st + hk * p.hd, p.dv_st, k0, p.T, p.hd, dv, ty, tx);
   }
-  const int i0 = first * kWinStep, i1 = (first + n_steps) * kWinStep;
-#pragma unroll
-  for (int c = 0; c < HD / 64; ++c)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int j = k0 + ty * 4 + r, d = c * 64 + tx * 4;
-      if (part != 0 || j >= p.T || d >= p.hd) continue;
-      if (!piece_finite<HD>(dk, c, r))
-        window_dkv_again<T, T, 4>(rows, b, hk, j, i0, i1, false, d, static_cast<T*>(p.dk) + (row0 + j) * p.dk_st + hk * p.hd + d);
-      if (!piece_finite<HD>(dv, c, r))
-        window_dkv_again<T, T, 4>(rows, b, hk, j, i0, i1, true, d, static_cast<T*>(p.dv) + (row0 + j) * p.dv_st + hk * p.hd + d);
-    }
-  if (sink_cta && p.sink_parts > 1) {
-    float* sum = p.sink_part + (((static_cast<long long>(part) * p.B + b) * p.sink_tiles + tile) * p.Hkv + hk) * 2 * kWinRows * p.hd;
+  const bool parts = sink_cta && p.sink_parts > 1;
+  float* sum = p.sink_part + (((static_cast<long long>(part) * p.B + b) * p.sink_tiles + tile) * p.Hkv + hk) * 2 * kWinRows * p.hd;
+  if (parts) {
     store_rows<float, HD>(sum, p.hd, 0, p.sinks - k0, p.hd, dk, ty, tx);
     store_rows<float, HD>(sum + kWinRows * p.hd, p.hd, 0, p.sinks - k0, p.hd, dv, ty, tx);
-#pragma unroll
-    for (int c = 0; c < HD / 64; ++c)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = k0 + ty * 4 + r, d = c * 64 + tx * 4;
-        if (j >= p.sinks || d >= p.hd) continue;
-        float* at = sum + (j - k0) * p.hd + d;
-        if (!piece_finite<HD>(dk, c, r)) window_dkv_again<T, float, 4>(rows, b, hk, j, i0, i1, false, d, at);
-        if (!piece_finite<HD>(dv, c, r)) window_dkv_again<T, float, 4>(rows, b, hk, j, i0, i1, true, d, at + kWinRows * p.hd);
-      }
+  }
+  const uint32_t bad_k = bad_rows<HD>(dk, p.hd, p.T, k0 + ty * 4, tx), bad_v = bad_rows<HD>(dv, p.hd, p.T, k0 + ty * 4, tx);
+  if (bad_k | bad_v) {
+    __syncwarp();   // the rows are read again by other lanes
+    const int r0 = static_cast<int>(threadIdx.x >> 5) * 8, j0 = k0 + r0, i0 = first * kWinStep, i1 = (first + n_steps) * kWinStep;
+    const uint32_t in_part = parts ? bit_range(0, p.sinks - j0) : 0u, whole = part == 0 ? ~in_part : 0u;
+    T *dk0 = static_cast<T*>(p.dk) + (row0 + j0) * p.dk_st + hk * p.hd, *dv0 = static_cast<T*>(p.dv) + (row0 + j0) * p.dv_st + hk * p.hd;
+    if (bad_k & in_part) key_rows_again<T, float, false>(rows, b, hk, j0, bad_k & in_part, i0, i1, sum + r0 * p.hd, p.hd);
+    if (bad_v & in_part) key_rows_again<T, float, true>(rows, b, hk, j0, bad_v & in_part, i0, i1, sum + (kWinRows + r0) * p.hd, p.hd);
+    if (bad_k & whole) key_rows_again<T, T, false>(rows, b, hk, j0, bad_k & whole, i0, i1, dk0, p.dk_st);
+    if (bad_v & whole) key_rows_again<T, T, true>(rows, b, hk, j0, bad_v & whole, i0, i1, dv0, p.dv_st);
   }
 }
 
