@@ -1118,8 +1118,8 @@ __device__ __noinline__ void dq_again(const WinRows& rows, const float* acc, lon
       if (!(bad & bit_range(r, r + L))) continue;
       const long long bt = (i0 + r - n_sink) / wv;
       const int h = static_cast<int>(i0 + r - n_sink - bt * wv) / L;
-      query_rows_again<bf16, true>(rows, static_cast<int>(bt / rows.T), h, static_cast<int>(bt % rows.T), 1u, dq + bt * dq_stride_t + h * HD,
-                                   dq_stride_t, nullptr);
+      query_rows_again<bf16, true, 1>(rows, static_cast<int>(bt / rows.T), h, static_cast<int>(bt % rows.T), 1u,
+                                      dq + bt * dq_stride_t + h * HD, dq_stride_t, nullptr);
     }
   }
 }

@@ -196,16 +196,17 @@ __device__ __forceinline__ void sum_lanes(float (&a)[N], int lane) {
   for (int m = 0; m < N; ++m) a[m] = __shfl_sync(0xffffffffu, own, m * (32 / N));
 }
 
-// Rows that are summed again, kAgain at a time over the same vectors: neighbours see much the same ones.
-constexpr int kAgain = 2, kPairs = 4;
+// Rows that are summed again, A at a time over the same vectors: neighbours see much the same ones.
+constexpr int kPairs = 4;
+template <int A>
 struct RowsAgain {
-  uint32_t want[kAgain];                      // as row_verdict returns them
-  float own[kAgain][kRowWords], pair[kAgain][kRowWords], acc[kAgain][kRowWords];
+  uint32_t want[A];                           // as row_verdict returns them
+  float own[A][kRowWords], pair[A][kRowWords], acc[A][kRowWords];
   // No wanted column is anything but NaN: more terms change nothing.
   __device__ __forceinline__ bool settled() const {
     bool open = false;
 #pragma unroll
-    for (int k = 0; k < kAgain; ++k)
+    for (int k = 0; k < A; ++k)
 #pragma unroll
       for (int e = 0; e < kRowWords; ++e) open = open || ((want[k] >> e & 1u) && acc[k][e] == acc[k][e]);
     return !__any_sync(0xffffffffu, open);
@@ -221,10 +222,10 @@ struct VectorsAgain {
 };
 
 // The terms of the first n of them; see(k, u): row k sees vector u.  lse and delta are the vectors' (KEYS) or the rows' own.
-template <typename T, bool DS, bool KEYS, typename S>
-__device__ __forceinline__ void add_pairs(RowsAgain& r, const VectorsAgain<T, DS>& v, const float (&lse)[kAgain], const float (&delta)[kAgain],
+template <typename T, bool DS, bool KEYS, int A, typename S>
+__device__ __forceinline__ void add_pairs(RowsAgain<A>& r, const VectorsAgain<T, DS>& v, const float (&lse)[A], const float (&delta)[A],
                                           float scale, int n, int lane, S see) {
-  constexpr int N = kAgain * kPairs;
+  constexpr int N = A * kPairs;
   float sums[DS ? 2 * N : N];
 #pragma unroll
   for (int m = 0; m < N; ++m) {
@@ -251,8 +252,9 @@ __device__ __forceinline__ void add_pairs(RowsAgain& r, const VectorsAgain<T, DS
 }
 
 // Rows i0 + r of O (or dQ) of head h, for the bits r of `bad`.  out: row i0, `stride` elements between tokens; lo (may be null):
-// what the rounding of O left, laid out the same.  A whole warp, which sees the rows, the log-sum-exp and delta as stored.
-template <typename T, bool DQ>
+// what the rounding of O left, laid out the same.  A: rows that are summed at a time.  A whole warp, which sees the rows, the
+// log-sum-exp and delta as stored.
+template <typename T, bool DQ, int A = 2>
 __device__ __noinline__ void query_rows_again(const WinRows& w, int b, int h, int i0, uint32_t bad, T* out, long long stride, bf16* lo) {
   const int lane = threadIdx.x & 31, hk = h / (w.Hq / w.Hkv), i = i0 + lane;
   const bool mine = bad >> lane & 1u;
@@ -306,12 +308,12 @@ __device__ __noinline__ void query_rows_again(const WinRows& w, int b, int h, in
   }
 #pragma unroll 1
   while (bad) {
-    int t[kAgain];
-    float x[kAgain][kRowWords], lse[kAgain], delta[kAgain];
-    RowsAgain rows{};
+    int t[A];
+    float x[A][kRowWords], lse[A], delta[A];
+    RowsAgain<A> rows{};
     uint32_t any = 0u;
 #pragma unroll
-    for (int k = 0; k < kAgain; ++k) {
+    for (int k = 0; k < A; ++k) {
       t[k] = -1;
       lse[k] = delta[k] = 0.f;
       if (!bad) continue;
@@ -328,7 +330,7 @@ __device__ __noinline__ void query_rows_again(const WinRows& w, int b, int h, in
       }
     }
     if (__any_sync(0xffffffffu, any)) {
-      const int last = t[kAgain - 1] < 0 ? t[0] : t[kAgain - 1];
+      const int last = t[A - 1] < 0 ? t[0] : t[A - 1];
       const int first = max(0, t[0] - w.window + 1), sinks = min(w.sinks, first), n = sinks + last - first + 1;
       const auto key = [&](int v) { return v < sinks ? v : first + v - sinks; };
 #pragma unroll 1
@@ -346,7 +348,7 @@ __device__ __noinline__ void query_rows_again(const WinRows& w, int b, int h, in
       }
     }
 #pragma unroll
-    for (int k = 0; k < kAgain; ++k)
+    for (int k = 0; k < A; ++k)
 #pragma unroll
       for (int e = 0; e < kRowWords; ++e) {
         const int d = column_of(e, lane);
@@ -365,6 +367,7 @@ __device__ __noinline__ void query_rows_again(const WinRows& w, int b, int h, in
 template <typename T, typename Out, bool VALUE>
 __device__ __noinline__ void key_rows_again(const WinRows& w, int b, int hk, int j0, uint32_t bad, int ia, int ib, Out* out,
                                             long long stride) {
+  constexpr int A = 2;
   const int lane = threadIdx.x & 31, G = w.Hq / w.Hkv, j = j0 + lane;
   const bool mine = bad >> lane & 1u;
   RowKinds kinds;
@@ -453,13 +456,13 @@ __device__ __noinline__ void key_rows_again(const WinRows& w, int b, int hk, int
   }
 #pragma unroll 1
   while (bad) {
-    int t[kAgain], until[kAgain];
-    const float unused[kAgain] = {};
-    float x[kAgain][kRowWords];
-    RowsAgain rows{};
+    int t[A], until[A];
+    const float unused[A] = {};
+    float x[A][kRowWords];
+    RowsAgain<A> rows{};
     uint32_t any = 0u;
 #pragma unroll
-    for (int k = 0; k < kAgain; ++k) {
+    for (int k = 0; k < A; ++k) {
       t[k] = w.T;
       until[k] = -1;
       if (!bad) continue;
@@ -476,7 +479,7 @@ __device__ __noinline__ void key_rows_again(const WinRows& w, int b, int hk, int
       const int from = max(ia, t[0]);
       int to = 0;
 #pragma unroll
-      for (int k = 0; k < kAgain; ++k) to = max(to, min(min(ib, w.T), until[k] + 1));
+      for (int k = 0; k < A; ++k) to = max(to, min(min(ib, w.T), until[k] + 1));
       bool open = from < to;
 #pragma unroll 1
       for (int h = hk * G; h < hk * G + G && open; ++h) {
@@ -498,7 +501,7 @@ __device__ __noinline__ void key_rows_again(const WinRows& w, int b, int hk, int
       }
     }
 #pragma unroll
-    for (int k = 0; k < kAgain; ++k)
+    for (int k = 0; k < A; ++k)
 #pragma unroll
       for (int e = 0; e < kRowWords; ++e) {
         const int d = column_of(e, lane);
