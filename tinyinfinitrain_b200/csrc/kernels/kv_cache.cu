@@ -585,6 +585,9 @@ struct PagedMma {
 // and two stages (192 sequences, window 1024 of up to 32768, 32 / 8 heads: 69 us, 5.6 TB/s; two CTAs and three stages 79 us),
 // hd 128 the other way round (131071 positions, 32 / 8 heads: 94 us, 5.7 TB/s; 102 us).  64 sequences of up to 8192 positions, 32 / 8
 // heads of 128: 97 us, 6.0 TB/s.  The first kernel, one CTA an item on the CUDA cores: 293 us, 21 ms, 1.35 ms.
+// V is multiplied by P rounded to bf16 and by what that rounding left: without the second the output was off by 0.177 %, 0.165 %
+// being its own rounding.  Up to eight heads leave half of the product's rows empty, which take the remainder for nothing; more
+// heads take a second product (64 x 8192 positions, 32 / 2 heads of 128: 101 -> 105 us).
 template <int HD, bool UPPER>
 __global__ void __launch_bounds__(kPagedThreads, PagedMma<HD>::kCtas) paged_mma_kernel(const PagedArgs p) {
   using Cfg = PagedMma<HD>;
@@ -648,7 +651,9 @@ __global__ void __launch_bounds__(kPagedThreads, PagedMma<HD>::kCtas) paged_mma_
   };
 
   uint32_t q[HD / 16][4];
-  float o[HD / 8][4];
+  // sums of V times P rounded to bf16, and times what that rounding left: with up to eight heads in rows 8 .. 15 of the same
+  // product, which would be empty, else (UPPER) in a product and an accumulator of their own
+  float o[HD / 8][4], rest[UPPER ? HD / 8 : 1][4];
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   const float sc = p.scale * 1.4426950408889634f;
   const int gr = lane >> 2, tq = lane & 3;
@@ -666,7 +671,10 @@ __global__ void __launch_bounds__(kPagedThreads, PagedMma<HD>::kCtas) paged_mma_
       q[k][3] = hi ? *reinterpret_cast<const uint32_t*>(src + (gr + 8) * HD + k * 16 + 8) : 0u;
     }
 #pragma unroll
-    for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+    for (int d = 0; d < HD / 8; ++d) {
+      o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+      if (UPPER) rest[d][0] = rest[d][1] = rest[d][2] = rest[d][3] = 0.f;
+    }
     m0 = m1 = -INFINITY;
     l0 = l1 = 0.f;
   };
@@ -734,26 +742,36 @@ __global__ void __launch_bounds__(kPagedThreads, PagedMma<HD>::kCtas) paged_mma_
         for (int d = 0; d < HD / 8; ++d) {
           o[d][0] *= a0;
           o[d][1] *= a0;
+          o[d][2] *= UPPER ? a1 : a0;
+          o[d][3] *= UPPER ? a1 : a0;
           if (UPPER) {
-            o[d][2] *= a1;
-            o[d][3] *= a1;
+            rest[d][0] *= a0;
+            rest[d][1] *= a0;
+            rest[d][2] *= a1;
+            rest[d][3] *= a1;
           }
         }
       }
       const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
-      uint32_t pf[KEYS / 16][4];
+      uint32_t pf[KEYS / 16][4], pr[UPPER ? KEYS / 16 : 1][4];
+      const auto left = [](float x0, float x1, uint32_t rounded) {
+        return pack_bf16x2(x0 - __uint_as_float(rounded << 16), x1 - __uint_as_float(rounded & 0xffff0000u));
+      };
 #pragma unroll
       for (int n = 0; n < KEYS / 8; ++n) {
         const float x0 = exp2_fast(s[n][0] - r0), x1 = exp2_fast(s[n][1] - r0);
         l0 += x0 + x1;
-        // the product takes P rounded to bf16; its sum is taken before that
-        pf[n / 2][(n & 1) * 2] = pack_bf16x2(x0, x1);
+        const uint32_t p0 = pack_bf16x2(x0, x1);
+        pf[n / 2][(n & 1) * 2] = p0;
         if (UPPER) {
           const float y0 = exp2_fast(s[n][2] - r1), y1 = exp2_fast(s[n][3] - r1);
           l1 += y0 + y1;
-          pf[n / 2][(n & 1) * 2 + 1] = pack_bf16x2(y0, y1);
+          const uint32_t p1 = pack_bf16x2(y0, y1);
+          pf[n / 2][(n & 1) * 2 + 1] = p1;
+          pr[n / 2][(n & 1) * 2] = left(x0, x1, p0);
+          pr[n / 2][(n & 1) * 2 + 1] = left(y0, y1, p1);
         } else {
-          pf[n / 2][(n & 1) * 2 + 1] = 0u;
+          pf[n / 2][(n & 1) * 2 + 1] = left(x0, x1, p0);
         }
       }
 #pragma unroll
@@ -765,6 +783,10 @@ __global__ void __launch_bounds__(kPagedThreads, PagedMma<HD>::kCtas) paged_mma_
           load_matrix4_t(f, vb + r * HD * 2 + (((2 * d + (lane >> 4)) ^ (r & 7)) << 4));
           mma16(o[2 * d], pf[n], f[0], f[1]);
           mma16(o[2 * d + 1], pf[n], f[2], f[3]);
+          if (UPPER) {
+            mma16(rest[2 * d], pr[n], f[0], f[1]);
+            mma16(rest[2 * d + 1], pr[n], f[2], f[3]);
+          }
         }
       }
     }
@@ -783,10 +805,15 @@ __global__ void __launch_bounds__(kPagedThreads, PagedMma<HD>::kCtas) paged_mma_
       // this warp's sums go where the step's rows were, which it has read; nothing is copied there before the next step
       __syncwarp();
       float* sum = reinterpret_cast<float*>(ring + st * Cfg::kStepBytes);
+      // an infinite V is infinite in the first sum; what it makes of the second, whose weights have any sign, does not count
+      const auto whole = [](float x, float r) { return fabsf(r) < INFINITY ? x + r : x; };
 #pragma unroll
       for (int d = 0; d < HD / 8; ++d) {
-        *reinterpret_cast<float2*>(sum + gr * HD + d * 8 + tq * 2) = make_float2(o[d][0], o[d][1]);
-        if (UPPER) *reinterpret_cast<float2*>(sum + (gr + 8) * HD + d * 8 + tq * 2) = make_float2(o[d][2], o[d][3]);
+        const float(&r)[4] = rest[UPPER ? d : 0];
+        *reinterpret_cast<float2*>(sum + gr * HD + d * 8 + tq * 2) =
+            make_float2(whole(o[d][0], UPPER ? r[0] : o[d][2]), whole(o[d][1], UPPER ? r[1] : o[d][3]));
+        if (UPPER)
+          *reinterpret_cast<float2*>(sum + (gr + 8) * HD + d * 8 + tq * 2) = make_float2(whole(o[d][2], r[2]), whole(o[d][3], r[3]));
       }
       finish_item<bf16, HG, 4>(p, info.y, info.z, item_ends && !began_before, began_before,
                                reinterpret_cast<const float*>(smem + st * Cfg::kStepBytes), STAGES * Cfg::kStepBytes / 4, HD, sm_m, sm_l);
