@@ -41,3 +41,36 @@ def check_digits(name, got, value, bound):
     if got.numel() >= 16384:
         rounded = (value.to(got.dtype).double() - value).norm().item()
         assert err.norm().item() <= 1.03 * rounded, f"{name}: {err.norm().item() / rounded:.3f} times the error of its rounding"
+
+
+def gradients64(q, k, v, do, mask, scale=None):
+    """{name: (value, bound)} of dq, dk, dv where the output's error is that of output64 and what its own rounding left is kept
+    (rounded itself, u^2).  The backward pass rounds P of dV and dS to the type, the choices that are left:
+      |d dV| <= u |dV| + (u + E_i + n e) P^T |dO|
+      |d dS| <= (u + E_i + 4 e) |dS| + scale P (hd e |dO||V|^T + |dO|.(|d O| - u |O| + u^2 |O|) + hd e |dO|.|O|)
+      |d dQ| <= u |dQ| + (|d dS| + n e |dS|) |K|, and so for dK."""
+    u = half_step(q.dtype)
+    o, o_err = (t.transpose(1, 2) for t in output64(q, k, v, mask, scale))
+    q, k, v, g = (t.detach().double().transpose(1, 2) for t in (q, k, v, do))
+    B, Hq, T, hd = q.shape
+    G = Hq // k.shape[1]
+    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
+    kr, vr = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
+    hidden, n = ~mask.to(q.device), mask.sum(-1).max().item()
+    s = (q @ kr.transpose(2, 3)) * scale
+    p = s.masked_fill(hidden, -math.inf).softmax(-1)
+    score_err = (hd * E * scale * (q.abs() @ kr.abs().transpose(2, 3)) + 2 * E * s.abs()).masked_fill(hidden, 0)
+    row = 2 * score_err.amax(-1, keepdim=True) + (n + 8) * E + 2.0 ** -20
+    share = lambda t: t.unflatten(1, (Hq // G, G)).sum(2)
+    terms = n + G * T
+    dv = share(p.transpose(2, 3) @ g)
+    dv_err = u * dv.abs() + share(((u + row + terms * E) * p).transpose(2, 3) @ g.abs())
+    ds = scale * p * (g @ vr.transpose(2, 3) - (g * o).sum(-1, keepdim=True))
+    delta_err = (g.abs() * (o_err - u * o.abs() + u * u * o.abs())).sum(-1, keepdim=True)
+    ds_err = (u + row + 4 * E) * ds.abs() + scale * p * (hd * E * (g.abs() @ vr.abs().transpose(2, 3)) + delta_err +
+                                                         hd * E * (g.abs() * o.abs()).sum(-1, keepdim=True))
+    ds_err = ds_err + terms * E * ds.abs()
+    dq, dk = ds @ kr, share(ds.transpose(2, 3) @ q)
+    back = lambda t: t.transpose(1, 2)
+    return {"dq": (back(dq), back(u * dq.abs() + ds_err @ kr.abs())), "dv": (back(dv), back(dv_err)),
+            "dk": (back(dk), back(u * dk.abs() + share(ds_err.transpose(2, 3) @ q.abs())))}
