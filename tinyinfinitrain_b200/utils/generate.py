@@ -58,7 +58,7 @@ def generate(model, prompts: Sequence[Sequence[int]], max_new_tokens: int,
     sample = sample or (lambda logits: logits.argmax(-1))
     device = model.lm_head.weight.device
     longest = max(len(p) for p in prompts)
-    cache = model.new_cache(len(prompts), longest + max_new_tokens, page_size)
+    cache = model.new_cache(len(prompts), longest + max_new_tokens - 1, page_size)     # the last token is not fed back
     idx = torch.zeros(len(prompts), longest, dtype=torch.int64)
     for row, p in zip(idx, prompts):
         row[:len(p)] = torch.as_tensor(p, dtype=torch.int64)
