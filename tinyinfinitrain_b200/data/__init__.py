@@ -121,6 +121,11 @@ class Tokenizer:
             tok = C.sample_mult(probs, coin)
             x[0, t] = tok
             out += self.Decode(tok)
+        if use_cache and cache.lengths.is_cuda:
+            from ..parallel.health import check_device_status
+
+            with torch.cuda.device(cache.lengths.device):
+                check_device_status()     # positions that the cache could not keep are reported there
         if stream is not None:
             stream.write(out + "\n")
         return out

@@ -5,6 +5,8 @@ from typing import Callable, List, Optional, Sequence
 
 import torch
 
+from ..parallel.health import check_device_status
+
 
 class DecodeStep:
     """One new token of every sequence of a cache: ``step(tokens)`` with tokens int64 [batch] appends them and returns the
@@ -50,7 +52,8 @@ def generate(model, prompts: Sequence[Sequence[int]], max_new_tokens: int,
              sample: Optional[Callable[[torch.Tensor], torch.Tensor]] = None, page_size: int = 64,
              use_graph: bool = True) -> List[List[int]]:
     """``max_new_tokens`` tokens behind each of the prompts (lists of token ids, of any lengths from one on).  ``sample`` maps the
-    logits [batch, vocab_size] to the next tokens, int64 [batch]; by default the most likely one."""
+    logits [batch, vocab_size] to the next tokens, int64 [batch]; by default the most likely one.  Raises if a kernel has reported an
+    error on the GPU (``parallel.health.check_device_status``)."""
     if not prompts or min(len(p) for p in prompts) < 1 or max_new_tokens < 0:
         raise ValueError("generate: every prompt needs a token, and max_new_tokens must not be negative")
     if max_new_tokens == 0:
@@ -69,4 +72,8 @@ def generate(model, prompts: Sequence[Sequence[int]], max_new_tokens: int,
     for _ in range(max_new_tokens - 1):
         tokens = sample(step(tokens))
         out.append(tokens)
-    return torch.stack(out, dim=1).tolist()
+    out = torch.stack(out, dim=1).tolist()
+    if device.type == "cuda":
+        with torch.cuda.device(device):
+            check_device_status()
+    return out
