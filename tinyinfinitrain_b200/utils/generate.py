@@ -37,7 +37,11 @@ class DecodeStep:
         cache._empty = empty
 
     def __call__(self, tokens: torch.Tensor) -> torch.Tensor:
-        self.idx.copy_(tokens.view(-1, 1), non_blocking=True)
+        if tokens.dim() == 0 or tokens.shape[0] != self.cache.batch or tokens.numel() != self.cache.batch:
+            raise ValueError(f"DecodeStep: tokens of shape {tuple(tokens.shape)} for a cache of {self.cache.batch} sequences")
+        if tokens.is_floating_point():
+            raise ValueError(f"DecodeStep: tokens must be integers, got {tokens.dtype}")
+        self.idx.copy_(tokens.reshape(-1, 1), non_blocking=True)
         if not self.use_graph:
             return self.model(self.idx, cache=self.cache)
         if self.graph is None:
