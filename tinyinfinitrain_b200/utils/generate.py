@@ -15,7 +15,8 @@ class DecodeStep:
 
     def __init__(self, model, cache, use_graph: bool = True):
         self.model, self.cache = model, cache
-        self.idx = torch.zeros(cache.batch, 1, dtype=torch.int64, device=cache.lengths.device)
+        self.device = cache.lengths.device
+        self.idx = torch.zeros(cache.batch, 1, dtype=torch.int64, device=self.device)
         self.use_graph = use_graph and self.idx.is_cuda
         self.graph = self.logits = None
 
@@ -23,17 +24,19 @@ class DecodeStep:
         # the steps before the capture append at the position that the first real one writes again
         cache = self.cache
         lengths, empty = cache.lengths.clone(), cache._empty
-        device = self.idx.device
-        side = torch.cuda.Stream(device=device)
-        side.wait_stream(torch.cuda.current_stream(device))
-        with torch.cuda.stream(side):
-            self.model(self.idx, cache=cache)
-            cache.lengths.copy_(lengths)
-        torch.cuda.current_stream(device).wait_stream(side)
-        torch.cuda.synchronize(device)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
-            self.logits = self.model(self.idx, cache=cache)
+        # kernels are launched on the cache's device, whichever the current one is: the capture has to be there too
+        with torch.cuda.device(self.device):
+            side = torch.cuda.Stream(device=self.device)
+            side.wait_stream(torch.cuda.current_stream(self.device))
+            with torch.cuda.stream(side):
+                self.model(self.idx, cache=cache)
+                cache.lengths.copy_(lengths)
+            torch.cuda.current_stream(self.device).wait_stream(side)
+            torch.cuda.synchronize(self.device)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                self.logits = self.model(self.idx, cache=cache)
+        self.graph = graph     # whole: a capture that failed is made again by the next call
         cache._empty = empty
 
     def __call__(self, tokens: torch.Tensor) -> torch.Tensor:
@@ -46,7 +49,8 @@ class DecodeStep:
             return self.model(self.idx, cache=self.cache)
         if self.graph is None:
             self._capture()
-        self.graph.replay()
+        with torch.cuda.device(self.device):
+            self.graph.replay()
         self.cache._empty = False
         return self.logits
 
