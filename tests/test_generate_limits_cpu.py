@@ -29,3 +29,12 @@ def test_tokens_behind_the_context():
     gpt2 = next(iter(_models()))
     with pytest.raises(ValueError, match="block size"):
         generate(gpt2, [[1] * 24], 2)
+
+
+def test_caches_of_no_size():
+    """No positions is not the default number of them."""
+    for model in _models():
+        for args in ((1, 0), (1, -3), (0, 8), (1, 8, 0), (1, None, -1)):
+            with pytest.raises(ValueError, match="must be positive"):
+                model.new_cache(*args)
+        assert model.new_cache(1).max_len == model.new_cache(1, None).max_len == 24 and model.new_cache(1, 5).max_len == 5

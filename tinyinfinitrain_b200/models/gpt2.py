@@ -163,10 +163,10 @@ class GPT2(nn.Module):
     def new_cache(self, batch: int, max_len: Optional[int] = None, page_size: int = 64) -> nn.PagedKVCache:
         """An empty cache for ``batch`` sequences of up to ``max_len`` tokens (the model's context by default, and at most)."""
         cfg, w = self.config, self.lm_head.weight
-        max_len = max_len or cfg.block_size
+        max_len = cfg.block_size if max_len is None else max_len
         if max_len > cfg.block_size:
             raise ValueError(f"a cache of {max_len} positions exceeds block size {cfg.block_size}")
-        if (max_len + page_size - 1) // page_size * page_size > cfg.block_size:
+        if page_size > 0 and (max_len + page_size - 1) // page_size * page_size > cfg.block_size:
             page_size = math.gcd(page_size, cfg.block_size)     # pages end with the position table
         return nn.PagedKVCache(cfg.n_layer, batch, max_len, cfg.n_head, cfg.n_embd // cfg.n_head, page_size,
                                cfg.attention_window or None, cfg.attention_sinks, w.device, w.dtype)

@@ -130,7 +130,7 @@ class LLaMA3(nn.Module):
     def new_cache(self, batch: int, max_len: Optional[int] = None, page_size: int = 64) -> nn.PagedKVCache:
         """An empty cache for ``batch`` sequences of up to ``max_len`` tokens (the model's context by default)."""
         cfg, w = self.config, self.lm_head.weight
-        return nn.PagedKVCache(cfg.n_layer, batch, max_len or cfg.block_size, cfg.n_kv_head, cfg.head_dim, page_size,
+        return nn.PagedKVCache(cfg.n_layer, batch, cfg.block_size if max_len is None else max_len, cfg.n_kv_head, cfg.head_dim, page_size,
                                cfg.attention_window or None, cfg.attention_sinks, w.device, w.dtype)
 
     @torch.no_grad()
