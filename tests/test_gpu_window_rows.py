@@ -34,3 +34,18 @@ def test_a_row_that_sees_itself_only_is_its_value(dtype, hd, training):
                 assert ((dv.double() - do.double()).abs() <= 2.0 ** -17 * do.double().abs()).all()
     torch.cuda.synchronize()
     assert C.status_read(True) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_no_query_heads(dtype):
+    """Nobody sees the keys: their gradients are zeros, as on the CPU."""
+    for device in ("cpu", DEV):
+        q = torch.zeros(2, 50, 0, 64, device=device, dtype=dtype, requires_grad=True)
+        k, v = (torch.ones(2, 50, 2, 64, device=device, dtype=dtype, requires_grad=True) for _ in range(2))
+        if device == DEV:       # memory that the gradients may be given holds something
+            del_me = [torch.full((2, 50, 2, 64), 7.0, device=device, dtype=dtype) for _ in range(4)]
+            del del_me
+        o = ops.window_attention(q, k, v, 5)
+        assert o.shape == q.shape
+        for grad in torch.autograd.grad(o, (q, k, v), torch.zeros_like(o)):
+            assert not grad.any()

@@ -203,8 +203,11 @@ struct WindowAttention : public torch::autograd::Function<WindowAttention> {
     c10::cuda::CUDAGuard guard(q.device());
     const Shape s{q.size(0), q.size(1), q.size(2), k.size(2), q.size(3)};
     at::AutoDispatchBelowADInplaceOrView below;
-    Tensor dq = at::empty({s.B, s.T, s.Hq, s.hd}, q.options()), dk = at::empty({s.B, s.T, s.Hkv, s.hd}, q.options()),
-           dv = at::empty({s.B, s.T, s.Hkv, s.hd}, q.options());
+    // no query heads: no kernel runs, and no query sees a key
+    const auto gradient = [&](int64_t heads) {
+      return s.Hq > 0 ? at::empty({s.B, s.T, heads, s.hd}, q.options()) : at::zeros({s.B, s.T, heads, s.hd}, q.options());
+    };
+    Tensor dq = gradient(s.Hq), dk = gradient(s.Hkv), dv = gradient(s.Hkv);
     window_backward(s, grads[0], rows_of(q), rows_of(k), rows_of(v), saved[3], saved[4], saved[5], rows_of(dq), rows_of(dk), rows_of(dv),
                     ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt(), ctx->saved_data["scale"].toDouble());
     grads = first_order_only({dq, dk, dv});
