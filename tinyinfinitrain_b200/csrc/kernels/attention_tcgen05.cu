@@ -126,7 +126,7 @@ struct FwdCfg {
 // heads: 48.8 -> 33.4 us; 4 x 2048: 138 -> 117 us; hd 128, 1 x 4096, 32 / 8 heads: 174 -> 153 us (897 TFLOP/s).
 //
 // WIN: a window and sinks.  The CTA visits the key blocks of the sinks and those from its first query's window to its own; a
-// block on either border of what the rows see is masked by a 128-bit mask per row, built from the row's two ranges of keys.
+// block on either border of what the rows see is masked by 64 bits per row, built from the row's two ranges of keys.
 // Up to kSinkCols sinks that lie before the window are a block of kSinkCols keys.  The few blocks of such a CTA do not hide its
 // set-up and its chain of dependent steps (S, maximum, exponentials, P, P V), so kCtas CTAs share the SM, with 64 keys a step
 // and P in tensor memory, as the A operand of P V: 48 or 96 KB of shared memory and 128 or 256 columns to a CTA.  At hd 64 P
@@ -136,8 +136,8 @@ struct FwdCfg {
 // being the roundings of dS and of dQ).  LO: a backward pass may follow, and what the rounding of o left is kept for its delta.
 // Measured (B200): hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: one CTA an SM 254 us, two with 128 keys a step, P over S
 // and S(j+1) issued behind P(j) V(j) 182 us, with the steps as they are 165 us (790 TFLOP/s of what the rows see), with LO 180,
-// with the second product 197 us; hd 64, 1 x 1999, 32 / 8 heads, window 512: 29 us before, 26 us, 28 with the look
-// for rows that are not finite, 30 with the second product.  Without that product a step of 64 keys takes 1660 cycles (hd 128) and 2140 (hd 64,
+// with the second product 197 us (tensor pipe 58 % of the cycles); a launch by itself on cold caches, hd 64, 1 x 1999, 32 / 8 heads, window 512: 29 us before, 26 us, 28 with the look
+// for rows that are not finite, 30 with the second product (24.9 among others like it).  Without that product a step of 64 keys takes 1660 cycles (hd 128) and 2140 (hd 64,
 // three CTAs), 920 and 1060 of them for the exponentials; a quarter of those on the multiply-add pipe changed nothing.  Set-up,
 // first loads and output take another 8000 and 5500 cycles of a CTA.
 template <int HD, bool WIN, bool LO>
@@ -615,7 +615,11 @@ __device__ __noinline__ void key_tile_again(const AttnArgs& p, const WinRows& ro
 // all later ones, which would make its CTA the last by far: its query blocks are split over sink_parts CTAs, which leave
 // fp32 sums of the sinks' rows that attn_window_finish_kernel adds in order.
 // Measured: hd 128, 1 x 8192, 32 / 8 heads, window 1024, sinks 4: 400 us (396 without the look for what is not finite),
-// 1070 TFLOP/s of the tiles it visits, an eighth of them masked and a tenth for the sinks; the same parts as above bound it.
+// 1070 TFLOP/s of the tiles it visits, an eighth of them masked and a tenth for the sinks; the same parts as above bound it
+// (tensor pipe 50 % of the cycles).
+// P of dV and dS are rounded to bf16, as without a window: o and the gradients together are off by 0.235 %, where the roundings
+// of the results alone give 0.165 %.  Products for what those roundings leave, as in the forward pass, would be three more of
+// five and need columns for them: tensor memory is full at both head sizes.
 template <int HD, bool WIN>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -1261,7 +1265,7 @@ static int attn_bwd_launch(const TitbAttnDesc* d, cudaStream_t st, int window = 
   if (WIN) {
     const SinkSplit split = sink_split(*d, window, sinks);
     a.window = window; a.sinks = sinks;
-      a.sink_blocks = split.blocks; a.sink_step = split.step; a.sink_parts = split.parts; a.sink_part = sink_part;
+    a.sink_blocks = split.blocks; a.sink_step = split.step; a.sink_parts = split.parts; a.sink_part = sink_part;
     jobs += split.blocks * (split.parts - 1);
   }
   dim3 grid(static_cast<unsigned>(d->Hkv) * d->B, jobs);

@@ -73,9 +73,12 @@ __device__ __forceinline__ void rope_sincos(int pos, double turns, float& sn, fl
 
 // A CTA takes up to kAppendTokens tokens and `per` of their heads.  The sines and cosines of its tokens go to shared memory once
 // (their 64-bit reduction costs more than a head's bytes), then a thread moves V neighbouring elements of both halves of a
-// head at a time, two of them in flight.  Bound by memory.  Before, every thread took the angles of eight heads of its own:
-// 112 registers, 13 warps on an SM, 31 us for 2 x 1999 tokens, 32 / 8 heads of 128 (106 MB); now 23.5 us (4.5 TB/s).  Asking
-// for the rows ahead of the angles (prefetch to the L2) did not help.  64 single tokens: 5 us, of which the launch, positions,
+// head at a time, two of them in flight.  Before, every thread took the angles of eight heads of its own:
+// 112 registers, 13 warps on an SM, 31 us for 2 x 1999 tokens, 32 / 8 heads of 128 (106 MB); now 23.5 us (4.5 TB/s).  Bound by
+// the latency of the reads: of 43000 cycles an SM works 33000, the others being the launch, the first reads and the end of the
+// one wave; there 28 warps (63 registers a thread) wait for their reads two fifths of the time and issue in half of the cycles.
+// Neither memory (DRAM 33 %, L2 26 %: what is written stays in the L2) nor issue is full.  Asking for the rows ahead of the
+// angles (prefetch to the L2) did not help.  64 single tokens: 5 us, of which the launch, positions,
 // page table and angles one behind the other are most.
 constexpr int kAppendTokens = 8, kAppendThreads = 256, kAppendCtas = 4;   // the last: CTAs of an SM
 
@@ -349,8 +352,8 @@ __device__ __forceinline__ void finish_item(const PagedArgs& p, int b, int item,
 
 // One CTA per CTA of the main kernel: the item that began in that one's run and went on behind it.  A warp takes a head's maxima
 // and denominators, a lane a part's, and leaves the parts' weights in shared memory; then a thread adds four elements of the
-// parts, eight loads in flight (a sequence alone on the card has some fifty parts to a head: with two dependent passes over them
-// the join took 14 of 99 us).
+// parts, eight loads in flight (a sequence alone on the card, 8 items on 296 CTAs, has 37 parts to a head: the join and its launch
+// take 9 of 95 us, and 14 of 99 with two dependent passes over the parts).
 template <typename T, int HG>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs p) {
   extern __shared__ float weight[];   // [HG][parts]

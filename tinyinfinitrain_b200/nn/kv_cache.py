@@ -89,6 +89,9 @@ class PagedKVCache:
                                window=self.window, sinks=self.sinks, return_k=T > 1)
         if T == 1:
             return ops.paged_attention(out[:, 0], k, v, self.page_table, self._ends, self.window, self.sinks)[:, None]
+        # Without a window ops.causal_attention gives the same sums: with heads of 64 it takes 35 us where this takes 54 (a prompt
+        # of 1999, 32 / 8 heads; 374 and 463 us at 8192), with heads of 128 50 and 46 (580 each; 9.0 and 10 ms at 32768).  It
+        # rounds the probabilities of bf16 models and lets a NaN reach earlier rows; here a prompt is as exact as the tokens behind it.
         values = qkv.unflatten(-1, (n_head + 2 * n_kv, hd))[:, :, n_head + n_kv:]
         return ops.window_attention(*out, values, self.window, self.sinks)
 
