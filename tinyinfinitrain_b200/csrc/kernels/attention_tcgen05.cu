@@ -827,9 +827,14 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         if (!ptx::mbar_wait(ds_full, it & 1, abort_flag)) break;
         if (!Cfg::kAlias && it > 0 && !ptx::mbar_wait(dq_free, (it - 1) & 1, abort_flag)) break;
         ptx::tc_fence_after_sync();
+        // reduction over the 128 keys; queries whose windows lie behind the block see its sinks only, and what the other keys
+        // hold (0 times NaN) stays out of their dQ
+        const int key_steps = sink_cta && (ib + it % nq - jb) * kBlk - (kBlk - 1) >= p.window ? (min(p.sinks - jb * kBlk, kBlk) + 15) / 16 : kBlk / 16;
 #pragma unroll
-        for (int k = 0; k < kBlk / 16; ++k)  // reduction over the 128 keys
+        for (int k = 0; k < kBlk / 16; ++k) {
+          if (WIN && k >= key_steps) break;
           ptx::mma_f16_ss(tmem_base + Cfg::kColDQ, desc_add(ds_mn, k * 2048), desc_add(k_mn, k * 2048), idesc_q, k > 0);
+        }
         ptx::tc_commit(dq_full);
 #pragma unroll
         for (int k = 0; k < kBlk / 16; ++k)  // reduction over the 128 queries
