@@ -569,8 +569,8 @@ struct BwdCfg {
 // Rows of key block jb that are not finite (`found`: bit 0 dV, bit 1 dK; a word for either half of a row), over query blocks
 // ib .. ib + nq - 1.  part: of a block with sinks, else -1.  All warps of the CTA, eight rows at a time.
 template <int HD>
-__device__ __noinline__ void key_tile_again(const AttnArgs& p, const WinRows& rows, const uint32_t* found, int b, int hk, int jb, int part,
-                                            int ib, int nq) {
+__device__ __noinline__ void key_tile_again(const AttnArgs& p, const WinRows& rows, const uint32_t* found, int b, int hk,
+                                            int jb, int part, int ib, int nq) {
   constexpr int kFew = 8;
   const int lane = threadIdx.x & 31, i0 = ib * kBlk, i1 = (ib + nq) * kBlk;
 #pragma unroll 1
@@ -578,17 +578,19 @@ __device__ __noinline__ void key_tile_again(const AttnArgs& p, const WinRows& ro
     const int which = x / (kBlk / kFew), row0 = x % (kBlk / kFew) * kFew, j0 = jb * kBlk + row0;
     const uint32_t mine = lane < kFew ? found[row0 + lane] | found[kBlk + row0 + lane] : 0u;
     const uint32_t bad = __ballot_sync(0xffffffffu, (mine >> which & 1u) && j0 + lane < p.T);
-    const uint32_t in_part = part >= 0 && p.sink_parts > 1 ? bad & bit_range(0, p.sinks - j0) : 0u, whole = part <= 0 ? bad & ~in_part : 0u;
+    const uint32_t in_part = part >= 0 && p.sink_parts > 1 ? bad & bit_range(0, p.sinks - j0) : 0u;
+    const uint32_t whole = part <= 0 ? bad & ~in_part : 0u;
     if (in_part) {
-      float* sum = p.sink_part + ((((static_cast<long long>(part) * p.B + b) * p.sink_blocks + jb) * p.Hkv + hk) * 2 + 1 - which) * (kBlk * HD) +
-                   row0 * HD;
+      const long long block = ((static_cast<long long>(part) * p.B + b) * p.sink_blocks + jb) * p.Hkv + hk;
+      float* sum = p.sink_part + (block * 2 + 1 - which) * (kBlk * HD) + row0 * HD;
       if (which == 0) key_rows_again<bf16, float, true>(rows, b, hk, j0, in_part, i0, i1, sum, HD);
       else key_rows_again<bf16, float, false>(rows, b, hk, j0, in_part, i0, i1, sum, HD);
     }
     if (whole) {
       const long long bt = static_cast<long long>(b) * p.T + j0;
-      if (which == 0) key_rows_again<bf16, bf16, true>(rows, b, hk, j0, whole, i0, i1, p.dv + bt * p.dv_stride_t + hk * HD, p.dv_stride_t);
-      else key_rows_again<bf16, bf16, false>(rows, b, hk, j0, whole, i0, i1, p.dk + bt * p.dk_stride_t + hk * HD, p.dk_stride_t);
+      bf16 *dv = p.dv + bt * p.dv_stride_t + hk * HD, *dk = p.dk + bt * p.dk_stride_t + hk * HD;
+      if (which == 0) key_rows_again<bf16, bf16, true>(rows, b, hk, j0, whole, i0, i1, dv, p.dv_stride_t);
+      else key_rows_again<bf16, bf16, false>(rows, b, hk, j0, whole, i0, i1, dk, p.dk_stride_t);
     }
   }
 }
@@ -829,7 +831,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         ptx::tc_fence_after_sync();
         // reduction over the 128 keys; queries whose windows lie behind the block see its sinks only, and what the other keys
         // hold (0 times NaN) stays out of their dQ
-        const int key_steps = sink_cta && (ib + it % nq - jb) * kBlk - (kBlk - 1) >= p.window ? (min(p.sinks - jb * kBlk, kBlk) + 15) / 16 : kBlk / 16;
+        const bool behind = sink_cta && (ib + it % nq - jb) * kBlk - (kBlk - 1) >= p.window;
+        const int key_steps = behind ? (min(p.sinks - jb * kBlk, kBlk) + 15) / 16 : kBlk / 16;
 #pragma unroll
         for (int k = 0; k < kBlk / 16; ++k) {
           if (WIN && k >= key_steps) break;
@@ -1113,7 +1116,8 @@ __global__ void attn_dq_convert_kernel(const float* __restrict__ acc, bf16* __re
 // What of a warp's dq (below) is not finite, over visible pairs only.  It starts over, since a call within the loop below took
 // registers from it.  HD / 8 neighbouring lanes hold a row, and a row lies in one warp: n_sink is a multiple of 32.
 template <int HD>
-__device__ __noinline__ void dq_again(const WinRows& rows, const float* acc, long long n_sink, long long n, bf16* dq, long long dq_stride_t) {
+__device__ __noinline__ void dq_again(const WinRows& rows, const float* acc, long long n_sink, long long n, bf16* dq,
+                                      long long dq_stride_t) {
   constexpr int L = HD / 8;
   const int wv = rows.Hq * L, lane = threadIdx.x & 31;
   for (long long i0 = blockIdx.x * (long long)blockDim.x + threadIdx.x - lane; i0 < n; i0 += (long long)gridDim.x * blockDim.x) {

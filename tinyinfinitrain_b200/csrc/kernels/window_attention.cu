@@ -14,7 +14,7 @@
 // with half as many distinct words a read changed nothing), and by tiles that are half masked where the window is short.
 // Measured (B200), 2 x 512 tokens, 12 heads of 64, window 128, sinks 2, forward and backward of one pass: 64 x 64 tiles 230 us, 32
 // rows a CTA 156, packed products 130, 32 x 32 tiles in two buffers 114 us, with the look for what is not
-// finite 117 (32 + 43 + 47 us and the join of 4).
+// finite 115 (27 + 37 + 42 us and the join of 3).
 #include <cuda_runtime.h>
 
 #include "api.h"
@@ -307,7 +307,8 @@ __global__ void __launch_bounds__(kWinThreads) window_fwd_kernel(const WinArgs p
     __syncwarp();   // rows and log-sum-exp are read again by other lanes
     const int i0 = q0 + static_cast<int>(threadIdx.x >> 5) * 8;
     const long long at = (row0 + i0) * p.o_st + h * p.hd;
-    query_rows_again<T, false>(rows, b, h, i0, bad, static_cast<T*>(p.o) + at, p.o_st, sizeof(T) == 2 && p.o_lo ? p.o_lo + at : nullptr);
+    query_rows_again<T, false>(rows, b, h, i0, bad, static_cast<T*>(p.o) + at, p.o_st,
+                               sizeof(T) == 2 && p.o_lo ? p.o_lo + at : nullptr);
   }
 }
 
@@ -476,19 +477,24 @@ __global__ void __launch_bounds__(kWinThreads) window_dkv_kernel(const WinArgs p
     store_rows<T, HD>(static_cast<T*>(p.dv) + row0 * p.dv_st + hk * p.hd, p.dv_st, k0, p.T, p.hd, dv, ty, tx);
   }
   const bool parts = sink_cta && p.sink_parts > 1;
-  float* sum = p.sink_part + (((static_cast<long long>(part) * p.B + b) * p.sink_tiles + tile) * p.Hkv + hk) * 2 * kWinRows * p.hd;
+  const long long block = ((static_cast<long long>(part) * p.B + b) * p.sink_tiles + tile) * p.Hkv + hk;
+  float* sum = p.sink_part + block * 2 * kWinRows * p.hd;
   if (parts) {
     store_rows<float, HD>(sum, p.hd, 0, p.sinks - k0, p.hd, dk, ty, tx);
     store_rows<float, HD>(sum + kWinRows * p.hd, p.hd, 0, p.sinks - k0, p.hd, dv, ty, tx);
   }
-  const uint32_t bad_k = bad_rows<HD>(dk, p.hd, p.T, k0 + ty * 4, tx), bad_v = bad_rows<HD>(dv, p.hd, p.T, k0 + ty * 4, tx);
+  const uint32_t bad_k = bad_rows<HD>(dk, p.hd, p.T, k0 + ty * 4, tx);
+  const uint32_t bad_v = bad_rows<HD>(dv, p.hd, p.T, k0 + ty * 4, tx);
   if (bad_k | bad_v) {
     __syncwarp();   // the rows are read again by other lanes
-    const int r0 = static_cast<int>(threadIdx.x >> 5) * 8, j0 = k0 + r0, i0 = first * kWinStep, i1 = (first + n_steps) * kWinStep;
+    const int r0 = static_cast<int>(threadIdx.x >> 5) * 8, j0 = k0 + r0;
+    const int i0 = first * kWinStep, i1 = (first + n_steps) * kWinStep;
     const uint32_t in_part = parts ? bit_range(0, p.sinks - j0) : 0u, whole = part == 0 ? ~in_part : 0u;
-    T *dk0 = static_cast<T*>(p.dk) + (row0 + j0) * p.dk_st + hk * p.hd, *dv0 = static_cast<T*>(p.dv) + (row0 + j0) * p.dv_st + hk * p.hd;
-    if (bad_k & in_part) key_rows_again<T, float, false>(rows, b, hk, j0, bad_k & in_part, i0, i1, sum + r0 * p.hd, p.hd);
-    if (bad_v & in_part) key_rows_again<T, float, true>(rows, b, hk, j0, bad_v & in_part, i0, i1, sum + (kWinRows + r0) * p.hd, p.hd);
+    float *sum_k = sum + r0 * p.hd, *sum_v = sum + (kWinRows + r0) * p.hd;
+    T* dk0 = static_cast<T*>(p.dk) + (row0 + j0) * p.dk_st + hk * p.hd;
+    T* dv0 = static_cast<T*>(p.dv) + (row0 + j0) * p.dv_st + hk * p.hd;
+    if (bad_k & in_part) key_rows_again<T, float, false>(rows, b, hk, j0, bad_k & in_part, i0, i1, sum_k, p.hd);
+    if (bad_v & in_part) key_rows_again<T, float, true>(rows, b, hk, j0, bad_v & in_part, i0, i1, sum_v, p.hd);
     if (bad_k & whole) key_rows_again<T, T, false>(rows, b, hk, j0, bad_k & whole, i0, i1, dk0, p.dk_st);
     if (bad_v & whole) key_rows_again<T, T, true>(rows, b, hk, j0, bad_v & whole, i0, i1, dv0, p.dv_st);
   }

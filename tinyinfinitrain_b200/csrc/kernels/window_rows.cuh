@@ -1,23 +1,25 @@
 // Window attention, the rows that came out not finite, over their visible pairs only.
 //
-// Inside a tile a pair that is masked has a probability of zero, but its values still take part in the products, and zero times
-// NaN or infinity is NaN.  So the kernels look at what they store, and a warp takes rows that are not finite again here, where
-// masked pairs do not appear.
+// Inside a tile a pair that is masked has a probability of zero, but its values still take part in the products, and
+// zero times NaN or infinity is NaN.  So the kernels look at what they store, and a warp takes rows that are not finite
+// again here, where masked pairs do not appear.
 //
 // Every output is a sum over pairs of a weight f (one number a pair) times a vector x that all rows of a warp share:
 //   O  = sum_j P_ij V_j      dQ = sum_j dS_ij K_j      dV = sum_i P_ij dO_i      dK = sum_i dS_ij Q_i
 // What is not finite by right is told from the few terms that are not, without the products of the others:
 //   - a log-sum-exp that is not finite means undefined probabilities: the row, and the keys that it sees, are NaN;
-//   - a finite score has a positive weight, so an infinity of V or dO is an infinity of the sum (NaN where both signs meet, or a
-//     score of -inf has weight zero), and a K that is not finite beside a finite log-sum-exp has a score of -inf: zero times K;
+//   - a finite score has a positive weight, so an infinity of V or dO is an infinity of the sum (NaN where both signs
+//     meet, or a score of -inf has weight zero), and a K that is not finite beside a finite log-sum-exp has a score of
+//     -inf: zero times K;
 //   - an infinite delta makes dS infinite or NaN for the whole row.
-// Finding them takes one pass over the vectors for 32 rows, which ends when nothing can be added.  Only columns that are finite
-// by right are summed again: those that a masked neighbour within the tiles' borders has spoilt, and sums that overflow on
-// their way; two neighbours at a time, a lane holding columns, so that vectors are read whole and once for both.
-// Measured (B200), 1 x 1024, 8 / 2 heads of 64 and 128, window 256 or none, forward and backward: 0.13 ms when all is finite, the
-// same with all gradients or values NaN, 1.2 to 5 ms with a single infinity in one of the operands.  As a thread's work, 16 columns
-// at a time and without an end but at an undefined weight, 30 to 110 ms.  Asking for the next vectors under the sums of those at
-// hand was slower: the registers are those that the tile kernels leave.
+// Finding them takes one pass over the vectors for 32 rows, which ends when nothing can be added.  Only columns that
+// are finite by right are summed again: those that a masked neighbour within the tiles' borders has spoilt, and sums
+// that overflow on their way; two neighbours at a time, a lane holding columns, so that vectors are read whole and once for
+// both.
+// Measured (B200), 1 x 1024, 8 / 2 heads of 64 and 128, window 256 or none, forward and backward: 0.13 ms when all is
+// finite, 0.2 ms with all gradients or values NaN, 0.2 to 5 ms with single infinities or NaN rows.  As a thread's work,
+// 16 columns at a time and without an end but at an undefined weight, 30 to 110 ms.  Asking for the next vectors under
+// the sums of those at hand was slower: the registers are those that the tile kernels leave.
 #pragma once
 #include "api.h"
 #include "common.cuh"
@@ -44,8 +46,8 @@ struct WinRows {
 };
 
 inline WinRows window_rows(const TitbAttnDesc& d, int window, int sinks) {
-  return {d.q, d.k, d.v, d.d_o, d.q_stride_t, d.k_stride_t, d.v_stride_t, d.do_stride_t, d.lse, d.delta, d.T, d.Hq, d.Hkv, d.hd,
-          window, sinks, d.scale};
+  return {d.q,   d.k,     d.v, d.d_o, d.q_stride_t, d.k_stride_t, d.v_stride_t, d.do_stride_t,
+          d.lse, d.delta, d.T, d.Hq,  d.Hkv,        d.hd,         window,       sinks,         d.scale};
 }
 
 // 0 while everything that was put in is finite, else NaN.
@@ -76,11 +78,12 @@ __device__ inline float row_dot(const T* a, const T* b, int n) {
   return s;
 }
 
-// Columns of a row of up to 128 elements, two neighbours and two 64 further on to a lane; a set of columns is a bit per lane in
-// four words.
+// Columns of a row of up to 128 elements, two neighbours and two 64 further on to a lane; a set of columns is a bit per
+// lane in four words.
 constexpr int kRowWords = 4;
 __device__ __forceinline__ int column_of(int e, int lane) { return (e >> 1) * 64 + lane * 2 + (e & 1); }
-__device__ __forceinline__ uint32_t columns_of(int e, int hd) { return bit_range(0, (hd - (e >> 1) * 64) / 2); }   // of a whole row
+// word e of the set of a whole row's
+__device__ __forceinline__ uint32_t columns_of(int e, int hd) { return bit_range(0, (hd - (e >> 1) * 64) / 2); }
 template <typename T>
 struct RowPart {
   Pack<T, 2> half[2];
@@ -155,11 +158,12 @@ struct VectorKinds {
   }
 };
 
-// Row r of the warp: x becomes what its columns are by right where that is not finite, else what the kernel stored.  Returns the
-// columns of this lane (a bit each) that have to be summed again: those stored that should be finite and are not, or `all` others.
+// Row r of the warp: x becomes what its columns are by right where that is not finite, else what the kernel stored.
+// Returns the columns of this lane (a bit each) that have to be summed again: those stored that should be finite and
+// are not, or `all` others.
 template <typename Out>
-__device__ __forceinline__ uint32_t row_verdict(const RowKinds& kinds, int r, bool all, const Out* stored, int hd, int lane,
-                                                float (&x)[kRowWords]) {
+__device__ __forceinline__ uint32_t row_verdict(const RowKinds& kinds, int r, bool all, const Out* stored, int hd,
+                                                int lane, float (&x)[kRowWords]) {
   uint32_t want = 0u;
 #pragma unroll
   for (int e = 0; e < kRowWords; ++e) {
@@ -175,8 +179,8 @@ __device__ __forceinline__ uint32_t row_verdict(const RowKinds& kinds, int r, bo
   return want;
 }
 
-// Every value's sum over the warp, in all lanes.  With each exchange a lane keeps half of the values, so that N of them take
-// N - 1 + log2(32 / N) of them and N to hand the sums out.
+// Every value's sum over the warp, in all lanes.  With each exchange a lane keeps half of the values, so that N of them
+// take N - 1 + log2(32 / N) exchanges, and N to hand the sums out.
 template <int N>
 __device__ __forceinline__ void sum_lanes(float (&a)[N], int lane) {
   int d = 16;
@@ -213,18 +217,19 @@ struct RowsAgain {
   }
 };
 
-// Some vectors and what belongs to them: x is what the rows' own vectors are scored with, y the other one, which takes part in
-// dP (DS) or is the one that is added (else).
+// Some vectors and what belongs to them: x is what the rows' own vectors are scored with, y the other one, which takes
+// part in dP (DS) or is the one that is added (else).
 template <typename T, bool DS>
 struct VectorsAgain {
   RowPart<T> x[kPairs], y[kPairs];
   float lse[kPairs], delta[kPairs];
 };
 
-// The terms of the first n of them; see(k, u): row k sees vector u.  lse and delta are the vectors' (KEYS) or the rows' own.
+// The terms of the first n of them; see(k, u): row k sees vector u.  lse and delta are the vectors' (KEYS) or the rows'
+// own.
 template <typename T, bool DS, bool KEYS, int A, typename S>
-__device__ __forceinline__ void add_pairs(RowsAgain<A>& r, const VectorsAgain<T, DS>& v, const float (&lse)[A], const float (&delta)[A],
-                                          float scale, int n, int lane, S see) {
+__device__ __forceinline__ void add_pairs(RowsAgain<A>& r, const VectorsAgain<T, DS>& v, const float (&lse)[A],
+                                          const float (&delta)[A], float scale, int n, int lane, S see) {
   constexpr int N = A * kPairs;
   float sums[DS ? 2 * N : N];
 #pragma unroll
@@ -251,11 +256,12 @@ __device__ __forceinline__ void add_pairs(RowsAgain<A>& r, const VectorsAgain<T,
   }
 }
 
-// Rows i0 + r of O (or dQ) of head h, for the bits r of `bad`.  out: row i0, `stride` elements between tokens; lo (may be null):
-// what the rounding of O left, laid out the same.  A: rows that are summed at a time.  A whole warp, which sees the rows, the
-// log-sum-exp and delta as stored.
+// Rows i0 + r of O (or dQ) of head h, for the bits r of `bad`.  out: row i0, `stride` elements between tokens; lo (may
+// be null): what the rounding of O left, laid out the same.  A: rows that are summed at a time.  A whole warp, which
+// sees the rows, the log-sum-exp and delta as stored.
 template <typename T, bool DQ, int A = 2>
-__device__ __noinline__ void query_rows_again(const WinRows& w, int b, int h, int i0, uint32_t bad, T* out, long long stride, bf16* lo) {
+__device__ __noinline__ void query_rows_again(const WinRows& w, int b, int h, int i0, uint32_t bad, T* out,
+                                              long long stride, bf16* lo) {
   const int lane = threadIdx.x & 31, hk = h / (w.Hq / w.Hkv), i = i0 + lane;
   const bool mine = bad >> lane & 1u;
   RowKinds kinds;
@@ -298,7 +304,10 @@ __device__ __noinline__ void query_rows_again(const WinRows& w, int b, int h, in
         if (!vec.take(x)) continue;
         if (!done && w.visible(i, j) && vec.news_to(kinds)) {
           bool zero = DQ;
-          if (!DQ) zero = row_dot(w.row<T>(w.q, w.q_st, b, i, h), w.row<T>(w.k, w.k_st, b, j, hk), w.hd) * w.scale == -INFINITY;
+          if (!DQ) {
+            const T *q = w.row<T>(w.q, w.q_st, b, i, h), *k = w.row<T>(w.k, w.k_st, b, j, hk);
+            zero = row_dot(q, k, w.hd) * w.scale == -INFINITY;
+          }
           vec.add_to(kinds, zero);
           done = kinds.settled(w.hd);
         }
@@ -362,11 +371,11 @@ __device__ __noinline__ void query_rows_again(const WinRows& w, int b, int h, in
   }
 }
 
-// Rows j0 + r of dV (VALUE) or dK of kv head hk, for the bits r of `bad`: their sums over queries [ia, ib).  out: row j0, `stride`
-// elements between rows.  A whole warp, as above.
+// Rows j0 + r of dV (VALUE) or dK of kv head hk, for the bits r of `bad`: their sums over queries [ia, ib).  out: row
+// j0, `stride` elements between rows.  A whole warp, as above.
 template <typename T, typename Out, bool VALUE>
-__device__ __noinline__ void key_rows_again(const WinRows& w, int b, int hk, int j0, uint32_t bad, int ia, int ib, Out* out,
-                                            long long stride) {
+__device__ __noinline__ void key_rows_again(const WinRows& w, int b, int hk, int j0, uint32_t bad, int ia, int ib,
+                                            Out* out, long long stride) {
   constexpr int A = 2;
   const int lane = threadIdx.x & 31, G = w.Hq / w.Hkv, j = j0 + lane;
   const bool mine = bad >> lane & 1u;
@@ -387,7 +396,8 @@ __device__ __noinline__ void key_rows_again(const WinRows& w, int b, int hk, int
 #pragma unroll 1
     for (int i32 = i_lo; i32 < i_hi && !settled; i32 += 32) {
       const bool real = i32 + lane < i_hi;
-      const float lse = real ? w.lse[w.stat(b, h, i32 + lane)] : 0.f, delta = !VALUE && real ? w.delta[w.stat(b, h, i32 + lane)] : 0.f;
+      const float lse = real ? w.lse[w.stat(b, h, i32 + lane)] : 0.f;
+      const float delta = !VALUE && real ? w.delta[w.stat(b, h, i32 + lane)] : 0.f;
       const bool undefined = !is_finite(lse) || delta != delta;
       const uint32_t no = __ballot_sync(0xffffffffu, undefined);
       if (mine && (no & bit_range(j - i32, last + 1 - i32))) {
