@@ -90,13 +90,19 @@ def _spoil(case, q, k, v, do):
         k[:, z, -1] = NAN
     elif case == "an infinite query":
         q[:, z, 0, 4] = INF
+    elif case == "infinities that meet a weight of zero":
+        # by sign of their query, rows see the second infinity of V, and keys that of dO, with a score of -inf
+        v[:, a, 0, 3] = v[:, a + 9, 0, 3] = INF
+        k[:, a + 9, 0, 1] = INF
+        do[:, a + 20, :, 5] = do[:, a + 21, :, 5] = do[:, a + 22, :, 5] = -INF
     else:
         q[:, a, 0, 0], v[:, a + 3, -1, 1], do[:, z, :, 6], k[:, z + 5, 0, 2] = NAN, -INF, INF, INF
 
 
 CASES = ["one infinite value", "both infinities in a column", "an undefined value", "all values undefined", "all values infinite",
          "one infinite gradient", "an undefined gradient", "all gradients undefined", "a column of infinite gradients",
-         "an infinite key", "an undefined key", "an infinite query", "some of each"]
+         "an infinite key", "an undefined key", "an infinite query", "infinities that meet a weight of zero",
+         "some of each"]
 
 
 def _run(q, k, v, do, window, sinks):

@@ -302,7 +302,16 @@ __device__ __noinline__ void query_rows_again(const WinRows& w, int b, int h, in
         columns(j, x);
         VectorKinds vec;
         if (!vec.take(x)) continue;
-        if (!done && w.visible(i, j) && vec.news_to(kinds)) {
+        // a weight of zero, which makes an infinity NaN that is known already, takes a K that is not finite
+        bool odd = false;
+        if (!DQ) {
+          probe = 0.f;
+          row_columns(w.row<T>(w.k, w.k_st, b, j, hk), w.hd, lane, x);
+#pragma unroll
+          for (int e = 0; e < kRowWords; ++e) probe_finite(probe, x[e]);
+          odd = __any_sync(0xffffffffu, probe != 0.f);
+        }
+        if (!done && w.visible(i, j) && (odd || vec.news_to(kinds))) {
           bool zero = DQ;
           if (!DQ) {
             const T *q = w.row<T>(w.q, w.q_st, b, i, h), *k = w.row<T>(w.k, w.k_st, b, j, hk);
@@ -390,6 +399,9 @@ __device__ __noinline__ void key_rows_again(const WinRows& w, int b, int hk, int
   const auto score = [&](int i, int h) {
     return row_dot(w.row<T>(w.q, w.q_st, b, i, h), w.row<T>(w.k, w.k_st, b, j, hk), w.hd) * w.scale;
   };
+  // a K whose scores may be -inf: a weight of zero makes NaN of an infinity that is known already
+  const T* own = w.row<T>(w.k, w.k_st, b, mine ? j : j0 + __ffs(bad) - 1, hk);
+  const bool odd = VALUE && !is_finite(row_dot(own, own, w.hd));
   bool settled = false;
 #pragma unroll 1
   for (int h = hk * G; h < hk * G + G && !settled; ++h) {
@@ -422,7 +434,7 @@ __device__ __noinline__ void key_rows_again(const WinRows& w, int b, int hk, int
             columns(i, h, x);
             VectorKinds vec;
             if (!vec.take(x)) continue;
-            if (!done && i >= j && i <= last && vec.news_to(kinds)) {
+            if (!done && i >= j && i <= last && (odd || vec.news_to(kinds))) {
               vec.add_to(kinds, score(i, h) == -INFINITY);
               done = kinds.settled(w.hd);
             }
